@@ -60,7 +60,9 @@ def build_kernels(force: bool = False) -> Path:
             CSRC / "mtq_awq_scale.hip", CSRC / "mtq_attention.hip", CSRC / "mtq_cpu.cpp"]
     hdrs = [CSRC / "mtq_device.hpp", INC / "mtq_amd.h"]
     OBJ.mkdir(parents=True, exist_ok=True)
-    flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Werror=misleading-indentation", "-Wno-unused-function", f"-I{INC}"]
+    flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Werror=misleading-indentation", "-Wno-unused-function", f"-I{INC}",
+             # no packed fp32 instructions: some of their forms have given wrong results on this card now and then
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     objs, jobs = [], []
     for src in srcs:
         obj = OBJ / (src.name + ".o")
