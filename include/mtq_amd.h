@@ -461,6 +461,86 @@ int mtq_attention_fwd(const void *q, const void *k, const void *v, void *o,
                       const int64_t *strides, int is_causal, double softmax_scale,
                       int p_qdq_mode, double p_qdq_scale, int dtype, hipStream_t stream);
 
+/* ---- microscaled operands and their products ------------------------------------------------
+ * The forms that quantised rows are handed over in (no reference counterpart as native code: the
+ * reference multiplies packed weights through Triton / TensorRT backends, backends/nvfp4_gemm.py,
+ * fp8_per_tensor_gemm.py):
+ *   MTQ_MXFP4       q[row][K / 2] E2M1 codes, even column low; scale[row][K / 32] E8M0 bytes
+ *   MTQ_MXFP8       q[row][K] E4M3; scale[row][K / 32] E8M0 bytes
+ *   MTQ_FP8_TENSOR  q[row][K] E4M3; scale[1] fp32 factor (value = q * factor)
+ *   MTQ_FP8_TOKEN   q[row][K] E4M3; scale[row] fp32 factors
+ * Values: the MX kinds as mtq_fused_amax_convert (E8M0 scales, block 32), FP8_TENSOR as
+ * mtq_fake_e4m3fy with the fp32 amax[0]; FP8_TOKEN: factor = max|x| / 448 (1 for a row of zeros). */
+enum mtq_row_kind { MTQ_MXFP4 = 0, MTQ_MXFP8 = 1, MTQ_FP8_TENSOR = 2, MTQ_FP8_TOKEN = 3 };
+
+/* Rows x[rows][cols] (row stride in elements; bf16 / f16 / f32) to q and scale; cols % 32 == 0 for
+ * the MX kinds; q 8-byte aligned. */
+int mtq_mx_quantize(const void *x, int64_t row_stride, int64_t rows, int64_t cols, int dtype,
+                    int kind, const float *amax, uint8_t *q, void *scale, hipStream_t stream);
+
+/* h = x + residual (rounded to dtype; h may be the residual itself), y = h * rsqrt(mean(h^2) + eps)
+ * * weight in fp32, quantised to q / scale as above without rounding y in between.  residual NULL:
+ * h = x and no h is written.  weight: dtype or fp32.  cols <= 65536. */
+int mtq_rms_norm_quantize(const void *x, int64_t x_stride, const void *residual, int64_t r_stride,
+                          const void *weight, int weight_dtype, double eps, void *h, uint8_t *q,
+                          void *scale, const float *amax, int64_t rows, int64_t cols, int dtype,
+                          int kind, hipStream_t stream);
+
+/* y[M][N] = xq[M][K] . W[N][K]^T + bias, W as MTQ_MXFP4 (MXFP4QTensor's bytes and scales), fp32
+ * sums, one rounding to y_dtype.  x_dtype >= 0: x is [M][K] of that dtype (row stride x_stride) and
+ * is quantised to `kind` on the way (amax for MTQ_FP8_TENSOR); x_dtype < 0: x and x_scale are the
+ * quantised rows.  w (and a quantised x) 16-byte aligned.  bias: y_dtype or fp32, or NULL.  ws:
+ * mtq_mx_linear_workspace_bytes bytes, 16-byte aligned, contents overwritten. */
+size_t mtq_mx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int kind, int x_dtype);
+int mtq_mx_linear(const void *x, int64_t x_stride, int x_dtype, const void *x_scale, int kind,
+                  const float *amax, const uint8_t *w, const uint8_t *w_scale, const void *bias,
+                  int bias_dtype, void *y, int y_dtype, int64_t M, int64_t N, int64_t K, void *ws,
+                  size_t ws_bytes, hipStream_t stream);
+
+/* ---- KV cache in 4 bits (NVFP4), in pages ------------------------------------------------------
+ * Place (page, head, token) of K (index 0) or V (1): head_dim / 2 bytes of E2M1 codes at data +
+ * page * data_strides[.][0] + head * [1] + token * [2] (bytes, multiples of 16) and head_dim / 16
+ * E4M3 scales at scale + ... (multiples of head_dim / 16); amax: the tensor's fp32 amax on the
+ * device (global scale amax / 2688).  Values as mtq_nvfp4_fake_quant of the rows.  page_size: a
+ * power of two in 16 .. 32768; head_dim 64, 128 or 256. */
+typedef struct {
+  void *data[2];
+  void *scale[2];
+  int64_t data_strides[2][3];
+  int64_t scale_strides[2][3];
+  const float *amax[2];
+  int num_pages, page_size, num_kv_heads, head_dim;
+} mtq_kv_cache;
+
+/* The last b_seq_len[b] of sequence b's b_seq_len_k[b] positions, rows b_start_loc[b] + i of the
+ * [rows][heads][head_dim] tensors k and v (element strides: k token, k head, v token, v head), into
+ * / out of the pages block_table[b * table_stride + position / page_size].  Positions without a page
+ * (an entry outside 0 .. num_pages - 1, a position past the table) are dropped / read as zeros;
+ * other rows are not touched.  A page that a call writes must belong to one sequence. */
+int mtq_kv_append(const mtq_kv_cache *cache, const void *k, const void *v, const int64_t *strides,
+                  int64_t rows, const int32_t *block_table, int64_t table_stride, int table_cols,
+                  const int32_t *b_start_loc, const int32_t *b_seq_len, const int32_t *b_seq_len_k,
+                  int batch, int max_len, int dtype, hipStream_t stream);
+int mtq_kv_read(const mtq_kv_cache *cache, void *k, void *v, const int64_t *strides, int64_t rows,
+                const int32_t *block_table, int64_t table_stride, int table_cols,
+                const int32_t *b_start_loc, const int32_t *b_seq_len, const int32_t *b_seq_len_k,
+                int batch, int max_len, int dtype, hipStream_t stream);
+
+/* o = softmax(softmax_scale q k^T) v for the queries (rows b_start_loc[b] + i, i < b_seq_len[b], the
+ * last positions of their sequence) over the cached keys; causal or not; keys without a page are not
+ * seen, a row that sees no key is zero, rows of no sequence are not touched.  q, o: [rows][heads]
+ * [head_dim] bf16 / f16 (element strides q token, q head, o token, o head, multiples of 8),
+ * 16-byte aligned.  max_len_k sizes the split over the keys (any value is correct).  ws:
+ * mtq_kv_attention_workspace_bytes bytes, 16-byte aligned, contents overwritten. */
+size_t mtq_kv_attention_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                                        int max_len_q, int max_len_k);
+int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const int64_t *strides,
+                     int64_t rows, int num_q_heads, const int32_t *block_table,
+                     int64_t table_stride, int table_cols, const int32_t *b_start_loc,
+                     const int32_t *b_seq_len, const int32_t *b_seq_len_k, int batch, int max_len_q,
+                     int max_len_k, int is_causal, double softmax_scale, int dtype, void *ws,
+                     size_t ws_bytes, hipStream_t stream);
+
 /* ---- dispatch registry (tracing) ----------------------------------------------------------
  * The launchers choose among kernel forms by shape, dtype and alignment (vector / block-group /
  * row-wave fake quant, persistent / row / column amax, ...); each launch of the families below

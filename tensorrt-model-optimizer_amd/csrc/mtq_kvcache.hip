@@ -1,0 +1,659 @@
+// mtq_kvcache.hip — a KV cache held in 4 bits (NVFP4), in pages, and the attention that reads it.
+//
+// A row (one token of one KV head, head_dim values) is D / 2 bytes of E2M1 codes (even column low)
+// and D / 16 E4M3 scales; with the tensor's gs = RN(amax / 2688) a value is
+//   code * RN(scale * gs),   scale = e4m3(min(RN(max|x| / RN(6 gs)), 448)) of its 16 columns,
+// code = e2m1(RN(x / RN(scale * gs))): element for element the NVFP4 fake quant that the K/V
+// quantizers simulate (mtq_nvfp4_fake_quant), whose blocks with scale * gs < 1e-5 come out as zeros
+// (stored here as scale 0, codes 0).
+//
+// Position p of sequence b lives on page table[b][p / page_size], place p % page_size.  The new
+// tokens of a call are the last len_q[b] of its len_k[b] positions; token i of sequence b is row
+// start[b] + i of q / k / v / o.  A table entry outside the cache's pages stands for no page: rows
+// for it are dropped, reads give zeros, the attention does not see its keys.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "mtq_amd.h"
+#include "mtq_device.hpp"
+
+using namespace mtq;
+
+namespace mtq {
+int host_check_launch();
+int host_num_cus();
+}
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+inline bool al16p(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+constexpr float kNegInf = -__builtin_inff(), kPShift = 12.0f;
+
+struct Cache {
+  uint8_t *data[2], *scale[2];                        // K, V
+  int64_t d_page[2], d_head[2], d_tok[2];             // byte strides of the codes
+  int64_t s_page[2], s_head[2], s_tok[2];             // ... and of the scales
+  const float *amax[2];
+  const int32_t *table, *start, *len_q, *len_k;
+  int64_t table_stride;
+  int table_cols, num_pages, shift, hkv, head_dim;
+};
+
+__device__ __forceinline__ float global_scale_of(const float *amax) {
+  const float gs = div_rn(*amax, 2688.0f, 1.0f / 2688.0f);
+  return gs > 0.f ? gs : 1e-12f;
+}
+
+// the page of position pos, -1 where there is none
+__device__ __forceinline__ int page_of(const Cache &c, int b, int pos) {
+  const int slot = pos >> c.shift;
+  if (pos < 0 || slot >= c.table_cols) return -1;
+  const int page = c.table[(int64_t)b * c.table_stride + slot];
+  return page >= 0 && page < c.num_pages ? page : -1;
+}
+
+// ---- rows into pages and back -------------------------------------------------------------------
+// A lane takes one block: 16 columns of one row.  Bound by HBM (32 + 9 bytes a block); consecutive
+// lanes take consecutive blocks, so a wave reads 2 KiB and writes 512 + 64 bytes in one piece each.
+struct RowArgs {
+  Cache c;
+  void *x[2];             // k, v
+  int64_t xt[2], xh[2];   // element strides (token, head)
+  int64_t rows;
+  int max_len, tok_per_wg;
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load16(const T *p, float (&v)[16]) {
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < 16; i += Vec<T>::N) {
+      const Vec<T> a = ldg_vec(p + i);
+#pragma unroll
+      for (int j = 0; j < Vec<T>::N; ++j) v[i + j] = Elem<T>::ld(a.e[j]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = Elem<T>::ld(p[i]);
+  }
+}
+
+// places a lane's block: false where the block is none of a live token's
+struct Place {
+  int kv, h, blk, page, at;
+  int64_t row;
+};
+__device__ __forceinline__ bool place_block(const RowArgs &a, int b, int lq, int lk, int t0, int idx, Place &p) {
+  const int bpr = a.c.head_dim / 16, bpt = 2 * a.c.hkv * bpr;
+  const int t = idx / bpt;
+  int rem = idx - t * bpt;
+  p.kv = rem / (a.c.hkv * bpr);
+  rem -= p.kv * a.c.hkv * bpr;
+  p.h = rem / bpr;
+  p.blk = rem - p.h * bpr;
+  const int i = t0 + t;
+  if (t >= a.tok_per_wg || i >= lq) return false;
+  p.row = (int64_t)a.c.start[b] + i;
+  if (p.row < 0 || p.row >= a.rows) return false;
+  const int pos = lk - lq + i;
+  p.page = page_of(a.c, b, pos);
+  p.at = pos & ((1 << a.c.shift) - 1);
+  return true;
+}
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void cache_append_kernel(RowArgs a) {
+  const int b = blockIdx.y, lq = a.c.len_q[b], lk = a.c.len_k[b], t0 = blockIdx.x * a.tok_per_wg;
+  if (t0 >= lq) return;
+  const float gs[2] = {global_scale_of(a.c.amax[0]), global_scale_of(a.c.amax[1])};
+  const int n = a.tok_per_wg * 2 * a.c.hkv * (a.c.head_dim / 16);
+  for (int idx = threadIdx.x; idx < n; idx += 256) {
+    Place p;
+    if (!place_block(a, b, lq, lk, t0, idx, p) || p.page < 0) continue;
+    const int kv = p.kv;
+    float v[16];
+    load16<T, VEC>(reinterpret_cast<const T *>(kv ? a.x[1] : a.x[0]) + p.row * (kv ? a.xt[1] : a.xt[0]) +
+                       p.h * (kv ? a.xh[1] : a.xh[0]) + 16 * p.blk, v);
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) m = max_skip_nan(m, v[j]);
+    const float g = kv ? gs[1] : gs[0], six = 6.0f * g;
+    float s8 = div_rn(m, six, 1.0f / six);
+    s8 = s8 < kE4M3Max ? s8 : kE4M3Max;
+    int sb = __builtin_amdgcn_cvt_pk_fp8_f32(s8, s8, 0, false) & 0xff;
+    const float q = __builtin_amdgcn_cvt_f32_fp8(sb, 0) * g;
+    uint32_t w[2] = {0, 0};
+    if (q >= 1e-5f) {
+      const float r = 1.0f / q;
+      float c[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float t = fminf(div_rn(fabsf(v[j]), q, r), 6.0f);  // inf and NaN: 6
+        c[j] = v[j] >= 0.f ? t : -t;
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float *e = c + 8 * k;
+        w[k] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[k], e[0], e[1], 1.0f, 0);
+        w[k] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[k], e[2], e[3], 1.0f, 1);
+        w[k] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[k], e[4], e[5], 1.0f, 2);
+        w[k] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[k], e[6], e[7], 1.0f, 3);
+      }
+    } else {
+      sb = 0;
+    }
+    uint8_t *d = (kv ? a.c.data[1] : a.c.data[0]) + p.page * (kv ? a.c.d_page[1] : a.c.d_page[0]) +
+                 p.h * (kv ? a.c.d_head[1] : a.c.d_head[0]) + p.at * (kv ? a.c.d_tok[1] : a.c.d_tok[0]);
+    uint8_t *s = (kv ? a.c.scale[1] : a.c.scale[0]) + p.page * (kv ? a.c.s_page[1] : a.c.s_page[0]) +
+                 p.h * (kv ? a.c.s_head[1] : a.c.s_head[0]) + p.at * (kv ? a.c.s_tok[1] : a.c.s_tok[0]);
+    *reinterpret_cast<uint2 *>(d + 8 * p.blk) = make_uint2(w[0], w[1]);
+    s[p.blk] = (uint8_t)sb;
+  }
+}
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void cache_read_kernel(RowArgs a) {
+  const int b = blockIdx.y, lq = a.c.len_q[b], lk = a.c.len_k[b], t0 = blockIdx.x * a.tok_per_wg;
+  if (t0 >= lq) return;
+  const float gs[2] = {global_scale_of(a.c.amax[0]), global_scale_of(a.c.amax[1])};
+  const int n = a.tok_per_wg * 2 * a.c.hkv * (a.c.head_dim / 16);
+  for (int idx = threadIdx.x; idx < n; idx += 256) {
+    Place p;
+    if (!place_block(a, b, lq, lk, t0, idx, p)) continue;
+    const int kv = p.kv;
+    uint2 w = make_uint2(0, 0);
+    int sb = 0;
+    if (p.page >= 0) {
+      w = *reinterpret_cast<const uint2 *>((kv ? a.c.data[1] : a.c.data[0]) + p.page * (kv ? a.c.d_page[1] : a.c.d_page[0]) +
+                                           p.h * (kv ? a.c.d_head[1] : a.c.d_head[0]) +
+                                           p.at * (kv ? a.c.d_tok[1] : a.c.d_tok[0]) + 8 * p.blk);
+      sb = ((kv ? a.c.scale[1] : a.c.scale[0]) + p.page * (kv ? a.c.s_page[1] : a.c.s_page[0]) +
+            p.h * (kv ? a.c.s_head[1] : a.c.s_head[0]) + p.at * (kv ? a.c.s_tok[1] : a.c.s_tok[0]))[p.blk];
+    }
+    const float q = __builtin_amdgcn_cvt_f32_fp8(sb, 0) * (kv ? gs[1] : gs[0]);
+    T *x = reinterpret_cast<T *>(kv ? a.x[1] : a.x[0]) + p.row * (kv ? a.xt[1] : a.xt[0]) + p.h * (kv ? a.xh[1] : a.xh[0]) +
+           16 * p.blk;
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t u = k ? w.y : w.x;
+      auto pair = [&](auto e, int i) { v[8 * k + 2 * i] = e[0] * q, v[8 * k + 2 * i + 1] = e[1] * q; };
+      pair(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 0), 0);
+      pair(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 1), 1);
+      pair(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 2), 2);
+      pair(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 3), 3);
+    }
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < 16; i += Vec<T>::N) {
+        Vec<T> o;
+#pragma unroll
+        for (int j = 0; j < Vec<T>::N; ++j) o.e[j] = Elem<T>::st(v[i + j]);
+        stg_vec(x + i, o);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = Elem<T>::st(v[i]);
+    }
+  }
+}
+
+// ---- attention -----------------------------------------------------------------------------------
+// o = softmax(sm_scale q k^T) v over the pages of a sequence, G query heads to a KV head.
+//
+// A row is (query token, head of the group); 16 rows are one column block of the matrix
+// instructions.  Scores are computed transposed, S^T = K q^T (v_mfma_f32_16x16x32_f16: lane
+// (c = lane & 15, g = lane >> 4) holds row c's scores of keys 4 g .. 4 g + 3), so a row's maximum and
+// sum are in-lane work and two exchanges, and the probabilities are already the second operand of
+// O^T += V^T P^T, whose contraction takes the keys in the order the lanes hold them.
+//   K: lane (t = lane & 15, g) loads the codes of key t's columns [D / 4 g, D / 4 (g + 1)) and turns
+//      them into fp16 products code * scale: exact (at most 6 significant bits, 2^-10 .. 2688); gs goes
+//      into the softmax factor.  The contraction over head_dim takes the columns in that order, q too.
+//   q: to fp16 with a power of two of its row that puts its largest value into [2^14, 2^15): 8
+//      (bf16) or 11 (fp16) bits stay exact down to 2^-28 of it.
+//   V: the same products, through LDS rows that ds_read_b64_tr_b16 reads transposed.
+//   P: fp16, 2^12 exp2(x - running maximum): off by 2^-12 of each weight, and a normal number down to
+//      2^-26 of the largest; the row sum carries the same 2^12.
+// Sums and the accumulators are fp32.
+//
+// A wave takes 32 keys at a time, the waves of a workgroup every fourth 32 keys, and keep statistics
+// of their own, joined through LDS at the end (in wave order).  Where there are few sequences the
+// keys are cut into splits; their partial results are joined by a second small kernel, in order.
+struct AttnArgs {
+  Cache c;
+  const void *q;
+  void *o;
+  float *part;  // [splits][batch][hkv][tiles][16][D + 2] (o, m, l) of each split
+  int64_t qt, qh, ot, oh, rows;
+  int group, causal, splits, chunk, tiles, batch;
+  float sm_log2;  // softmax_scale * log2(e)
+};
+
+// fp16 values of a lane's D / 4 codes times their block scales; ok false: zeros
+template <int D>
+__device__ __forceinline__ void dequant(const uint32_t (&w)[D / 32], uint32_t sc, bool ok, h8 (&f)[D / 32]) {
+  // the lane's columns are D / 64 blocks of 16 = 2 dwords each
+#pragma unroll
+  for (int k = 0; k < D / 64; ++k) {
+    const float s = ok ? (k == 0 ? __builtin_amdgcn_cvt_f32_fp8(sc, 0) : k == 1 ? __builtin_amdgcn_cvt_f32_fp8(sc, 1) : k == 2 ? __builtin_amdgcn_cvt_f32_fp8(sc, 2) : __builtin_amdgcn_cvt_f32_fp8(sc, 3)) : 0.f;
+    const _Float16 h = (_Float16)s;
+    const h2 hs = {h, h};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t u = w[2 * k + i];
+      const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(u, 1.0f, 0)) * hs;
+      const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(u, 1.0f, 1)) * hs;
+      const h2 c = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(u, 1.0f, 2)) * hs;
+      const h2 d = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(u, 1.0f, 3)) * hs;
+      f[2 * k + i] = h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+    }
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void load_codes(const uint8_t *d, const uint8_t *s, uint32_t (&w)[D / 32], uint32_t &sc) {
+  if constexpr (D == 64) {
+    const uint2 a = *reinterpret_cast<const uint2 *>(d);
+    w[0] = a.x, w[1] = a.y;
+    sc = *s;
+  } else {
+#pragma unroll
+    for (int i = 0; i < D / 128; ++i) {
+      const uint4 a = *reinterpret_cast<const uint4 *>(d + 16 * i);
+      w[4 * i] = a.x, w[4 * i + 1] = a.y, w[4 * i + 2] = a.z, w[4 * i + 3] = a.w;
+    }
+    if constexpr (D == 128)
+      sc = *reinterpret_cast<const uint16_t *>(s);
+    else
+      sc = *reinterpret_cast<const uint32_t *>(s);
+  }
+}
+
+__device__ __forceinline__ float max_g(float v) {  // over the 4 lanes of a row (lane ^ 16, lane ^ 32)
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float sum_g(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_decode_kernel(AttnArgs a) {
+  constexpr int NF = D / 32;                // fragments of a row in the contraction over head_dim
+  constexpr int NB = D / 16;                // 16-column blocks of the output
+  constexpr int VP = 2 * D + 32;            // V row pitch in LDS
+  constexpr int kVBytes = 32 * VP;
+  constexpr int kOBytes = 4 * 16 * (D + 4) * 4;
+  constexpr int kBytes = 4 * kVBytes > kOBytes ? 4 * kVBytes : kOBytes;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kBytes];
+  __shared__ float ml[2][4][16];
+  const Cache &c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), t = lane & 15, g = lane >> 4;
+  const int split = blockIdx.x, kvh = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles, b = blockIdx.z;
+  const int lq = c.len_q[b];
+  int lk = c.len_k[b];
+  const int cap = c.table_cols << c.shift;
+  const int off = lk - lq;  // a query token's place in its sequence
+  lk = lk < cap ? lk : cap;
+  const int nrows = lq > 0 ? lq * a.group : 0;
+  if (16 * tile >= nrows) return;
+  const int last_tok = (16 * tile + 15 < nrows ? 16 * tile + 15 : nrows - 1) / a.group;
+  int kv_end = a.causal ? off + last_tok + 1 : lk;
+  kv_end = kv_end < lk ? kv_end : lk;
+  const int t0 = split * a.chunk;
+  if (split > 0 && t0 >= kv_end) return;  // the join knows the splits that there are
+  // the last split takes what is left, should a sequence be longer than the call's max_len_k
+  const int t1 = split + 1 < a.splits && t0 + a.chunk < kv_end ? t0 + a.chunk : kv_end;
+
+  // ---- this lane's row of q
+  const int row = 16 * tile + t, rtok = row / a.group, head = kvh * a.group + row % a.group;
+  const int64_t qrow = (int64_t)c.start[b] + rtok;
+  const bool row_ok = row < nrows && qrow >= 0 && qrow < a.rows;
+  const int see = row_ok ? (a.causal ? (off + rtok + 1 < lk ? off + rtok + 1 : lk) : lk) : 0;  // keys it sees
+  h8 qf[NF];
+  float qscale;
+  {
+    float v[NF][8];
+    float m = 0.f;
+    const T *qp = reinterpret_cast<const T *>(a.q) + (row_ok ? qrow : 0) * a.qt + head * a.qh + g * (D / 4);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      const Vec<T> x = row_ok ? ldg_vec(qp + 8 * f) : Vec<T>{};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[f][j] = row_ok ? Elem<T>::ld(x.e[j]) : 0.f;
+        m = max_skip_nan(m, v[f][j]);
+      }
+    }
+    m = max_g(m);
+    int e = (int)(__float_as_uint(m) >> 23) - 127;   // m >= 0
+    e = m == 0.f || e == 128 ? 0 : e < -100 ? -100 : e;  // inf: left as it is
+    const float up = pow2f(14 - e < 127 ? 14 - e : 127);
+    qscale = a.sm_log2 * global_scale_of(c.amax[0]) * (1.0f / up);
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) qf[f][j] = (_Float16)(v[f][j] * up);
+  }
+
+  f32x4 acc[NB];
+#pragma unroll
+  for (int d = 0; d < NB; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = kNegInf, l = 0.f;
+  unsigned char *const vb = lds + wave * kVBytes;
+  const uint8_t *kd = c.data[0] + kvh * c.d_head[0] + g * (D / 8), *ks = c.scale[0] + kvh * c.s_head[0] + g * (D / 64);
+  const uint8_t *vd = c.data[1] + kvh * c.d_head[1] + g * (D / 8), *vs = c.scale[1] + kvh * c.s_head[1] + g * (D / 64);
+
+  for (int kv = t0 + 32 * wave; kv < t1; kv += 128) {
+    uint32_t kw[2][NF], vw[2][NF], ksc[2], vsc[2];
+    bool has[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {  // 16 keys: one page
+      const int page = __builtin_amdgcn_readfirstlane(page_of(c, b, kv + 16 * u));
+      has[u] = page >= 0;
+      const int64_t pg = has[u] ? page : 0;
+      const int at = ((kv + 16 * u) & ((1 << c.shift) - 1)) + t;
+      load_codes<D>(kd + pg * c.d_page[0] + at * c.d_tok[0], ks + pg * c.s_page[0] + at * c.s_tok[0], kw[u], ksc[u]);
+      load_codes<D>(vd + pg * c.d_page[1] + at * c.d_tok[1], vs + pg * c.s_page[1] + at * c.s_tok[1], vw[u], vsc[u]);
+    }
+    // ---- scores
+    f32x4 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      h8 kf[NF];
+      dequant<D>(kw[u], ksc[u], true, kf);
+      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int f = 0; f < NF; ++f) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[f], qf[f], s[u], 0, 0, 0);
+    }
+    // ---- V to LDS (rows that hold no token of this sequence as zeros: 0 * NaN is NaN)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      h8 vf[NF];
+      dequant<D>(vw[u], vsc[u], has[u] && kv + 16 * u + t < lk, vf);
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+        *reinterpret_cast<h8 *>(vb + (16 * u + t) * VP + g * (D / 2) + 16 * f) = vf[f];
+    }
+    // ---- softmax: keys kv + 16 u + 4 g + j
+    float x[2][4], mx = kNegInf;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[u][j] = has[u] && kv + 16 * u + 4 * g + j < see ? s[u][j] * qscale : kNegInf;
+        mx = fmaxf(mx, x[u][j]);
+      }
+    const float mn = fmaxf(m, max_g(mx));
+    const float mu = mn == kNegInf ? 0.f : mn;
+    const float corr = __builtin_amdgcn_exp2f(m - mu);
+    m = mn;
+    h8 p;
+    float ls = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = __builtin_amdgcn_exp2f(x[u][j] - (mu - kPShift));
+        ls += e;
+        p[4 * u + j] = (_Float16)e;
+      }
+    l = l * corr + ls;  // this lane's keys only; joined at the end
+#pragma unroll
+    for (int d = 0; d < NB; ++d) acc[d] *= corr;
+    // ---- O^T += V^T P^T
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int d = 0; d < NB; ++d) {
+      const unsigned char *base = vb + (4 * g + (t >> 2)) * VP + 32 * d + 8 * (t & 3);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)base);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(base + 16 * VP));
+      const h4 a0 = __builtin_bit_cast(h4, lo), a1 = __builtin_bit_cast(h4, hi);
+      const h8 vt = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+      acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, p, acc[d], 0, 0, 0);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // ---- join the waves: rows t, columns 16 d + 4 g + j
+  l = sum_g(l);
+  __syncthreads();  // every wave is done with its V rows
+  float *ob = reinterpret_cast<float *>(lds) + wave * 16 * (D + 4);
+#pragma unroll
+  for (int d = 0; d < NB; ++d) *reinterpret_cast<f32x4 *>(ob + t * (D + 4) + 16 * d + 4 * g) = acc[d];
+  if (g == 0) {
+    ml[0][wave][t] = m;
+    ml[1][wave][t] = l;
+  }
+  __syncthreads();
+  const float gv = global_scale_of(c.amax[1]);
+  for (int i = tid; i < 16 * (D / 4); i += 256) {
+    const int r = i / (D / 4), d4 = 4 * (i % (D / 4)), rr = 16 * tile + r;
+    if (rr >= nrows) continue;
+    float mm = kNegInf;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[0][w][r]);
+    const float mu = mm == kNegInf ? 0.f : mm;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float ls = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(ml[0][w][r] - mu);
+      ls += ml[1][w][r] * f;
+      o += *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(lds) + (w * 16 + r) * (D + 4) + d4) * f;
+    }
+    if (a.splits > 1) {
+      float *pp = a.part + ((((int64_t)split * a.batch + b) * c.hkv + kvh) * a.tiles + tile) * 16 * (D + 4) + r * (D + 4);
+      *reinterpret_cast<f32x4 *>(pp + d4) = o;
+      if (d4 == 0) pp[D] = mm, pp[D + 1] = ls;
+    } else {
+      const int64_t orow = (int64_t)c.start[b] + rr / a.group;
+      if (orow < 0 || orow >= a.rows) continue;
+      const float inv = ls > 0.f ? gv / ls : 0.f;
+      T *op = reinterpret_cast<T *>(a.o) + orow * a.ot + (kvh * a.group + rr % a.group) * a.oh + d4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) op[j] = Elem<T>::st(ls == ls && ls == 0.f ? 0.f : o[j] * inv);
+    }
+  }
+}
+
+// the splits of a row, in order
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  const Cache &c = a.c;
+  const int kvh = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles, b = blockIdx.z;
+  const int lq = c.len_q[b];
+  int lk = c.len_k[b];
+  const int cap = c.table_cols << c.shift, off = lk - lq;
+  lk = lk < cap ? lk : cap;
+  const int nrows = lq > 0 ? lq * a.group : 0;
+  if (16 * tile >= nrows) return;
+  const int last_tok = (16 * tile + 15 < nrows ? 16 * tile + 15 : nrows - 1) / a.group;
+  int kv_end = a.causal ? off + last_tok + 1 : lk;
+  kv_end = kv_end < lk ? kv_end : lk;
+  int n = kv_end > 0 ? (kv_end + a.chunk - 1) / a.chunk : 1;
+  n = n < a.splits ? n : a.splits;
+  const float gv = global_scale_of(c.amax[1]);
+  const int64_t step = (int64_t)a.batch * c.hkv * a.tiles * 16 * (D + 4);
+  for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
+    const int r = i / (D / 4), d4 = 4 * (i % (D / 4)), rr = 16 * tile + r;
+    const int64_t orow = (int64_t)c.start[b] + rr / a.group;
+    if (rr >= nrows || orow < 0 || orow >= a.rows) continue;
+    const float *pp = a.part + (((int64_t)b * c.hkv + kvh) * a.tiles + tile) * 16 * (D + 4) + r * (D + 4);
+    float mm = kNegInf;
+    for (int s = 0; s < n; ++s) mm = fmaxf(mm, pp[s * step + D]);
+    const float mu = mm == kNegInf ? 0.f : mm;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float ls = 0.f;
+    for (int s = 0; s < n; ++s) {
+      const float f = __builtin_amdgcn_exp2f(pp[s * step + D] - mu);
+      ls += pp[s * step + D + 1] * f;
+      o += *reinterpret_cast<const f32x4 *>(pp + s * step + d4) * f;
+    }
+    const float inv = gv / ls;
+    T *op = reinterpret_cast<T *>(a.o) + orow * a.ot + (kvh * a.group + rr % a.group) * a.oh + d4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) op[j] = Elem<T>::st(ls == 0.f ? 0.f : o[j] * inv);
+  }
+}
+
+bool make_cache(const mtq_kv_cache *k, const int32_t *table, int64_t table_stride, int table_cols, const int32_t *start,
+                const int32_t *len_q, const int32_t *len_k, int batch, Cache &c) {
+  if (!k || !table || !start || !len_q || !len_k || batch < 1 || table_cols < 1 || (batch > 1 && table_stride < table_cols)) return false;
+  if (k->page_size < 16 || k->page_size > 32768 || (k->page_size & (k->page_size - 1))) return false;
+  if (k->num_pages < 1 || k->num_kv_heads < 1) return false;
+  if (k->head_dim != 64 && k->head_dim != 128 && k->head_dim != 256) return false;
+  if ((int64_t)table_cols * k->page_size > (int64_t)INT32_MAX / 2) return false;  // positions are ints
+  for (int i = 0; i < 2; ++i) {
+    c.data[i] = (uint8_t *)k->data[i], c.scale[i] = (uint8_t *)k->scale[i], c.amax[i] = k->amax[i];
+    c.d_page[i] = k->data_strides[i][0], c.d_head[i] = k->data_strides[i][1], c.d_tok[i] = k->data_strides[i][2];
+    c.s_page[i] = k->scale_strides[i][0], c.s_head[i] = k->scale_strides[i][1], c.s_tok[i] = k->scale_strides[i][2];
+    if (!c.data[i] || !c.scale[i] || !c.amax[i]) return false;
+    const int sb = k->head_dim / 16;
+    // rows: 16-byte aligned codes, scales aligned to a row of theirs
+    if ((uintptr_t)c.data[i] % 16 || (uintptr_t)c.scale[i] % sb) return false;
+    for (int j = 0; j < 3; ++j)
+      if (k->data_strides[i][j] < 0 || k->data_strides[i][j] % 16 || k->scale_strides[i][j] < 0 || k->scale_strides[i][j] % sb) return false;
+  }
+  c.table = table, c.start = start, c.len_q = len_q, c.len_k = len_k, c.table_stride = table_stride;
+  c.table_cols = table_cols, c.num_pages = k->num_pages, c.hkv = k->num_kv_heads, c.head_dim = k->head_dim;
+  c.shift = 0;
+  while ((1 << c.shift) < k->page_size) c.shift++;
+  return true;
+}
+
+int rows_call(bool append, const mtq_kv_cache *cache, void *k, void *v, const int64_t *strides, int64_t rows,
+              const int32_t *table, int64_t table_stride, int table_cols, const int32_t *start, const int32_t *len_q,
+              const int32_t *len_k, int batch, int max_len, int dtype, hipStream_t stream) {
+  if (dtype != MTQ_BF16 && dtype != MTQ_F16 && dtype != MTQ_F32) return MTQ_ERR_DTYPE;
+  RowArgs a;
+  if (!strides || rows < 0 || max_len < 0 || batch < 0 || batch > 65535) return MTQ_ERR_INVALID_ARG;
+  if (batch == 0 || max_len == 0 || rows == 0) return MTQ_OK;
+  if (!k || !v || !make_cache(cache, table, table_stride, table_cols, start, len_q, len_k, batch, a.c)) return MTQ_ERR_INVALID_ARG;
+  a.x[0] = k, a.x[1] = v;
+  a.xt[0] = strides[0], a.xh[0] = strides[1], a.xt[1] = strides[2], a.xh[1] = strides[3];
+  a.rows = rows, a.max_len = max_len;
+  const int bpt = 2 * a.c.hkv * (a.c.head_dim / 16);
+  a.tok_per_wg = bpt >= 512 ? 1 : 512 / bpt;  // two blocks a lane
+  if (a.tok_per_wg > max_len) a.tok_per_wg = max_len;
+  const int es = dtype == MTQ_F32 ? 4 : 2;
+  bool vec = al16p(k) && al16p(v);
+  for (int i = 0; i < 4; ++i) {
+    if (strides[i] < 0) return MTQ_ERR_INVALID_ARG;
+    vec = vec && (strides[i] * es) % 16 == 0;
+  }
+  const dim3 g((unsigned)((max_len + a.tok_per_wg - 1) / a.tok_per_wg), (unsigned)batch);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    if (append)
+      vec ? cache_append_kernel<T, true><<<g, 256, 0, stream>>>(a) : cache_append_kernel<T, false><<<g, 256, 0, stream>>>(a);
+    else
+      vec ? cache_read_kernel<T, true><<<g, 256, 0, stream>>>(a) : cache_read_kernel<T, false><<<g, 256, 0, stream>>>(a);
+    return host_check_launch();
+  };
+  return dtype == MTQ_BF16 ? go(__bf16{}) : dtype == MTQ_F16 ? go(_Float16{}) : go(float{});
+}
+
+// keys of a split: enough workgroups to fill the card, at least 128 keys (one 32-key step a wave)
+struct Plan {
+  int tiles, chunk, splits;
+};
+Plan attn_plan(int batch, int hkv, int group, int max_len_q, int max_len_k) {
+  Plan p;
+  p.tiles = (int)(((int64_t)max_len_q * group + 15) / 16);
+  const int64_t wgs = (int64_t)batch * hkv * p.tiles, want = 8 * 256;
+  int64_t splits = (want + wgs - 1) / wgs;
+  const int64_t most = (max_len_k + 127) / 128;
+  splits = splits < most ? splits : most;
+  splits = splits < 1 ? 1 : splits > 256 ? 256 : splits;
+  int64_t chunk = (max_len_k + splits - 1) / splits;
+  chunk = (chunk + 127) / 128 * 128;
+  p.chunk = (int)(chunk < 128 ? 128 : chunk);
+  p.splits = (max_len_k + p.chunk - 1) / p.chunk;
+  if (p.splits < 1) p.splits = 1;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mtq_kv_append(const mtq_kv_cache *cache, const void *k, const void *v, const int64_t *strides, int64_t rows,
+                  const int32_t *block_table, int64_t table_stride, int table_cols, const int32_t *b_start_loc,
+                  const int32_t *b_seq_len, const int32_t *b_seq_len_k, int batch, int max_len, int dtype, hipStream_t stream) {
+  return rows_call(true, cache, const_cast<void *>(k), const_cast<void *>(v), strides, rows, block_table, table_stride,
+                   table_cols, b_start_loc, b_seq_len, b_seq_len_k, batch, max_len, dtype, stream);
+}
+
+int mtq_kv_read(const mtq_kv_cache *cache, void *k, void *v, const int64_t *strides, int64_t rows, const int32_t *block_table,
+                int64_t table_stride, int table_cols, const int32_t *b_start_loc, const int32_t *b_seq_len,
+                const int32_t *b_seq_len_k, int batch, int max_len, int dtype, hipStream_t stream) {
+  return rows_call(false, cache, k, v, strides, rows, block_table, table_stride, table_cols, b_start_loc, b_seq_len,
+                   b_seq_len_k, batch, max_len, dtype, stream);
+}
+
+size_t mtq_kv_attention_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim, int max_len_q, int max_len_k) {
+  if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_len_q < 1 || head_dim < 1) return 0;
+  const Plan p = attn_plan(batch, num_kv_heads, num_q_heads / num_kv_heads, max_len_q, max_len_k);
+  return p.splits > 1 ? (size_t)p.splits * batch * num_kv_heads * p.tiles * 16 * (head_dim + 4) * sizeof(float) : 0;
+}
+
+int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const int64_t *strides, int64_t rows, int num_q_heads,
+                     const int32_t *block_table, int64_t table_stride, int table_cols, const int32_t *b_start_loc,
+                     const int32_t *b_seq_len, const int32_t *b_seq_len_k, int batch, int max_len_q, int max_len_k,
+                     int is_causal, double softmax_scale, int dtype, void *ws, size_t ws_bytes, hipStream_t stream) {
+  if (dtype != MTQ_BF16 && dtype != MTQ_F16) return MTQ_ERR_DTYPE;
+  if (!strides || rows < 0 || max_len_q < 0 || max_len_k < 0 || batch < 0 || batch > 65535) return MTQ_ERR_INVALID_ARG;
+  if (batch == 0 || max_len_q == 0 || rows == 0) return MTQ_OK;
+  AttnArgs a;
+  if (!q || !o || !make_cache(cache, block_table, table_stride, table_cols, b_start_loc, b_seq_len, b_seq_len_k, batch, a.c))
+    return MTQ_ERR_INVALID_ARG;
+  if (num_q_heads < 1 || num_q_heads % a.c.hkv) return MTQ_ERR_INVALID_ARG;
+  for (int i = 0; i < 4; ++i)
+    if (strides[i] < 0 || strides[i] % 8) return MTQ_ERR_INVALID_ARG;
+  if (!al16p(q) || !al16p(o) || !(softmax_scale == softmax_scale)) return MTQ_ERR_INVALID_ARG;
+  const int64_t cap = (int64_t)table_cols * cache->page_size;
+  if (max_len_k > cap) max_len_k = (int)cap;
+  a.group = num_q_heads / a.c.hkv;
+  if ((int64_t)max_len_q * a.group > INT32_MAX - 16) return MTQ_ERR_INVALID_ARG;
+  const Plan p = attn_plan(batch, a.c.hkv, a.group, max_len_q, max_len_k);
+  if ((int64_t)p.tiles * a.c.hkv > 65535) return MTQ_ERR_INVALID_ARG;
+  const size_t need = mtq_kv_attention_workspace_bytes(batch, num_q_heads, a.c.hkv, a.c.head_dim, max_len_q, max_len_k);
+  if (need && (!ws || ws_bytes < need || !al16p(ws))) return MTQ_ERR_INVALID_ARG;
+  a.q = q, a.o = o, a.part = (float *)ws;
+  a.qt = strides[0], a.qh = strides[1], a.ot = strides[2], a.oh = strides[3], a.rows = rows;
+  a.causal = is_causal ? 1 : 0;
+  a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles, a.batch = batch;
+  a.sm_log2 = (float)(softmax_scale * 1.44269504088896);
+  const dim3 g((unsigned)p.splits, (unsigned)(p.tiles * a.c.hkv), (unsigned)batch), gj(1, g.y, g.z);
+  auto go = [&](auto t, auto d) {
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    attn_decode_kernel<T, D><<<g, 256, 0, stream>>>(a);
+    const int st = host_check_launch();
+    if (st != MTQ_OK || p.splits == 1) return st;
+    attn_join_kernel<T, D><<<gj, 256, 0, stream>>>(a);
+    return host_check_launch();
+  };
+  auto dims = [&](auto t) {
+    switch (a.c.head_dim) {
+    case 64: return go(t, std::integral_constant<int, 64>{});
+    case 128: return go(t, std::integral_constant<int, 128>{});
+    default: return go(t, std::integral_constant<int, 256>{});
+    }
+  };
+  return dtype == MTQ_BF16 ? dims(__bf16{}) : dims(_Float16{});
+}
+
+}  // extern "C"

@@ -1,0 +1,600 @@
+// mtq_mx.hip — microscaled operands and their products on gfx950: quantising activations, the RMS
+// norm that quantises its output, and y = xq . W^T with W packed as MXFP4.
+//
+// Formats.  A row of K values is held as K / 32 blocks; block b has an exponent e_b (E8M0 byte
+// e_b + 127) and 32 elements q, value = q * 2^e_b:
+//   e_b = ceil(log2(max|x| / most)), q = round(x / 2^e_b), most = 6 (E2M1, two codes a byte, the
+//   even column low) or 448 (E4M3, a byte each)
+// -- the values of the dynamic block fake quant (mtq_fused_amax_convert with E8M0 scales): a block
+// of zeros has e = 0, NaN is left out of the maximum, an infinity counts as FLT_MAX and saturates,
+// a NaN element becomes +6 in E2M1 and stays NaN in E4M3.  Two plain FP8 formats stand beside them:
+// per tensor (values of mtq_fake_e4m3fy: q = e4m3(x * s), s = RN(RN(1 / amax) * 448), factor 1 / s)
+// and per token (factor max|x| / 448 of the row, 1 for a row of zeros, q = e4m3(x / factor)).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mtq_amd.h"
+#include "mtq_device.hpp"
+
+using namespace mtq;
+
+namespace mtq {
+int host_check_launch();
+int host_num_cus();
+}
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+inline bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// ---- 8 consecutive values --------------------------------------------------------------------
+// VEC: 16-byte aligned groups of 8 columns, none of them past the row; else element by element.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T *p, int64_t col, int64_t cols, float (&v)[8]) {
+  if constexpr (VEC) {
+    constexpr int N = Vec<T>::N;
+#pragma unroll
+    for (int i = 0; i < 8; i += N) {
+      const Vec<T> a = ldg_vec(p + col + i);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[i + j] = Elem<T>::ld(a.e[j]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? Elem<T>::ld(p[col + i]) : 0.f;
+  }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T *p, int64_t col, int64_t cols, const float (&v)[8]) {
+  if constexpr (VEC) {
+    constexpr int N = Vec<T>::N;
+#pragma unroll
+    for (int i = 0; i < 8; i += N) {
+      Vec<T> a;
+#pragma unroll
+      for (int j = 0; j < N; ++j) a.e[j] = Elem<T>::st(v[i + j]);
+      stg_vec(p + col + i, a);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < cols) p[col + i] = Elem<T>::st(v[i]);
+  }
+}
+
+// |x| for a block's maximum: NaN left out, infinities as FLT_MAX
+__device__ __forceinline__ float mx_abs(float v) { return clamp_flt_max(abs_or_zero(v)); }
+
+// 8 values -> 8 E2M1 codes of v / 2^e (unscale = 2^e): v_cvt_scalef32_pk_fp4_f32 rounds to nearest,
+// halves to the even code, and saturates; it turns NaN into +-6, so NaN enters as +inf
+// (the convert is checked for scales 2^-125 .. 2^125: blocks further out are moved by 2^64, exactly)
+__device__ __forceinline__ uint32_t e2m1_codes8(const float (&v)[8], float unscale) {
+  float a[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = v[j] != v[j] ? __builtin_inff() : v[j];
+  if (!(unscale >= 0x1p-100f && unscale <= 0x1p100f)) {
+    const float k = unscale < 1.f ? 0x1p64f : 0x1p-64f;
+    unscale *= k;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] *= k;
+  }
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, a[0], a[1], unscale, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, a[2], a[3], unscale, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, a[4], a[5], unscale, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, a[6], a[7], unscale, 3);
+  return w;
+}
+// 8 values -> 8 E4M3 bytes of v * s, saturating, NaN kept
+__device__ __forceinline__ uint2 e4m3_codes8(const float (&v)[8], float s) {
+  float a[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = clamp_nan(v[j] * s, -kE4M3Max, kE4M3Max);
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(a[0], a[1], lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(a[2], a[3], lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(a[4], a[5], hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(a[6], a[7], hi, true);
+  return make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+
+// One block of 32 in 4 consecutive lanes of 8 values: codes to the row q, the exponent byte to sc[]
+template <int KIND>
+__device__ __forceinline__ void mx_store8(const float (&v)[8], int64_t col, uint8_t *q, uint8_t *sc, bool live) {
+  float m = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = fmaxf(m, mx_abs(v[j]));
+  m = group_max_f<4>(m);
+  float scale, unscale;
+  e8m0_scale(m, KIND == MTQ_MXFP4 ? 6.0f : kE4M3Max, scale, unscale);
+  if (!live) return;
+  if constexpr (KIND == MTQ_MXFP4)
+    *reinterpret_cast<uint32_t *>(q + col / 2) = e2m1_codes8(v, unscale);
+  else
+    *reinterpret_cast<uint2 *>(q + col) = e4m3_codes8(v, scale);
+  if ((col & 31) == 0) {
+    // unscale = 2^e, e in [-127, 127]: its exponent field, 0 for the subnormal 2^-127
+    sc[col / 32] = (uint8_t)((__float_as_uint(unscale) >> 23) & 0xff);
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void fp8_store8(const float (&v)[8], float s, int64_t col, int64_t cols, uint8_t *q) {
+  const uint2 w = e4m3_codes8(v, s);
+  if constexpr (VEC) {
+    *reinterpret_cast<uint2 *>(q + col) = w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (col + j < cols) q[col + j] = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
+  }
+}
+
+// ---- sums and maxima over a workgroup (its waves' results through LDS, in wave order) ----------
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// ---- residual addition + RMS norm + quantised output ------------------------------------------
+// h = RN_T(x + r); y = h * rsqrt(mean(h^2) + eps) * w in fp32, quantised from the fp32 value (no
+// rounding of y to T in between: an unfused norm rounds there because it has to store y).
+// Bound by HBM: x, r, h and a byte of codes per element, each touched once.  A workgroup takes one
+// row and keeps it in registers (NV groups of 8 columns a lane) between the sum of squares and the
+// output, so nothing is read twice.
+struct NormArgs {
+  const void *x, *r, *w;
+  void *h;
+  uint8_t *q;
+  void *scale;
+  const float *amax;
+  int64_t xs, rs, cols;
+  float eps;
+  int w_dtype;
+};
+
+template <typename T, int KIND, int NV, bool VEC>
+__global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
+  __shared__ float red[2][16];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
+  const T *x = reinterpret_cast<const T *>(a.x) + row * a.xs;
+  float f[NV][8];
+  float ss = 0.f;
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int64_t col = 8 * ((int64_t)u * blockDim.x + tid);
+    if (col >= a.cols) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[u][j] = 0.f;
+      continue;
+    }
+    load8<T, VEC>(x, col, a.cols, f[u]);
+    if (a.r) {
+      float r[8];
+      load8<T, VEC>(reinterpret_cast<const T *>(a.r) + row * a.rs, col, a.cols, r);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[u][j] = Elem<T>::ld(Elem<T>::st(f[u][j] + r[j]));
+      store8<T, VEC>(reinterpret_cast<T *>(a.h) + row * a.cols, col, a.cols, f[u]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(f[u][j], f[u][j], ss);
+  }
+  ss = wave_sum(ss);
+  if (lane == 0) red[0][wave] = ss;
+  __syncthreads();
+  ss = 0.f;
+  for (int i = 0; i < nw; ++i) ss += red[0][i];
+  const float rstd = 1.0f / __builtin_sqrtf(ss / (float)a.cols + a.eps);
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int64_t col = 8 * ((int64_t)u * blockDim.x + tid);
+    if (col >= a.cols) continue;
+    float w[8];
+    if (a.w_dtype == MTQ_F32)
+      load8<float, VEC>(reinterpret_cast<const float *>(a.w), col, a.cols, w);
+    else
+      load8<T, VEC>(reinterpret_cast<const T *>(a.w), col, a.cols, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[u][j] = f[u][j] * rstd * w[j];
+  }
+  constexpr bool MX = KIND == MTQ_MXFP4 || KIND == MTQ_MXFP8;
+  float s = 1.f;
+  if constexpr (KIND == MTQ_FP8_TOKEN) {
+    float m = 0.f;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = fmaxf(m, mx_abs(f[u][j]));  // columns past the row are 0
+    m = wave_max(m);
+    if (lane == 0) red[1][wave] = m;
+    __syncthreads();
+    m = 0.f;
+    for (int i = 0; i < nw; ++i) m = fmaxf(m, red[1][i]);
+    float d = m / kE4M3Max;
+    d = d > 0.f ? d : 1.f;
+    if (tid == 0) reinterpret_cast<float *>(a.scale)[row] = d;
+    s = 1.0f / d;
+  } else if constexpr (KIND == MTQ_FP8_TENSOR) {
+    const Fp8Q p = make_fp8q(*a.amax);
+    s = p.s;
+    if (row == 0 && tid == 0) *reinterpret_cast<float *>(a.scale) = p.inv;
+  }
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int64_t col = 8 * ((int64_t)u * blockDim.x + tid);
+    if constexpr (MX) {
+      // a block's 4 lanes are all live or all past the row (cols % 32 == 0)
+      uint8_t *q = a.q + row * (KIND == MTQ_MXFP4 ? a.cols / 2 : a.cols);
+      mx_store8<KIND>(f[u], col, q, reinterpret_cast<uint8_t *>(a.scale) + row * (a.cols / 32), col < a.cols);
+    } else if (col < a.cols) {
+      fp8_store8<VEC>(f[u], s, col, a.cols, a.q + row * a.cols);
+    }
+  }
+}
+
+template <typename T, int KIND, bool VEC>
+int launch_norm(const NormArgs &a, int64_t rows, hipStream_t stream) {
+  // 256 lanes of 8 columns a group, up to 4 groups in registers; wider rows take more lanes
+  const int64_t groups = (a.cols + 7) / 8;
+  int threads = 256;
+  while (threads < 1024 && groups > 4 * threads) threads *= 2;
+  if (groups < 256) threads = (int)((groups + 63) / 64 * 64);
+  const int nv = (int)((groups + threads - 1) / threads);
+  const unsigned g = (unsigned)rows;
+  if (nv <= 1)
+    rms_norm_kernel<T, KIND, 1, VEC><<<g, threads, 0, stream>>>(a);
+  else if (nv <= 2)
+    rms_norm_kernel<T, KIND, 2, VEC><<<g, threads, 0, stream>>>(a);
+  else if (nv <= 4)
+    rms_norm_kernel<T, KIND, 4, VEC><<<g, threads, 0, stream>>>(a);
+  else
+    rms_norm_kernel<T, KIND, 8, VEC><<<g, threads, 0, stream>>>(a);
+  return host_check_launch();
+}
+template <typename T, int KIND> int launch_norm_v(const NormArgs &a, bool vec, int64_t rows, hipStream_t stream) {
+  return vec ? launch_norm<T, KIND, true>(a, rows, stream) : launch_norm<T, KIND, false>(a, rows, stream);
+}
+template <typename T> int launch_norm_k(const NormArgs &a, int kind, bool vec, int64_t rows, hipStream_t stream) {
+  switch (kind) {
+  case MTQ_MXFP4: return launch_norm_v<T, MTQ_MXFP4>(a, vec, rows, stream);
+  case MTQ_MXFP8: return launch_norm_v<T, MTQ_MXFP8>(a, vec, rows, stream);
+  case MTQ_FP8_TENSOR: return launch_norm_v<T, MTQ_FP8_TENSOR>(a, vec, rows, stream);
+  default: return launch_norm_v<T, MTQ_FP8_TOKEN>(a, vec, rows, stream);
+  }
+}
+
+// ---- quantising rows ---------------------------------------------------------------------------
+// MX and per-tensor FP8: 8 values a lane over all rows (a block's 4 lanes are neighbours).
+template <typename T, int KIND, bool VEC>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ x, int64_t xs, int64_t rows, int64_t cols,
+                                                          const float *__restrict__ amax, uint8_t *__restrict__ q,
+                                                          void *__restrict__ scale) {
+  const int64_t gpr = (cols + 7) / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / gpr, col = (i - row * gpr) * 8;
+  const bool live = row < rows;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (live) load8<T, VEC>(x + row * xs, col, cols, v);
+  if constexpr (KIND == MTQ_FP8_TENSOR) {
+    const Fp8Q p = make_fp8q(*amax);
+    if (i == 0) *reinterpret_cast<float *>(scale) = p.inv;
+    if (live) fp8_store8<VEC>(v, p.s, col, cols, q + row * cols);
+  } else {
+    mx_store8<KIND>(v, col, q + row * (KIND == MTQ_MXFP4 ? cols / 2 : cols),
+                    reinterpret_cast<uint8_t *>(scale) + row * (cols / 32), live);
+  }
+}
+
+// per token: one workgroup a row, two passes over it (the second from the caches)
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void token_quantize_kernel(const T *__restrict__ x, int64_t xs, int64_t cols,
+                                                             uint8_t *__restrict__ q, float *__restrict__ scale) {
+  __shared__ float red[4];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  x += row * xs;
+  float m = 0.f;
+  for (int64_t col = 8 * tid; col < cols; col += 2048) {
+    float v[8];
+    load8<T, VEC>(x, col, cols, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, mx_abs(v[j]));
+  }
+  m = wave_max(m);
+  if ((tid & 63) == 0) red[tid >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float d = m / kE4M3Max;
+  d = d > 0.f ? d : 1.f;
+  if (tid == 0) scale[row] = d;
+  const float s = 1.0f / d;
+  for (int64_t col = 8 * tid; col < cols; col += 2048) {
+    float v[8];
+    load8<T, VEC>(x, col, cols, v);
+    fp8_store8<VEC>(v, s, col, cols, q + row * cols);
+  }
+}
+
+template <typename T, bool VEC>
+int launch_quantize(const T *x, int64_t xs, int64_t rows, int64_t cols, int kind, const float *amax, uint8_t *q,
+                    void *scale, hipStream_t stream) {
+  const int64_t n = rows * ((cols + 7) / 8);
+  const unsigned g = (unsigned)((n + 255) / 256);
+  switch (kind) {
+  case MTQ_MXFP4: mx_quantize_kernel<T, MTQ_MXFP4, VEC><<<g, 256, 0, stream>>>(x, xs, rows, cols, amax, q, scale); break;
+  case MTQ_MXFP8: mx_quantize_kernel<T, MTQ_MXFP8, VEC><<<g, 256, 0, stream>>>(x, xs, rows, cols, amax, q, scale); break;
+  case MTQ_FP8_TENSOR:
+    mx_quantize_kernel<T, MTQ_FP8_TENSOR, VEC><<<g, 256, 0, stream>>>(x, xs, rows, cols, amax, q, scale);
+    break;
+  default: token_quantize_kernel<T, VEC><<<(unsigned)rows, 256, 0, stream>>>(x, xs, cols, q, (float *)scale); break;
+  }
+  return host_check_launch();
+}
+
+// ---- y = xq . W^T for few rows -------------------------------------------------------------------
+// v_mfma_scale_f32_16x16x128_f8f6f4, first operand 16 rows of W, second 16 rows of xq: lane
+// (r = lane & 15, g = lane >> 4) gives row r's block g of a 128-column step (E2M1: 16 bytes) and that
+// block's exponent byte; an E4M3 operand gives columns 16 g .. + 15 and 64 + 16 g .. + 15 of the step
+// (the layout was read off the instruction on the card), its lane's byte still being block g's.  The
+// result holds y^T: lane (r, g) has row r of xq and 4 consecutive rows 4 g .. of W.
+//
+// The call is bound by reading W once (17/32 byte per weight), so a workgroup is 8 waves that split K
+// over the same 16 * NT rows of W, every wave streaming its part straight into the operand registers
+// (nothing of W is shared, so LDS would only add a trip), and the 8 partial tiles meet in LDS at the end,
+// summed in wave order.
+struct SkinnyArgs {
+  const void *x;             // xq, or the 16-bit activations (FUSED)
+  const uint8_t *xsc;        // exponent bytes [M, K / 32] (MX formats)
+  const float *xf;           // factor per row (per token) or one (per tensor)
+  const uint8_t *w, *wsc;    // [N, K / 2], [N, K / 32]
+  const void *bias;
+  void *y;
+  int64_t xs;                // row stride of the 16-bit activations
+  int M, N, K;
+  int xf_stride;             // 1: a factor per row, 0: one
+  int bias_f32;
+};
+
+enum { kOpFp4 = 0, kOpFp8 = 1, kOpFused = 2 };
+constexpr int kSkinnyWaves = 8;
+
+template <typename T, int OP, int MT, int NT>
+__global__ __launch_bounds__(64 * kSkinnyWaves) void mx_skinny_kernel(SkinnyArgs a) {
+  constexpr int CH = MT * NT < 4 ? MT * NT : 4;  // tiles joined at a time
+  __shared__ f32x4 red[kSkinnyWaves][CH][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
+  const int nb = a.K / 32, steps = (nb + 3) / 4;
+  const int s0 = (int)((int64_t)steps * wave / kSkinnyWaves), s1 = (int)((int64_t)steps * (wave + 1) / kSkinnyWaves);
+  const uint8_t *wp[NT], *wsp[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int n = n0 + 16 * j + r < a.N ? n0 + 16 * j + r : a.N - 1;  // rows past N: never stored
+    wp[j] = a.w + (int64_t)n * (a.K / 2);
+    wsp[j] = a.wsc + (int64_t)n * nb;
+  }
+  int xrow[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xrow[i] = m0 + 16 * i + r < a.M ? m0 + 16 * i + r : a.M - 1;
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (int s = s0; s < s1; ++s) {
+    const int b = 4 * s + g;
+    const bool in = b < nb;  // the last step of a K that 128 does not divide
+    const int bc = in ? b : 0;
+    i32x8 wf[NT];
+    int ws[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      u32x4 d = *reinterpret_cast<const u32x4 *>(wp[j] + (int64_t)bc * 16);
+      ws[j] = wsp[j][bc];
+      if (!in) d = u32x4{0, 0, 0, 0};  // zero codes: whatever the other operand holds there is lost
+      if (!in) ws[j] = 127;
+      wf[j] = i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, 0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      i32x8 xf;
+      int xs = 127;
+      if constexpr (OP == kOpFused) {
+        const T *xp = reinterpret_cast<const T *>(a.x) + xrow[i] * a.xs + (int64_t)bc * 32;
+        float v[4][8];
+        float m = 0.f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          load8<T, true>(xp, 8 * t, 0, v[t]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m = fmaxf(m, mx_abs(v[t][j]));
+        }
+        float sc, un;
+        e8m0_scale(m, 6.0f, sc, un);
+        xs = (int)((__float_as_uint(un) >> 23) & 0xff);
+        xf = i32x8{(int)e2m1_codes8(v[0], un), (int)e2m1_codes8(v[1], un), (int)e2m1_codes8(v[2], un),
+                   (int)e2m1_codes8(v[3], un), 0, 0, 0, 0};
+      } else if constexpr (OP == kOpFp4) {
+        const uint8_t *xp = reinterpret_cast<const uint8_t *>(a.x) + (int64_t)xrow[i] * (a.K / 2);
+        const u32x4 d = *reinterpret_cast<const u32x4 *>(xp + (int64_t)bc * 16);
+        xs = a.xsc[(int64_t)xrow[i] * nb + bc];
+        xf = i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, 0, 0, 0, 0};
+      } else {
+        const uint8_t *xp = reinterpret_cast<const uint8_t *>(a.x) + (int64_t)xrow[i] * a.K;
+        const int k0 = 128 * s + 16 * g, k1 = k0 + 64;  // 16 columns each; past K: columns 0 .. 15
+        const u32x4 d = *reinterpret_cast<const u32x4 *>(xp + (k0 < a.K ? k0 : 0));
+        const u32x4 e = *reinterpret_cast<const u32x4 *>(xp + (k1 < a.K ? k1 : 0));
+        if (a.xsc) xs = a.xsc[(int64_t)xrow[i] * nb + bc];
+        xf = i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, (int)e.x, (int)e.y, (int)e.z, (int)e.w};
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], xf, acc[i][j], 4, OP == kOpFp8 ? 0 : 4, 0, ws[j],
+                                                                     0, xs);
+    }
+  }
+
+#pragma unroll
+  for (int c = 0; c < MT * NT; c += CH) {
+    if (c) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < CH; ++t) red[wave][t][lane] = acc[(c + t) / NT][(c + t) % NT];
+    __syncthreads();
+    if (tid < 64 * CH) {
+      const int t = wave, m = m0 + 16 * ((c + t) / NT) + r, n = n0 + 16 * ((c + t) % NT) + 4 * g;
+      f32x4 v = red[0][t][lane];
+#pragma unroll
+      for (int w = 1; w < kSkinnyWaves; ++w) v += red[w][t][lane];
+      if (m < a.M) {
+        const float f = a.xf ? a.xf[(int64_t)m * a.xf_stride] : 1.f;
+        T *y = reinterpret_cast<T *>(a.y) + (int64_t)m * a.N;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (n + k < a.N) {
+            float o = v[k] * f;
+            if (a.bias) o += a.bias_f32 ? reinterpret_cast<const float *>(a.bias)[n + k] : Elem<T>::ld(reinterpret_cast<const T *>(a.bias)[n + k]);
+            y[n + k] = Elem<T>::st(o);
+          }
+      }
+    }
+  }
+}
+
+template <typename T, int OP> int launch_skinny(const SkinnyArgs &a, hipStream_t stream) {
+  // rows of W a wave takes: more of them share one read of xq (worth it once there are workgroups
+  // enough to fill the card)
+  const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
+  const int tiles = (a.N + 15) / 16;
+  const dim3 g((unsigned)tiles, (unsigned)((a.M + 16 * mt - 1) / (16 * mt)));
+  if (mt == 1)
+    mx_skinny_kernel<T, OP, 1, 1><<<g, 64 * kSkinnyWaves, 0, stream>>>(a);
+  else if constexpr (OP != kOpFused) {
+    if (mt == 2)
+      mx_skinny_kernel<T, OP, 2, 1><<<g, 64 * kSkinnyWaves, 0, stream>>>(a);
+    else
+      mx_skinny_kernel<T, OP, 4, 1><<<g, 64 * kSkinnyWaves, 0, stream>>>(a);
+  }
+  return host_check_launch();
+}
+
+struct LinearWs {
+  size_t q, scale, bytes;  // offsets
+};
+LinearWs linear_ws(int64_t M, int64_t K, int kind) {
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  LinearWs w;
+  w.q = 0;
+  w.scale = up((size_t)M * (kind == MTQ_MXFP4 ? K / 2 : K));
+  w.bytes = w.scale + up(kind == MTQ_MXFP4 || kind == MTQ_MXFP8 ? (size_t)M * (K / 32) : kind == MTQ_FP8_TOKEN ? 4 * (size_t)M : 4);
+  return w;
+}
+// up to this many rows a wave quantises its part of x in its own registers (mx_skinny_kernel FUSED)
+constexpr int kFusedRows = 16;
+
+bool known_kind(int kind) { return kind >= MTQ_MXFP4 && kind <= MTQ_FP8_TOKEN; }
+bool is_mx(int kind) { return kind == MTQ_MXFP4 || kind == MTQ_MXFP8; }
+
+}  // namespace
+
+extern "C" {
+
+int mtq_mx_quantize(const void *x, int64_t row_stride, int64_t rows, int64_t cols, int dtype, int kind, const float *amax,
+                    uint8_t *q, void *scale, hipStream_t stream) {
+  if (!known_kind(kind)) return MTQ_ERR_FORMAT;
+  if (dtype != MTQ_BF16 && dtype != MTQ_F16 && dtype != MTQ_F32) return MTQ_ERR_DTYPE;
+  if (rows < 0 || cols < 1 || (is_mx(kind) && cols % 32) || (rows > 1 && row_stride < cols)) return MTQ_ERR_INVALID_ARG;
+  if (rows == 0) return MTQ_OK;
+  if (!x || !q || !scale || (kind == MTQ_FP8_TENSOR && !amax)) return MTQ_ERR_INVALID_ARG;
+  if (rows > (int64_t)INT32_MAX || rows * ((cols + 7) / 8) > (int64_t)INT32_MAX * 256) return MTQ_ERR_INVALID_ARG;
+  if ((uintptr_t)q % 8) return MTQ_ERR_INVALID_ARG;
+  const int es = dtype == MTQ_F32 ? 4 : 2;
+  const bool vec = al16(x) && cols % 8 == 0 && (rows == 1 || (row_stride * es) % 16 == 0);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    const T *p = reinterpret_cast<const T *>(x);
+    return vec ? launch_quantize<T, true>(p, row_stride, rows, cols, kind, amax, q, scale, stream)
+               : launch_quantize<T, false>(p, row_stride, rows, cols, kind, amax, q, scale, stream);
+  };
+  return dtype == MTQ_BF16 ? go(__bf16{}) : dtype == MTQ_F16 ? go(_Float16{}) : go(float{});
+}
+
+int mtq_rms_norm_quantize(const void *x, int64_t x_stride, const void *residual, int64_t r_stride, const void *weight,
+                          int weight_dtype, double eps, void *h, uint8_t *q, void *scale, const float *amax, int64_t rows,
+                          int64_t cols, int dtype, int kind, hipStream_t stream) {
+  if (!known_kind(kind)) return MTQ_ERR_FORMAT;
+  if (dtype != MTQ_BF16 && dtype != MTQ_F16 && dtype != MTQ_F32) return MTQ_ERR_DTYPE;
+  if (weight_dtype != dtype && weight_dtype != MTQ_F32) return MTQ_ERR_DTYPE;
+  if (rows < 0 || cols < 1 || cols > 65536 || (is_mx(kind) && cols % 32)) return MTQ_ERR_INVALID_ARG;
+  if (rows > (int64_t)INT32_MAX || (rows > 1 && (x_stride < cols || (residual && r_stride < cols)))) return MTQ_ERR_INVALID_ARG;
+  if (!(eps >= 0.0 && eps < 3.4e38)) return MTQ_ERR_INVALID_ARG;
+  if (rows == 0) return MTQ_OK;
+  if (!x || !weight || !q || !scale || (residual && !h) || (kind == MTQ_FP8_TENSOR && !amax)) return MTQ_ERR_INVALID_ARG;
+  if ((uintptr_t)q % 8) return MTQ_ERR_INVALID_ARG;
+  const int es = dtype == MTQ_F32 ? 4 : 2;
+  const bool vec = cols % 8 == 0 && al16(x) && al16(weight) && (rows == 1 || (x_stride * es) % 16 == 0) &&
+                   (!residual || (al16(residual) && al16(h) && (rows == 1 || (r_stride * es) % 16 == 0)));
+  const NormArgs a{x, residual, weight, h, q, scale, amax, x_stride, r_stride, cols, (float)eps, weight_dtype};
+  if (dtype == MTQ_BF16) return launch_norm_k<__bf16>(a, kind, vec, rows, stream);
+  if (dtype == MTQ_F16) return launch_norm_k<_Float16>(a, kind, vec, rows, stream);
+  return launch_norm_k<float>(a, kind, vec, rows, stream);
+}
+
+size_t mtq_mx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int kind, int x_dtype) {
+  if (M < 1 || N < 1 || K < 32 || !known_kind(kind) || x_dtype < 0) return 0;
+  return linear_ws(M, K, kind).bytes;
+}
+
+int mtq_mx_linear(const void *x, int64_t x_stride, int x_dtype, const void *x_scale, int kind, const float *amax,
+                  const uint8_t *w, const uint8_t *w_scale, const void *bias, int bias_dtype, void *y, int y_dtype, int64_t M,
+                  int64_t N, int64_t K, void *ws, size_t ws_bytes, hipStream_t stream) {
+  if (!known_kind(kind)) return MTQ_ERR_FORMAT;
+  if (y_dtype != MTQ_BF16 && y_dtype != MTQ_F16 && y_dtype != MTQ_F32) return MTQ_ERR_DTYPE;
+  if (x_dtype >= 0 && x_dtype != MTQ_BF16 && x_dtype != MTQ_F16 && x_dtype != MTQ_F32) return MTQ_ERR_DTYPE;
+  if (bias && bias_dtype != y_dtype && bias_dtype != MTQ_F32) return MTQ_ERR_DTYPE;
+  if (M < 0 || N < 1 || K < 32 || K % 32 || M > (1 << 24) || N > (1 << 24) || K > (1 << 24)) return MTQ_ERR_INVALID_ARG;
+  if (M == 0) return MTQ_OK;
+  if (!x || !w || !w_scale || !y || !al16(w)) return MTQ_ERR_INVALID_ARG;
+  if (x_dtype < 0 ? !x_scale || !al16(x) : (M > 1 && x_stride < K) || (kind == MTQ_FP8_TENSOR && !amax)) return MTQ_ERR_INVALID_ARG;
+  SkinnyArgs a{};
+  a.w = w, a.wsc = w_scale, a.bias = bias, a.y = y, a.M = (int)M, a.N = (int)N, a.K = (int)K;
+  a.bias_f32 = bias && bias_dtype == MTQ_F32;
+  const bool vec = x_dtype >= 0 && x_dtype != MTQ_F32 && al16(x) && (M == 1 || x_stride % 8 == 0);
+  const bool fused = vec && kind == MTQ_MXFP4 && M <= kFusedRows && x_dtype == y_dtype;
+  if (fused) {
+    a.x = x, a.xs = x_stride;
+    return y_dtype == MTQ_BF16 ? launch_skinny<__bf16, kOpFused>(a, stream) : launch_skinny<_Float16, kOpFused>(a, stream);
+  }
+  if (x_dtype >= 0) {
+    const LinearWs o = linear_ws(M, K, kind);
+    if (!ws || ws_bytes < o.bytes || !al16(ws)) return MTQ_ERR_INVALID_ARG;
+    uint8_t *q = (uint8_t *)ws + o.q;
+    void *sc = (uint8_t *)ws + o.scale;
+    const int st = mtq_mx_quantize(x, x_stride, M, K, x_dtype, kind, amax, q, sc, stream);
+    if (st != MTQ_OK) return st;
+    x = q, x_scale = sc;
+  }
+  a.x = x;
+  if (is_mx(kind)) {
+    a.xsc = (const uint8_t *)x_scale;
+  } else {
+    a.xf = (const float *)x_scale;
+    a.xf_stride = kind == MTQ_FP8_TOKEN;
+  }
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    return kind == MTQ_MXFP4 ? launch_skinny<T, kOpFp4>(a, stream) : launch_skinny<T, kOpFp8>(a, stream);
+  };
+  return y_dtype == MTQ_BF16 ? go(__bf16{}) : y_dtype == MTQ_F16 ? go(_Float16{}) : go(float{});
+}
+
+}  // extern "C"

@@ -1182,6 +1182,272 @@ void attention_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v
                "attention_fwd");
 }
 
+// ---- microscaled rows and products ------------------------------------------------------------
+namespace {
+
+// x as [rows, cols] with a row stride and contiguous columns, copied only where it is no such view
+at::Tensor as_rows(const at::Tensor &x) {
+  if (x.dim() == 2 && x.stride(1) == 1 && (x.size(0) < 2 || x.stride(0) >= x.size(1))) return x;
+  return (x.is_contiguous() ? x : x.contiguous()).view({-1, x.size(-1)});
+}
+
+int row_kind(int64_t kind, const char *what) {
+  TORCH_CHECK_VALUE(kind >= MTQ_MXFP4 && kind <= MTQ_FP8_TOKEN, what, ": unknown format");
+  return (int)kind;
+}
+
+const float *amax_of(const c10::optional<at::Tensor> &amax, int kind, const at::Tensor &x, const char *what) {
+  if (kind != MTQ_FP8_TENSOR) return nullptr;
+  TORCH_CHECK_VALUE(amax.has_value() && amax->defined(), what, ": the per-tensor FP8 format needs amax");
+  TORCH_CHECK_VALUE(amax->numel() == 1 && amax->scalar_type() == at::kFloat && amax->device() == x.device(), what,
+                    ": amax must be one fp32 value on the input's device");
+  return amax->data_ptr<float>();
+}
+
+// (codes, scales) of rows shaped like x
+std::pair<at::Tensor, at::Tensor> row_outputs(const at::Tensor &x, int kind, const char *what) {
+  std::vector<int64_t> qs(x.sizes().begin(), x.sizes().end()), ss = qs;
+  const int64_t cols = qs.back();
+  const bool mx = kind == MTQ_MXFP4 || kind == MTQ_MXFP8;
+  TORCH_CHECK_VALUE(!mx || cols % 32 == 0, what, ": the last dimension (", cols, ") must be a multiple of 32");
+  if (kind == MTQ_MXFP4) qs.back() = cols / 2;
+  ss.back() = mx ? cols / 32 : 1;
+  if (kind == MTQ_FP8_TENSOR) ss = {1};
+  return {at::empty(qs, x.options().dtype(kind == MTQ_MXFP4 ? at::kByte : at::kFloat8_e4m3fn)),
+          at::empty(ss, x.options().dtype(mx ? at::kByte : at::kFloat))};
+}
+
+void check_float_rows(const at::Tensor &x, const char *what) {
+  check_device(x, what);
+  const int dt = dtype_code(x.scalar_type());
+  TORCH_CHECK(dt == MTQ_BF16 || dt == MTQ_F16 || dt == MTQ_F32, what, ": bf16, fp16 or fp32 input expected, got ",
+              x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, what, ": at least one column expected");
+}
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> mx_quantize(const at::Tensor &x, int64_t kind_, const c10::optional<at::Tensor> &amax) {
+  const char *what = "mx_quantize";
+  const int kind = row_kind(kind_, what);
+  check_float_rows(x, what);
+  at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  auto [q, s] = row_outputs(x, kind, what);
+  const float *am = amax_of(amax, kind, x, what);
+  if (x.numel() == 0) return {q, s};
+  const at::Tensor v = as_rows(x);
+  check_status(mtq_mx_quantize(v.data_ptr(), v.stride(0), v.size(0), v.size(1), dtype_code(v.scalar_type()), kind, am,
+                               (uint8_t *)q.data_ptr(), s.data_ptr(), cur_stream(v)), what);
+  return {q, s};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_quantize(const at::Tensor &x, const c10::optional<at::Tensor> &residual,
+                                                                 const at::Tensor &weight, double eps, int64_t kind_,
+                                                                 const c10::optional<at::Tensor> &amax) {
+  const char *what = "rms_norm_quantize";
+  const int kind = row_kind(kind_, what);
+  check_float_rows(x, what);
+  const int64_t cols = x.size(-1);
+  TORCH_CHECK_VALUE(cols <= 65536, what, ": rows of more than 65536 columns are not supported");
+  TORCH_CHECK_VALUE(eps >= 0.0, what, ": eps must not be negative");
+  TORCH_CHECK_VALUE(weight.dim() == 1 && weight.numel() == cols && weight.device() == x.device(), what, ": weight must be [", cols,
+                    "] on the input's device");
+  TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat, what,
+              ": weight must have the input's dtype or fp32");
+  const bool has_r = residual.has_value() && residual->defined();
+  if (has_r)
+    TORCH_CHECK_VALUE(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type() &&
+                          residual->device() == x.device(),
+                      what, ": residual must have the input's shape, dtype and device");
+  at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  auto [q, s] = row_outputs(x, kind, what);
+  const float *am = amax_of(amax, kind, x, what);
+  at::Tensor h = has_r ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  if (x.numel() == 0) return {q, s, h};
+  const at::Tensor v = as_rows(x), w = weight.contiguous();
+  const at::Tensor r = has_r ? as_rows(*residual) : at::Tensor();
+  check_status(mtq_rms_norm_quantize(v.data_ptr(), v.stride(0), has_r ? r.data_ptr() : nullptr, has_r ? r.stride(0) : 0,
+                                     w.data_ptr(), dtype_code(w.scalar_type()), eps, has_r ? h.data_ptr() : nullptr,
+                                     (uint8_t *)q.data_ptr(), s.data_ptr(), am, v.size(0), cols, dtype_code(v.scalar_type()),
+                                     kind, cur_stream(v)), what);
+  return {q, s, h};
+}
+
+at::Tensor mx_linear(const at::Tensor &x, const c10::optional<at::Tensor> &x_scale, const at::Tensor &w, const at::Tensor &w_scale,
+                     const c10::optional<at::Tensor> &bias, int64_t kind_, const c10::optional<at::Tensor> &amax,
+                     c10::optional<at::ScalarType> out_dtype) {
+  const char *what = "mx_linear";
+  const int kind = row_kind(kind_, what);
+  const bool packed = x_scale.has_value() && x_scale->defined();
+  check_device(x, what);
+  TORCH_CHECK_VALUE(w.dim() == 2 && w.scalar_type() == at::kByte && w.device() == x.device(), what,
+                    ": weight must be [N, K / 2] packed E2M1 codes (uint8) on the input's device");
+  const int64_t N = w.size(0), K = 2 * w.size(1);
+  TORCH_CHECK_VALUE(N >= 1 && K >= 32 && K % 32 == 0, what, ": K (", K, ") must be a multiple of 32");
+  TORCH_CHECK_VALUE(w_scale.scalar_type() == at::kByte && w_scale.numel() == N * (K / 32) && w_scale.device() == x.device(), what,
+                    ": weight_scale must be [N, K / 32] E8M0 bytes (uint8) on the input's device");
+  TORCH_CHECK_VALUE(x.dim() >= 1, what, ": a row of inputs expected");
+  const at::ScalarType od = out_dtype.has_value() ? *out_dtype : packed ? at::kBFloat16 : x.scalar_type();
+  const int yd = dtype_code(od);
+  TORCH_CHECK(yd == MTQ_BF16 || yd == MTQ_F16 || yd == MTQ_F32, what, ": bf16, fp16 or fp32 output expected");
+  const int64_t xcols = packed && kind == MTQ_MXFP4 ? K / 2 : K;
+  TORCH_CHECK_VALUE(x.size(-1) == xcols, what, ": input has ", x.size(-1), " columns, the weight asks for ", xcols);
+  const int64_t M = x.numel() / xcols;
+  at::Tensor xs;
+  if (packed) {
+    const bool mx = kind == MTQ_MXFP4 || kind == MTQ_MXFP8;
+    TORCH_CHECK_VALUE(x.scalar_type() == (kind == MTQ_MXFP4 ? at::kByte : at::kFloat8_e4m3fn), what,
+                      ": quantised input has the wrong dtype for its format");
+    const int64_t want = mx ? M * (K / 32) : kind == MTQ_FP8_TOKEN ? M : 1;
+    TORCH_CHECK_VALUE(x_scale->scalar_type() == (mx ? at::kByte : at::kFloat) && x_scale->numel() == want &&
+                          x_scale->device() == x.device(),
+                      what, ": x_scale does not fit the format");
+    xs = x_scale->contiguous();
+  } else {
+    check_float_rows(x, what);
+  }
+  at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  const float *am = packed ? nullptr : amax_of(amax, kind, x, what);
+  at::Tensor b;
+  if (bias.has_value() && bias->defined()) {
+    TORCH_CHECK_VALUE(bias->numel() == N && bias->dim() == 1 && bias->device() == x.device() &&
+                          (bias->scalar_type() == od || bias->scalar_type() == at::kFloat),
+                      what, ": bias must be [N] in the output's dtype or fp32");
+    b = bias->contiguous();
+  }
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  at::Tensor y = at::empty(shape, x.options().dtype(od));
+  if (M == 0) return y;
+  auto dense16 = [](const at::Tensor &t) {  // contiguous and 16-byte aligned (a copy only where it is neither)
+    at::Tensor c = t.contiguous();
+    return (uintptr_t)c.data_ptr() % 16 ? c.clone() : c;
+  };
+  const at::Tensor v = packed ? dense16(x) : as_rows(x), wc = dense16(w), wsc = w_scale.contiguous();
+  const int xd = packed ? -1 : dtype_code(x.scalar_type());
+  const size_t nb = mtq_mx_linear_workspace_bytes(M, N, K, kind, xd);
+  at::Tensor ws = nb ? at::empty({(int64_t)nb}, x.options().dtype(at::kByte)) : at::Tensor();
+  check_status(mtq_mx_linear(v.data_ptr(), packed ? K : v.stride(0), xd, packed ? xs.data_ptr() : nullptr, kind, am,
+                             wc.data_ptr<uint8_t>(), wsc.data_ptr<uint8_t>(), b.defined() ? b.data_ptr() : nullptr,
+                             b.defined() ? dtype_code(b.scalar_type()) : 0, y.data_ptr(), yd, M, N, K,
+                             nb ? ws.data_ptr() : nullptr, nb, cur_stream(x)), what);
+  return y;
+}
+
+// ---- KV cache in 4 bits -------------------------------------------------------------------------
+namespace {
+
+struct KvCall {
+  mtq_kv_cache c;
+  at::Tensor start, len_q, len_k, table;
+  int batch;
+};
+
+// data: [pages, heads, page_size, D / 2] uint8, scale: [pages, heads, page_size, D / 16] e4m3, any strides
+// over the first three dimensions
+KvCall kv_call(const at::TensorList &t, const at::Tensor &start, const at::Tensor &len_q, const at::Tensor &len_k,
+               const at::Tensor &table, const at::Tensor &like, const char *what) {
+  KvCall k;
+  TORCH_CHECK_VALUE(t.size() == 6, what, ": k_data, k_scale, v_data, v_scale, k_amax, v_amax expected");
+  for (const at::Tensor &x : t) TORCH_CHECK_VALUE(x.is_cuda() && x.device() == like.device(), what, ": the cache must be on the input's device");
+  const int64_t D = 2 * t[0].size(-1);
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor &d = t[2 * i], &s = t[2 * i + 1], &a = t[4 + i];
+    TORCH_CHECK_VALUE(d.dim() == 4 && s.dim() == 4 && d.scalar_type() == at::kByte && s.element_size() == 1 &&
+                          d.sizes() == t[0].sizes() && s.size(0) == d.size(0) && s.size(1) == d.size(1) &&
+                          s.size(2) == d.size(2) && s.size(3) * 16 == D && d.stride(3) == 1 && s.stride(3) == 1,
+                      what, ": cache tensors must be [pages, kv_heads, page_size, head_dim / 2] codes and [.., head_dim / 16] scales");
+    TORCH_CHECK_VALUE(a.numel() == 1 && a.scalar_type() == at::kFloat, what, ": amax must be one fp32 value");
+    k.c.data[i] = d.data_ptr(), k.c.scale[i] = s.data_ptr(), k.c.amax[i] = a.data_ptr<float>();
+    for (int j = 0; j < 3; ++j) k.c.data_strides[i][j] = d.stride(j), k.c.scale_strides[i][j] = s.stride(j);
+  }
+  TORCH_CHECK_VALUE(t[0].size(0) <= INT32_MAX && t[0].size(1) <= 65535 && t[0].size(2) <= 32768, what, ": cache too large");
+  k.c.num_pages = (int)t[0].size(0), k.c.num_kv_heads = (int)t[0].size(1), k.c.page_size = (int)t[0].size(2), k.c.head_dim = (int)D;
+  const int64_t batch = len_q.numel();
+  auto ints = [&](const at::Tensor &x, const char *name) {
+    TORCH_CHECK_VALUE(x.scalar_type() == at::kInt && x.device() == like.device() && x.dim() == 1 && x.numel() == batch, what, ": ", name,
+                      " must hold one int32 per sequence on the input's device");
+    return x.contiguous();
+  };
+  k.start = ints(start, "b_start_loc"), k.len_q = ints(len_q, "b_seq_len"), k.len_k = ints(len_k, "b_seq_len_k");
+  TORCH_CHECK_VALUE(table.scalar_type() == at::kInt && table.device() == like.device() && table.dim() == 2 && table.size(0) == batch &&
+                        (batch == 0 || table.size(1) >= 1) && table.size(1) <= INT32_MAX,
+                    what, ": block_table must be [batch, pages per sequence] int32 on the input's device");
+  k.table = table.size(1) < 2 || (table.stride(1) == 1 && table.stride(0) >= table.size(1)) ? table : table.contiguous();
+  if (k.table.size(1) == 1 && k.table.stride(0) < 1) k.table = k.table.contiguous();
+  k.batch = (int)batch;
+  return k;
+}
+
+void check_kv_rows(const at::Tensor &x, const KvCall &k, const char *name, const char *what) {
+  TORCH_CHECK_VALUE(x.dim() == 3 && x.size(2) == k.c.head_dim && x.stride(2) == 1, what, ": ", name,
+                    " must be [tokens, heads, ", k.c.head_dim, "] with contiguous rows");
+}
+
+}  // namespace
+
+void kv_append(at::TensorList cache, const at::Tensor &k, const at::Tensor &v, const at::Tensor &start, const at::Tensor &len_q,
+               const at::Tensor &len_k, const at::Tensor &table, int64_t max_len) {
+  const char *what = "kv_append";
+  check_float_rows(k, what);
+  const KvCall c = kv_call(cache, start, len_q, len_k, table, k, what);
+  check_kv_rows(k, c, "k", what);
+  check_kv_rows(v, c, "v", what);
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(1) == c.c.num_kv_heads && v.scalar_type() == k.scalar_type() &&
+                        v.device() == k.device(), what, ": k and v must be alike, with the cache's heads");
+  TORCH_CHECK_VALUE(max_len >= 0 && max_len <= INT32_MAX, what, ": max_input_len");
+  at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(k.device());
+  const int64_t st[4] = {k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
+  check_status(mtq_kv_append(&c.c, k.data_ptr(), v.data_ptr(), st, k.size(0), c.table.data_ptr<int32_t>(), c.table.stride(0),
+                             (int)c.table.size(1), c.start.data_ptr<int32_t>(), c.len_q.data_ptr<int32_t>(),
+                             c.len_k.data_ptr<int32_t>(), c.batch, (int)max_len, dtype_code(k.scalar_type()), cur_stream(k)), what);
+}
+
+void kv_read(at::TensorList cache, at::Tensor k, at::Tensor v, const at::Tensor &start, const at::Tensor &len_q,
+             const at::Tensor &len_k, const at::Tensor &table, int64_t max_len) {
+  const char *what = "kv_read";
+  check_float_rows(k, what);
+  const KvCall c = kv_call(cache, start, len_q, len_k, table, k, what);
+  check_kv_rows(k, c, "k", what);
+  check_kv_rows(v, c, "v", what);
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(1) == c.c.num_kv_heads && v.scalar_type() == k.scalar_type() &&
+                        v.device() == k.device(), what, ": k and v must be alike, with the cache's heads");
+  TORCH_CHECK_VALUE(max_len >= 0 && max_len <= INT32_MAX, what, ": max_input_len");
+  at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(k.device());
+  const int64_t st[4] = {k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
+  check_status(mtq_kv_read(&c.c, k.data_ptr(), v.data_ptr(), st, k.size(0), c.table.data_ptr<int32_t>(), c.table.stride(0),
+                           (int)c.table.size(1), c.start.data_ptr<int32_t>(), c.len_q.data_ptr<int32_t>(),
+                           c.len_k.data_ptr<int32_t>(), c.batch, (int)max_len, dtype_code(k.scalar_type()), cur_stream(k)), what);
+}
+
+void kv_attention(at::TensorList cache, const at::Tensor &q, at::Tensor o, const at::Tensor &start, const at::Tensor &len_q,
+                  const at::Tensor &len_k, const at::Tensor &table, int64_t max_len_q, int64_t max_len_k, bool is_causal,
+                  double softmax_scale) {
+  const char *what = "kv_attention";
+  check_device(q, "q");
+  const int dt = dtype_code(q.scalar_type());
+  TORCH_CHECK(dt == MTQ_BF16 || dt == MTQ_F16, what, ": q must be bf16 or fp16");
+  const KvCall c = kv_call(cache, start, len_q, len_k, table, q, what);
+  check_kv_rows(q, c, "q", what);
+  check_kv_rows(o, c, "o", what);
+  TORCH_CHECK_VALUE(o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.device() == q.device(), what, ": o must be like q");
+  TORCH_CHECK_VALUE(q.size(1) >= 1 && q.size(1) % c.c.num_kv_heads == 0, what, ": num_q_heads ", q.size(1),
+                    " must be a multiple of num_kv_heads ", c.c.num_kv_heads);
+  TORCH_CHECK_VALUE(max_len_q >= 0 && max_len_q <= INT32_MAX && max_len_k >= 0, what, ": max_input_len / max_kv_len");
+  max_len_k = std::min<int64_t>(max_len_k, c.table.size(1) * c.c.page_size);
+  TORCH_CHECK_VALUE(max_len_k <= INT32_MAX / 2, what, ": block_table too wide");
+  at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
+  const int64_t st[4] = {q.stride(0), q.stride(1), o.stride(0), o.stride(1)};
+  const size_t nb = mtq_kv_attention_workspace_bytes(c.batch, (int)q.size(1), c.c.num_kv_heads, c.c.head_dim, (int)max_len_q,
+                                                     (int)max_len_k);
+  at::Tensor ws = nb ? at::empty({(int64_t)nb}, q.options().dtype(at::kByte)) : at::Tensor();
+  check_status(mtq_kv_attention(&c.c, q.data_ptr(), o.data_ptr(), st, q.size(0), (int)q.size(1), c.table.data_ptr<int32_t>(),
+                                c.table.stride(0), (int)c.table.size(1), c.start.data_ptr<int32_t>(),
+                                c.len_q.data_ptr<int32_t>(), c.len_k.data_ptr<int32_t>(), c.batch, (int)max_len_q,
+                                (int)max_len_k, is_causal, softmax_scale, dt, nb ? ws.data_ptr() : nullptr, nb, cur_stream(q)),
+               what);
+}
+
 TORCH_LIBRARY(modelopt_amd, m) {
   m.def("quantize_op(Tensor input, Tensor amax, int num_bits, int exponent_bits, bool unsigned, "
         "bool narrow_range) -> Tensor");
@@ -1242,6 +1508,17 @@ TORCH_LIBRARY(modelopt_amd, m) {
   m.def("attention_fwd(Tensor q, Tensor k, Tensor v, Tensor(a!) o, Tensor b_start_loc, Tensor b_seq_len, "
         "Tensor b_start_loc_k, Tensor b_seq_len_k, int max_len_q, bool is_causal, float softmax_scale, "
         "int p_qdq_mode, float p_qdq_scale) -> ()");
+  m.def("mx_quantize(Tensor x, int kind, Tensor? amax=None) -> (Tensor, Tensor)");
+  m.def("rms_norm_quantize(Tensor x, Tensor? residual, Tensor weight, float eps, int kind, Tensor? amax=None) -> "
+        "(Tensor, Tensor, Tensor)");
+  m.def("mx_linear(Tensor x, Tensor? x_scale, Tensor weight, Tensor weight_scale, Tensor? bias, int kind, "
+        "Tensor? amax=None, ScalarType? out_dtype=None) -> Tensor");
+  m.def("kv_append(Tensor[] cache, Tensor k, Tensor v, Tensor b_start_loc, Tensor b_seq_len, Tensor b_seq_len_k, "
+        "Tensor block_table, int max_input_len) -> ()");
+  m.def("kv_read(Tensor[] cache, Tensor(a!) k, Tensor(b!) v, Tensor b_start_loc, Tensor b_seq_len, Tensor b_seq_len_k, "
+        "Tensor block_table, int max_input_len) -> ()");
+  m.def("kv_attention(Tensor[] cache, Tensor q, Tensor(a!) o, Tensor b_start_loc, Tensor b_seq_len, Tensor b_seq_len_k, "
+        "Tensor block_table, int max_input_len, int max_kv_len, bool is_causal, float softmax_scale) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(modelopt_amd, CUDA, m) {
@@ -1285,6 +1562,12 @@ TORCH_LIBRARY_IMPL(modelopt_amd, CUDA, m) {
   m.impl("mse_sweep", &mse_sweep);
   m.impl("awq_clip_search", &awq_clip_search);
   m.impl("attention_fwd", &attention_fwd);
+  m.impl("mx_quantize", &mx_quantize);
+  m.impl("rms_norm_quantize", &rms_norm_quantize);
+  m.impl("mx_linear", &mx_linear);
+  m.impl("kv_append", &kv_append);
+  m.impl("kv_read", &kv_read);
+  m.impl("kv_attention", &kv_attention);
 }
 
 // the reference's "cpu" registration (tensor_quant.py:252-256), on the host kernels

@@ -1,0 +1,80 @@
+"""Quantised rows and their product with packed MXFP4 weights on gfx950 (csrc/mtq_mx.hip).
+
+Formats of a row of K values (``format``):
+
+=============  =================================  ==========================================
+``"mxfp4"``    ``uint8 [..., K / 2]`` E2M1 codes   ``uint8 [..., K / 32]`` E8M0 exponent bytes
+``"mxfp8"``    ``float8_e4m3fn [..., K]``          ``uint8 [..., K / 32]`` E8M0 exponent bytes
+``"fp8"``      ``float8_e4m3fn [..., K]``          ``float32 [1]`` factor (per tensor, from ``amax``)
+``"fp8_token"``  ``float8_e4m3fn [..., K]``        ``float32 [..., 1]`` factor per row
+=============  =================================  ==========================================
+
+The values are those of the quantizers' fake quant: ``"mxfp4"`` / ``"mxfp8"`` of the dynamic MX block
+quant (block 32), ``"fp8"`` of the per-tensor FP8 quant with a calibrated ``amax``.  Two E2M1 codes share a
+byte, the even column in the low half -- ``MXFP4QTensor``'s layout, so the ``weight`` / ``_scale`` of a
+compressed linear are ``mx_linear``'s ``weight`` / ``weight_scale`` as they are.
+
+Forward only: an input that needs a gradient is refused while gradients are recorded.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from ...._ext import ops
+
+__all__ = ["FORMATS", "mx_linear", "mx_quantize"]
+
+FORMATS = {"mxfp4": 0, "mxfp8": 1, "fp8": 2, "fp8_token": 3}
+
+
+def format_code(format: str) -> int:
+    kind = FORMATS.get(format)
+    if kind is None:
+        raise ValueError(f"format must be one of {sorted(FORMATS)}, got {format!r}")
+    return kind
+
+
+def refuse_grad(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError(f"{name}: forward only; call it under torch.no_grad() or on detached tensors")
+
+
+def check_device(name: str, x: torch.Tensor) -> None:
+    if not x.is_cuda:
+        raise RuntimeError(f"{name}: tensors must be on a ROCm (HIP) device; the MI355X-native path has no CPU kernels")
+
+
+def mx_quantize(x: torch.Tensor, format: str = "mxfp4", amax: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows ``x [..., K]`` (bf16, fp16 or fp32) -> ``(data, scale)`` in ``format``.
+
+    ``K`` must be a multiple of 32 for the MX formats; ``amax``: one fp32 value on the device, for
+    ``"fp8"``."""
+    kind = format_code(format)
+    check_device("mx_quantize", x)
+    refuse_grad("mx_quantize", x)
+    return ops().mx_quantize(x, kind, amax)
+
+
+def mx_linear(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    weight_scale: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    *,
+    format: str = "mxfp4",
+    x_scale: torch.Tensor | None = None,
+    amax: torch.Tensor | None = None,
+    out_dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """``quantised(x) @ W.T + bias`` with ``W [N, K]`` packed as MXFP4, fp32 sums, rounded once.
+
+    ``x [..., K]`` in bf16 / fp16 / fp32 is quantised to ``format`` on the way (``amax`` as in
+    ``mx_quantize``); with ``x_scale`` it is already quantised (``mx_quantize``'s or
+    ``rms_norm_quantize``'s pair).  ``weight uint8 [N, K / 2]``, ``weight_scale uint8`` with ``N * K / 32``
+    entries; ``bias [N]`` in the output's dtype or fp32.  ``out_dtype``: default ``x.dtype``, bf16 for a
+    quantised ``x``."""
+    kind = format_code(format)
+    check_device("mx_linear", x)
+    refuse_grad("mx_linear", x, bias)
+    return ops().mx_linear(x, x_scale, weight, weight_scale, bias, kind, amax, out_dtype)
