@@ -133,7 +133,7 @@ __device__ __forceinline__ void fp8_store8(const float (&v)[8], float s, int64_t
 }
 
 // ---- sums and maxima over a workgroup (its waves' results through LDS, in wave order) ----------
-__device__ __forceinline__ float wave_sum(float v) {
+__device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
@@ -150,6 +150,9 @@ __device__ __forceinline__ float wave_max(float v) {
 // Bound by HBM: x, r, h and a byte of codes per element, each touched once.  A workgroup takes one
 // row and keeps it in registers (NV groups of 8 columns a lane) between the sum of squares and the
 // output, so nothing is read twice.
+// A code flips where y or a block's maximum lies within its own error of a rounding border, so that
+// error is kept near half a unit of fp32: squares are summed in fp32 by eights and those sums in
+// double, rsqrt is a pair of floats, and x * w of 16-bit operands is exact before the one product.
 struct NormArgs {
   const void *x, *r, *w;
   void *h;
@@ -157,18 +160,19 @@ struct NormArgs {
   void *scale;
   const float *amax;
   int64_t xs, rs, cols;
-  float eps;
+  double eps;
   int w_dtype;
 };
 
 template <typename T, int KIND, int NV, bool VEC>
 __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
-  __shared__ float red[2][16];
+  __shared__ double red[16];
+  __shared__ float redm[16];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
   const T *x = reinterpret_cast<const T *>(a.x) + row * a.xs;
   float f[NV][8];
-  float ss = 0.f;
+  double ss = 0.0;
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
     const int64_t col = 8 * ((int64_t)u * blockDim.x + tid);
@@ -185,15 +189,18 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
       for (int j = 0; j < 8; ++j) f[u][j] = Elem<T>::ld(Elem<T>::st(f[u][j] + r[j]));
       store8<T, VEC>(reinterpret_cast<T *>(a.h) + row * a.cols, col, a.cols, f[u]);
     }
+    float s8 = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(f[u][j], f[u][j], ss);
+    for (int j = 0; j < 8; ++j) s8 = __builtin_fmaf(f[u][j], f[u][j], s8);
+    ss += (double)s8;
   }
   ss = wave_sum(ss);
-  if (lane == 0) red[0][wave] = ss;
+  if (lane == 0) red[wave] = ss;
   __syncthreads();
-  ss = 0.f;
-  for (int i = 0; i < nw; ++i) ss += red[0][i];
-  const float rstd = 1.0f / __builtin_sqrtf(ss / (float)a.cols + a.eps);
+  ss = 0.0;
+  for (int i = 0; i < nw; ++i) ss += red[i];
+  const double rd = 1.0 / __builtin_sqrt(ss / (double)a.cols + a.eps);
+  const float rh = (float)rd, rl = (float)(rd - (double)rh);
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
     const int64_t col = 8 * ((int64_t)u * blockDim.x + tid);
@@ -204,7 +211,10 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
     else
       load8<T, VEC>(reinterpret_cast<const T *>(a.w), col, a.cols, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[u][j] = f[u][j] * rstd * w[j];
+    for (int j = 0; j < 8; ++j) {
+      const float p = f[u][j] * w[j];
+      f[u][j] = __builtin_fmaf(p, rh, p * rl);
+    }
   }
   constexpr bool MX = KIND == MTQ_MXFP4 || KIND == MTQ_MXFP8;
   float s = 1.f;
@@ -215,10 +225,10 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) m = fmaxf(m, mx_abs(f[u][j]));  // columns past the row are 0
     m = wave_max(m);
-    if (lane == 0) red[1][wave] = m;
+    if (lane == 0) redm[wave] = m;
     __syncthreads();
     m = 0.f;
-    for (int i = 0; i < nw; ++i) m = fmaxf(m, red[1][i]);
+    for (int i = 0; i < nw; ++i) m = fmaxf(m, redm[i]);
     float d = m / kE4M3Max;
     d = d > 0.f ? d : 1.f;
     if (tid == 0) reinterpret_cast<float *>(a.scale)[row] = d;
@@ -487,22 +497,346 @@ template <typename T, int OP> int launch_skinny(const SkinnyArgs &a, hipStream_t
   return host_check_launch();
 }
 
-struct LinearWs {
-  size_t q, scale, bytes;  // offsets
+// ---- y = xq . W^T for many rows ------------------------------------------------------------------
+// Bound by the matrix cores (16x16x128: 16 cycles of E2M1 x E2M1, 32 with an E4M3 operand).  A
+// workgroup is 8 waves on a 256 x 256 tile of y, a wave on 128 rows of xq x 64 of W; K advances by
+// BK = 256 columns (E2M1) or 128 (E4M3 rows of xq), so a K tile is 128 bytes of each xq row in LDS and
+// as many MFMA cycles in both forms.  The schedule is that of the 16-bit search kernel
+// (mtq_awq_gemm.hip, awq_search_pp_kernel): operands come by LDS-DMA into two buffers of four
+// half-tiles, a K tile is four phases of a 64 x 32 quadrant each, every phase issues the DMA of one
+// half-tile two to five phases ahead and waits with a counted vmcnt, and waves 4-7 run one barrier
+// behind waves 0-3, so that one wave of a SIMD reads LDS while the other multiplies.
+// The exponent bytes are laid out by K tile first ([K tile][row][BK / 32], zero past the matrix; one
+// small pass per operand), so a tile's are two DMAs a wave into a ring of three; a lane's exponents of
+// both 128-column steps are one 16-bit read, its blocks of a K tile being 2 g and 2 g + 1 (the
+// order in which the columns of a K tile are multiplied is free).
+// LDS rows are 16-byte chunks stored at chunk ^ (row bits) (the XOR is applied to the global
+// address): conflict-free fragment reads.
+// Columns past K (K % BK != 0): chunks there are read from the row's first chunk of the tile, and
+// their exponents are 2^-127 on both sides, so what they add vanishes (below 2^-230).
+struct PpArgs {
+  const uint8_t *x, *w, *xsc, *wsc;  // xsc / wsc: tiled exponents; xsc null: all 2^0
+  const float *xf;
+  const void *bias;
+  void *y;
+  int M, N, K, tiles_m, tiles_n, xf_stride, bias_f32;
 };
-LinearWs linear_ws(int64_t M, int64_t K, int kind) {
+constexpr int kPpTile = 256, kPpThreads = 512;
+constexpr int pp_bk(bool f8) { return f8 ? 128 : 256; }
+
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t wave_rsrc(const void *base, uint32_t bytes) {
+  const uint64_t a = (uint64_t)base;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc((void *)(((uint64_t)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+// buffer_load ... lds: BYTES (4 or 16) a lane to lds + lane * BYTES (the builtin exists in the device pass only)
+#if defined(__HIP_DEVICE_COMPILE__)
+#define MX_DMA(rsrc, lds, bytes, voff, soff) \
+  __builtin_amdgcn_raw_ptr_buffer_load_lds((rsrc), (__attribute__((address_space(3))) void *)(lds), bytes, (voff), (soff), 0, 0)
+#else
+#define MX_DMA(rsrc, lds, bytes, voff, soff) ((void)(rsrc), (void)(lds), (void)(voff), (void)(soff))
+#endif
+
+template <bool F8> __device__ __forceinline__ f32x4 pp_mma(const i32x8 &w, const i32x8 &x, f32x4 c, int s, int ws, int xs) {
+  if (F8) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, 0, 0, ws, 0, xs);
+  return s ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, 4, 1, ws, 1, xs)
+           : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, 4, 0, ws, 0, xs);
+}
+
+template <typename T, bool F8>
+__global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
+  constexpr int BK = pp_bk(F8), NB = BK / 32;         // K tile, its blocks
+  constexpr int AH = 128 * 128, BH = 128 * (BK / 2);  // bytes of a half-tile of xq, of W
+  constexpr int BUF = 2 * AH + 2 * BH, SOP = kPpTile * NB, SBUF = 2 * SOP;
+  constexpr int AU = 2, BU = F8 ? 1 : 2, SU = F8 ? 1 : 2;  // DMAs a wave: half-tiles, a tile's exponents
+  constexpr int CNT = 2 * AU + 2 * BU + SU;
+  constexpr int NS = F8 ? 1 : 2;                       // 128-column steps of a K tile
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF + 3 * SBUF];
+  unsigned char *const sring = lds + 2 * BUF;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int grp = wave >> 2, wn = wave & 3, fr = lane & 15, fq = lane >> 4;
+
+  // tile order: units of 8 row tiles x 4 column tiles on one XCD at a time (its L2 then holds 12
+  // operand panels for 32 workgroups), consecutive units on the 8 XCDs
+  int tm, tn;
+  {
+    const int orig = blockIdx.x, xcd = orig % 8, li = orig / 8;
+    const int slot = li % 32, u = (li / 32) * 8 + xcd;
+    const int mgn = (p.tiles_m + 7) / 8;
+    tm = (u % mgn) * 8 + slot % 8;
+    tn = (u / mgn) * 4 + slot / 8;
+    if (tm >= p.tiles_m || tn >= p.tiles_n) return;  // the whole workgroup, before any barrier
+  }
+  const int64_t m0 = (int64_t)tm * kPpTile, n0 = (int64_t)tn * kPpTile;
+  const int xrow = F8 ? p.K : p.K / 2, wrow = p.K / 2;  // bytes of a row
+  const int nt = (p.K + BK - 1) / BK;
+  const int rows_x = (int)(p.M - m0 < kPpTile ? p.M - m0 : kPpTile), rows_w = (int)(p.N - n0 < kPpTile ? p.N - n0 : kPpTile);
+
+  // ---- DMA sources.  xq half h, round u: LDS row rr = u * 64 + wave * 8 + lane / 8, chunk slot lane % 8;
+  // W half h: the same, or (64-byte rows) rr = wave * 16 + lane / 4, slot lane % 4.  Rows past the
+  // matrix re-read its last one (their results are not stored).
+  unsigned a_off[2][AU], b_off[2][BU];
+  unsigned a_tail, b_tail;  // what to step back by where the chunk lies past K in the last tile
+  {
+    const int a_chunk = (lane & 7) ^ (((wave * 8 + (lane >> 3)) >> 1) & 7);
+    const int b_chunk = F8 ? (lane & 3) ^ (((lane >> 2) >> 2) & 3) : a_chunk;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int u = 0; u < AU; ++u) {
+        const int rr = u * 64 + wave * 8 + (lane >> 3), row = (rr >> 6) * 128 + h * 64 + (rr & 63);
+        a_off[h][u] = (unsigned)(row < rows_x ? row : rows_x - 1) * (unsigned)xrow + a_chunk * 16;
+      }
+#pragma unroll
+      for (int u = 0; u < BU; ++u) {
+        const int rr = F8 ? wave * 16 + (lane >> 2) : u * 64 + wave * 8 + (lane >> 3);
+        const int row = (rr >> 5) * 64 + h * 32 + (rr & 31);
+        b_off[h][u] = (unsigned)(row < rows_w ? row : rows_w - 1) * (unsigned)wrow + b_chunk * 16;
+      }
+    }
+    const int k0 = (nt - 1) * BK;  // a chunk: 16 columns of E4M3, 32 of E2M1
+    a_tail = k0 + a_chunk * (F8 ? 16 : 32) < p.K ? 0 : a_chunk * 16;
+    b_tail = k0 + b_chunk * 32 < p.K ? 0 : b_chunk * 16;
+  }
+  const __amdgpu_buffer_rsrc_t xr = wave_rsrc(p.x + m0 * xrow, (uint32_t)rows_x * (uint32_t)xrow);
+  const __amdgpu_buffer_rsrc_t wr = wave_rsrc(p.w + n0 * wrow, (uint32_t)rows_w * (uint32_t)wrow);
+  const int xpad = p.tiles_m * kPpTile, wpad = p.tiles_n * kPpTile;  // rows of the tiled exponents
+  const uint8_t *const xs_base = p.xsc ? p.xsc + m0 * NB : p.wsc + n0 * NB;  // no exponents: any (not read)
+  const int xs_step = (p.xsc ? xpad : wpad) * NB, ws_step = wpad * NB;
+  const __amdgpu_buffer_rsrc_t xsr = wave_rsrc(xs_base, (uint32_t)(nt - 1) * xs_step + SOP);
+  const __amdgpu_buffer_rsrc_t wsr = wave_rsrc(p.wsc + n0 * NB, (uint32_t)(nt - 1) * ws_step + SOP);
+
+  auto load_a = [&](int h, int t) {
+    unsigned char *dst = lds + (t & 1) * BUF + h * AH + wave * 1024;
+    const int tt = t < nt ? t : nt - 1;  // past the end: harmless re-loads
+    const uint32_t soff = __builtin_amdgcn_readfirstlane((uint32_t)tt * 128);
+    const unsigned back = tt == nt - 1 ? a_tail : 0;
+#pragma unroll
+    for (int u = 0; u < AU; ++u) MX_DMA(xr, dst + u * 8192, 16, a_off[h][u] - back, soff);
+  };
+  auto load_b = [&](int h, int t) {
+    unsigned char *dst = lds + (t & 1) * BUF + 2 * AH + h * BH + wave * 1024;
+    const int tt = t < nt ? t : nt - 1;
+    const uint32_t soff = __builtin_amdgcn_readfirstlane((uint32_t)tt * (BK / 2));
+    const unsigned back = tt == nt - 1 ? b_tail : 0;
+#pragma unroll
+    for (int u = 0; u < BU; ++u) MX_DMA(wr, dst + u * 8192, 16, b_off[h][u] - back, soff);
+  };
+  auto load_s = [&](int t, int slot) {
+    unsigned char *dst = sring + slot * SBUF;
+    const int tt = t < nt ? t : nt - 1;
+    const uint32_t sx = __builtin_amdgcn_readfirstlane((uint32_t)tt * xs_step), sw = __builtin_amdgcn_readfirstlane((uint32_t)tt * ws_step);
+    if constexpr (F8) {  // 1 KiB each: waves 0-3 and 4-7
+      if (wave < 4)
+        MX_DMA(xsr, dst + wave * 256, 4, (unsigned)(wave * 256 + lane * 4), sx);
+      else
+        MX_DMA(wsr, dst + SOP + (wave - 4) * 256, 4, (unsigned)((wave - 4) * 256 + lane * 4), sw);
+    } else {
+      MX_DMA(xsr, dst + wave * 256, 4, (unsigned)(wave * 256 + lane * 4), sx);
+      MX_DMA(wsr, dst + SOP + wave * 256, 4, (unsigned)(wave * 256 + lane * 4), sw);
+    }
+  };
+
+  // ---- fragments.  E2M1 operand, step s: block 2 fq + s (E4M3 form: block fq of 4); E4M3 operand:
+  // columns 16 fq .. and 64 + 16 fq ..
+  const int sw8 = (lane >> 1) & 7, sw4 = (lane >> 2) & 3;
+  auto ld4 = [&](const unsigned char *q) -> i32x8 {
+    const u32x4 d = *reinterpret_cast<const u32x4 *>(q);
+    return i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, 0, 0, 0, 0};
+  };
+  auto read_a = [&](const unsigned char *buf, int i, int s) -> i32x8 {
+    const unsigned char *row = buf + (i >> 2) * AH + (grp * 64 + (i & 3) * 16 + fr) * 128;
+    if constexpr (F8) {
+      const u32x4 d = *reinterpret_cast<const u32x4 *>(row + ((fq ^ sw8) << 4));
+      const u32x4 e = *reinterpret_cast<const u32x4 *>(row + (((4 + fq) ^ sw8) << 4));
+      return i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, (int)e.x, (int)e.y, (int)e.z, (int)e.w};
+    } else {
+      return ld4(row + (((2 * fq + s) ^ sw8) << 4));
+    }
+  };
+  auto read_b = [&](const unsigned char *buf, int j, int s) -> i32x8 {
+    const unsigned char *row = buf + 2 * AH + (j >> 1) * BH + (wn * 32 + (j & 1) * 16 + fr) * (BK / 2);
+    return ld4(row + (F8 ? (fq ^ sw4) << 4 : ((2 * fq + s) ^ sw8) << 4));
+  };
+  auto read_s = [&](const unsigned char *base, int row) -> int {
+    if constexpr (F8) return base[row * NB + fq];
+    return *reinterpret_cast<const uint16_t *>(base + row * NB + 2 * fq);
+  };
+
+  f32x4 acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // stream order of the DMAs: per K tile t  B1(t+1) | A1(t+1) | B0(t+2) | S(t+2) A0(t+2); CNT are those
+  // issued after the half-tile that the next phase reads
+  load_b(0, 0);
+  load_s(0, 0);
+  load_a(0, 0);
+  load_b(1, 0);
+  load_a(1, 0);
+  load_b(0, 1);
+  load_s(1, 1);
+  load_a(0, 1);
+  wait_vm<CNT>();
+  __builtin_amdgcn_s_barrier();
+  if (grp == 1) __builtin_amdgcn_s_barrier();  // one barrier behind
+
+  i32x8 af[4][NS], b0f[2][NS], b1f[2][NS];
+  int sa[4], sb0[2], sb1[2];
+  int slot = 0;
+  for (int t = 0; t < nt; ++t) {
+    const unsigned char *cur = lds + (t & 1) * BUF;
+    const unsigned char *sx = sring + slot * SBUF, *sw = sx + SOP;
+    const int slot2 = slot == 0 ? 2 : slot - 1;  // (t + 2) % 3
+    // rows without exponents: 2^0, past K 2^-127
+    const int unit = F8 && !p.xsc ? ((t == nt - 1 && (nt - 1) * BK + 32 * fq >= p.K) ? 0 : 127) : 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int mq = (q == 0 || q == 1) ? 0 : 1;
+      const int nq = (q == 1 || q == 2) ? 1 : 0;
+      if (q == 0 || q == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int s = 0; s < NS; ++s) af[i][s] = read_a(cur, 4 * mq + i, s);
+          sa[i] = F8 && !p.xsc ? unit : read_s(sx, grp * 128 + 16 * (4 * mq + i) + fr);
+        }
+      }
+      if (q == 0) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int s = 0; s < NS; ++s) b0f[j][s] = read_b(cur, j, s);
+          sb0[j] = read_s(sw, wn * 64 + 16 * j + fr);
+        }
+      }
+      if (q == 1) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int s = 0; s < NS; ++s) b1f[j][s] = read_b(cur, 2 + j, s);
+          sb1[j] = read_s(sw, wn * 64 + 16 * (2 + j) + fr);
+        }
+      }
+      if (q == 0) load_b(1, t + 1);
+      if (q == 1) load_a(1, t + 1);
+      if (q == 2) load_b(0, t + 2);
+      if (q == 3) {
+        load_s(t + 2, slot2);
+        load_a(0, t + 2);
+      }
+      wait_vm<CNT>();
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            acc[4 * mq + i][2 * nq + j] =
+                pp_mma<F8>(nq ? b1f[j][s] : b0f[j][s], af[i][s], acc[4 * mq + i][2 * nq + j], s, nq ? sb1[j] : sb0[j], sa[i]);
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_s_barrier();
+    }
+    slot = slot == 2 ? 0 : slot + 1;
+  }
+  if (grp == 0) __builtin_amdgcn_s_barrier();  // balance the stagger
+  wait_vm<0>();  // the re-loads past the end land before the workgroup's LDS is given away
+
+  // ---- lane: y[m][n .. n + 3], m = 16 i + fr, n = 16 j + 4 fq of the wave's 128 x 64
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t m = m0 + grp * 128 + 16 * i + fr;
+    if (m >= p.M) continue;
+    const float f = p.xf ? p.xf[m * p.xf_stride] : 1.f;
+    T *y = reinterpret_cast<T *>(p.y) + m * p.N;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t n = n0 + wn * 64 + 16 * j + 4 * fq;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (n + k < p.N) {
+          float o = acc[i][j][k] * f;
+          if (p.bias) o += p.bias_f32 ? reinterpret_cast<const float *>(p.bias)[n + k] : Elem<T>::ld(reinterpret_cast<const T *>(p.bias)[n + k]);
+          y[n + k] = Elem<T>::st(o);
+        }
+    }
+  }
+}
+
+// exponents [rows][nb] -> [K tile][rows padded to 256][NB], 0 past the matrix
+template <int NB>
+__global__ __launch_bounds__(256) void mx_tile_scales_kernel(const uint8_t *__restrict__ s, int rows, int nb, int pad, int nt,
+                                                             uint8_t *__restrict__ o) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / nt;
+  const int t = (int)(i - row * nt);
+  if (row >= pad) return;
+  uint32_t w[NB / 4];
+#pragma unroll
+  for (int k = 0; k < NB / 4; ++k) {
+    w[k] = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int b = t * NB + 4 * k + j;
+      if (row < rows && b < nb) w[k] |= (uint32_t)s[row * nb + b] << (8 * j);
+    }
+  }
+  uint32_t *d = reinterpret_cast<uint32_t *>(o + ((int64_t)t * pad + row) * NB);
+#pragma unroll
+  for (int k = 0; k < NB / 4; ++k) d[k] = w[k];
+}
+
+bool is_mx(int kind) { return kind == MTQ_MXFP4 || kind == MTQ_MXFP8; }
+
+// up to this many rows a wave quantises its part of x in its own registers (mx_skinny_kernel FUSED)
+constexpr int kFusedRows = 16;
+// rows up to which the weight-streaming kernel is taken
+constexpr int kSkinnyRows = 64;
+bool use_pp(int64_t M, int64_t N, int64_t K) {
+  // 32-bit offsets inside a 256-row panel and inside the tiled exponents
+  const int64_t pad = (M > N ? M : N) + kPpTile;
+  return M > kSkinnyRows && K <= (1 << 22) && pad * (K / 32 + 8) < (1ll << 31);
+}
+struct LinearWs {
+  size_t q, scale, xt, wt, bytes;  // offsets: codes and scales of x, both operands' tiled exponents
+};
+LinearWs linear_ws(int64_t M, int64_t N, int64_t K, int kind, bool quantise) {
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   LinearWs w;
   w.q = 0;
-  w.scale = up((size_t)M * (kind == MTQ_MXFP4 ? K / 2 : K));
-  w.bytes = w.scale + up(kind == MTQ_MXFP4 || kind == MTQ_MXFP8 ? (size_t)M * (K / 32) : kind == MTQ_FP8_TOKEN ? 4 * (size_t)M : 4);
+  w.scale = quantise ? up((size_t)M * (kind == MTQ_MXFP4 ? K / 2 : K)) : 0;
+  w.xt = w.scale + (quantise ? up(is_mx(kind) ? (size_t)M * (K / 32) : kind == MTQ_FP8_TOKEN ? 4 * (size_t)M : 4) : 0);
+  w.wt = w.bytes = w.xt;
+  if (use_pp(M, N, K)) {
+    const int bk = pp_bk(kind != MTQ_MXFP4);
+    const size_t nt = (size_t)((K + bk - 1) / bk);
+    w.wt = w.xt + (is_mx(kind) ? nt * up(M) * (bk / 32) : 0);
+    w.bytes = w.wt + nt * up(N) * (bk / 32);
+  }
   return w;
 }
-// up to this many rows a wave quantises its part of x in its own registers (mx_skinny_kernel FUSED)
-constexpr int kFusedRows = 16;
+template <bool F8> int launch_tile_scales(const uint8_t *s, int rows, int K, uint8_t *o, hipStream_t stream) {
+  constexpr int BK = pp_bk(F8);
+  const int nt = (K + BK - 1) / BK, pad = (rows + 255) / 256 * 256;
+  mx_tile_scales_kernel<BK / 32><<<(unsigned)(((int64_t)pad * nt + 255) / 256), 256, 0, stream>>>(s, rows, K / 32, pad, nt, o);
+  return host_check_launch();
+}
+template <typename T, bool F8> int launch_pp(PpArgs a, hipStream_t stream) {
+  a.tiles_m = (a.M + kPpTile - 1) / kPpTile, a.tiles_n = (a.N + kPpTile - 1) / kPpTile;
+  const int64_t units = (int64_t)((a.tiles_m + 7) / 8) * ((a.tiles_n + 3) / 4);
+  mx_pp_kernel<T, F8><<<(unsigned)((units + 7) / 8 * 8 * 32), kPpThreads, 0, stream>>>(a);
+  return host_check_launch();
+}
 
 bool known_kind(int kind) { return kind >= MTQ_MXFP4 && kind <= MTQ_FP8_TOKEN; }
-bool is_mx(int kind) { return kind == MTQ_MXFP4 || kind == MTQ_MXFP8; }
 
 }  // namespace
 
@@ -543,15 +877,15 @@ int mtq_rms_norm_quantize(const void *x, int64_t x_stride, const void *residual,
   const int es = dtype == MTQ_F32 ? 4 : 2;
   const bool vec = cols % 8 == 0 && al16(x) && al16(weight) && (rows == 1 || (x_stride * es) % 16 == 0) &&
                    (!residual || (al16(residual) && al16(h) && (rows == 1 || (r_stride * es) % 16 == 0)));
-  const NormArgs a{x, residual, weight, h, q, scale, amax, x_stride, r_stride, cols, (float)eps, weight_dtype};
+  const NormArgs a{x, residual, weight, h, q, scale, amax, x_stride, r_stride, cols, eps, weight_dtype};
   if (dtype == MTQ_BF16) return launch_norm_k<__bf16>(a, kind, vec, rows, stream);
   if (dtype == MTQ_F16) return launch_norm_k<_Float16>(a, kind, vec, rows, stream);
   return launch_norm_k<float>(a, kind, vec, rows, stream);
 }
 
 size_t mtq_mx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int kind, int x_dtype) {
-  if (M < 1 || N < 1 || K < 32 || !known_kind(kind) || x_dtype < 0) return 0;
-  return linear_ws(M, K, kind).bytes;
+  if (M < 1 || N < 1 || K < 32 || !known_kind(kind)) return 0;
+  return linear_ws(M, N, K, kind, x_dtype >= 0).bytes;
 }
 
 int mtq_mx_linear(const void *x, int64_t x_stride, int x_dtype, const void *x_scale, int kind, const float *amax,
@@ -574,9 +908,9 @@ int mtq_mx_linear(const void *x, int64_t x_stride, int x_dtype, const void *x_sc
     a.x = x, a.xs = x_stride;
     return y_dtype == MTQ_BF16 ? launch_skinny<__bf16, kOpFused>(a, stream) : launch_skinny<_Float16, kOpFused>(a, stream);
   }
+  const LinearWs o = linear_ws(M, N, K, kind, x_dtype >= 0);
+  if (o.bytes && (!ws || ws_bytes < o.bytes || !al16(ws))) return MTQ_ERR_INVALID_ARG;
   if (x_dtype >= 0) {
-    const LinearWs o = linear_ws(M, K, kind);
-    if (!ws || ws_bytes < o.bytes || !al16(ws)) return MTQ_ERR_INVALID_ARG;
     uint8_t *q = (uint8_t *)ws + o.q;
     void *sc = (uint8_t *)ws + o.scale;
     const int st = mtq_mx_quantize(x, x_stride, M, K, x_dtype, kind, amax, q, sc, stream);
@@ -589,6 +923,20 @@ int mtq_mx_linear(const void *x, int64_t x_stride, int x_dtype, const void *x_sc
   } else {
     a.xf = (const float *)x_scale;
     a.xf_stride = kind == MTQ_FP8_TOKEN;
+  }
+  if (use_pp(M, N, K)) {
+    const bool f8 = kind != MTQ_MXFP4;
+    uint8_t *xt = is_mx(kind) ? (uint8_t *)ws + o.xt : nullptr, *wt = (uint8_t *)ws + o.wt;
+    int st = MTQ_OK;
+    if (xt) st = f8 ? launch_tile_scales<true>(a.xsc, a.M, a.K, xt, stream) : launch_tile_scales<false>(a.xsc, a.M, a.K, xt, stream);
+    if (st == MTQ_OK) st = f8 ? launch_tile_scales<true>(w_scale, a.N, a.K, wt, stream) : launch_tile_scales<false>(w_scale, a.N, a.K, wt, stream);
+    if (st != MTQ_OK) return st;
+    const PpArgs p{(const uint8_t *)x, w, xt, wt, a.xf, bias, y, a.M, a.N, a.K, 0, 0, a.xf_stride, a.bias_f32};
+    auto go = [&](auto t) {
+      using T = decltype(t);
+      return f8 ? launch_pp<T, true>(p, stream) : launch_pp<T, false>(p, stream);
+    };
+    return y_dtype == MTQ_BF16 ? go(__bf16{}) : y_dtype == MTQ_F16 ? go(_Float16{}) : go(float{});
   }
   auto go = [&](auto t) {
     using T = decltype(t);
