@@ -546,6 +546,23 @@ template <bool F8> __device__ __forceinline__ f32x4 pp_mma(const i32x8 &w, const
            : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, 4, 0, ws, 0, xs);
 }
 
+// one lane's 8 values of a row of y
+template <typename T> __device__ __forceinline__ void pp_store8(T *y, const float (&v)[8], int64_t n, int N, bool vec) {
+  if (vec && n + 8 <= N) {
+#pragma unroll
+    for (int k = 0; k < 8; k += Vec<T>::N) {
+      Vec<T> o;
+#pragma unroll
+      for (int e = 0; e < Vec<T>::N; ++e) o.e[e] = Elem<T>::st(v[k + e]);
+      stg_vec(y + n + k, o);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (n + k < N) y[n + k] = Elem<T>::st(v[k]);
+  }
+}
+
 template <typename T, bool F8>
 __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
   constexpr int BK = pp_bk(F8), NB = BK / 32;         // K tile, its blocks
@@ -554,36 +571,46 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
   constexpr int AU = 2, BU = F8 ? 1 : 2, SU = F8 ? 1 : 2;  // DMAs a wave: half-tiles, a tile's exponents
   constexpr int CNT = 2 * AU + 2 * BU + SU;
   constexpr int NS = F8 ? 1 : 2;                       // 128-column steps of a K tile
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF + 3 * SBUF];
+  constexpr int OP = 64 + 4, OBUF = 8 * OP;            // epilogue: 8 rows x 64 columns of a wave, fp32
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF + 3 * SBUF + 8 * OBUF * 4];
   unsigned char *const sring = lds + 2 * BUF;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int grp = wave >> 2, wn = wave & 3, fr = lane & 15, fq = lane >> 4;
+  float *const ostage = reinterpret_cast<float *>(lds + 2 * BUF + 3 * SBUF) + wave * OBUF;
 
-  // tile order: units of 8 row tiles x 4 column tiles on one XCD at a time (its L2 then holds 12
-  // operand panels for 32 workgroups), consecutive units on the 8 XCDs
-  int tm, tn;
-  {
-    const int orig = blockIdx.x, xcd = orig % 8, li = orig / 8;
-    const int slot = li % 32, u = (li / 32) * 8 + xcd;
-    const int mgn = (p.tiles_m + 7) / 8;
-    tm = (u % mgn) * 8 + slot % 8;
-    tn = (u / mgn) * 4 + slot / 8;
-    if (tm >= p.tiles_m || tn >= p.tiles_n) return;  // the whole workgroup, before any barrier
-  }
-  const int64_t m0 = (int64_t)tm * kPpTile, n0 = (int64_t)tn * kPpTile;
   const int xrow = F8 ? p.K : p.K / 2, wrow = p.K / 2;  // bytes of a row
   const int nt = (p.K + BK - 1) / BK;
-  const int rows_x = (int)(p.M - m0 < kPpTile ? p.M - m0 : kPpTile), rows_w = (int)(p.N - n0 < kPpTile ? p.N - n0 : kPpTile);
+  const int xpad = p.tiles_m * kPpTile, wpad = p.tiles_n * kPpTile;  // rows of the tiled exponents
+  const int xs_step = (p.xsc ? xpad : wpad) * NB, ws_step = wpad * NB;
+  const int a_chunk = (lane & 7) ^ (((wave * 8 + (lane >> 3)) >> 1) & 7);
+  const int b_chunk = F8 ? (lane & 3) ^ ((lane >> 4) & 3) : a_chunk;
+  // what to step back by where the chunk lies past K in the last tile (a chunk: 16 columns of E4M3, 32 of E2M1)
+  const unsigned a_tail = (nt - 1) * BK + a_chunk * (F8 ? 16 : 32) < p.K ? 0 : a_chunk * 16;
+  const unsigned b_tail = (nt - 1) * BK + b_chunk * 32 < p.K ? 0 : b_chunk * 16;
 
-  // ---- DMA sources.  xq half h, round u: LDS row rr = u * 64 + wave * 8 + lane / 8, chunk slot lane % 8;
-  // W half h: the same, or (64-byte rows) rr = wave * 16 + lane / 4, slot lane % 4.  Rows past the
-  // matrix re-read its last one (their results are not stored).
+  // ---- a tile of y and its DMA sources.  Tile order: units of 8 row tiles x 4 column tiles on one
+  // XCD at a time (its L2 then holds 12 operand panels for 32 workgroups), consecutive units on the
+  // 8 XCDs; the workgroups (a multiple of 8) step through the order.
+  const int mgn = (p.tiles_m + 7) / 8, total = (mgn * ((p.tiles_n + 3) / 4) + 7) / 8 * 8 * 32;
+  int tm = 0, tn = 0;
+  auto next_tile = [&](int &id) -> bool {
+    for (; id < total; id += gridDim.x) {
+      const int xcd = id % 8, li = id / 8, slot = li % 32, u = (li / 32) * 8 + xcd;
+      tm = (u % mgn) * 8 + slot % 8;
+      tn = (u / mgn) * 4 + slot / 8;
+      if (tm < p.tiles_m && tn < p.tiles_n) return true;
+    }
+    return false;
+  };
   unsigned a_off[2][AU], b_off[2][BU];
-  unsigned a_tail, b_tail;  // what to step back by where the chunk lies past K in the last tile
-  {
-    const int a_chunk = (lane & 7) ^ (((wave * 8 + (lane >> 3)) >> 1) & 7);
-    const int b_chunk = F8 ? (lane & 3) ^ (((lane >> 2) >> 2) & 3) : a_chunk;
+  __amdgpu_buffer_rsrc_t xr, wr, xsr, wsr;
+  auto set_tile = [&]() {
+    const int64_t m0 = (int64_t)tm * kPpTile, n0 = (int64_t)tn * kPpTile;
+    const int rows_x = (int)(p.M - m0 < kPpTile ? p.M - m0 : kPpTile), rows_w = (int)(p.N - n0 < kPpTile ? p.N - n0 : kPpTile);
+    // xq half h, round u: LDS row rr = u * 64 + wave * 8 + lane / 8, chunk slot lane % 8; W half h: the
+    // same, or (64-byte rows) rr = wave * 16 + lane / 4, slot lane % 4.  Rows past the matrix re-read
+    // its last one (their results are not stored).
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -598,17 +625,12 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
         b_off[h][u] = (unsigned)(row < rows_w ? row : rows_w - 1) * (unsigned)wrow + b_chunk * 16;
       }
     }
-    const int k0 = (nt - 1) * BK;  // a chunk: 16 columns of E4M3, 32 of E2M1
-    a_tail = k0 + a_chunk * (F8 ? 16 : 32) < p.K ? 0 : a_chunk * 16;
-    b_tail = k0 + b_chunk * 32 < p.K ? 0 : b_chunk * 16;
-  }
-  const __amdgpu_buffer_rsrc_t xr = wave_rsrc(p.x + m0 * xrow, (uint32_t)rows_x * (uint32_t)xrow);
-  const __amdgpu_buffer_rsrc_t wr = wave_rsrc(p.w + n0 * wrow, (uint32_t)rows_w * (uint32_t)wrow);
-  const int xpad = p.tiles_m * kPpTile, wpad = p.tiles_n * kPpTile;  // rows of the tiled exponents
-  const uint8_t *const xs_base = p.xsc ? p.xsc + m0 * NB : p.wsc + n0 * NB;  // no exponents: any (not read)
-  const int xs_step = (p.xsc ? xpad : wpad) * NB, ws_step = wpad * NB;
-  const __amdgpu_buffer_rsrc_t xsr = wave_rsrc(xs_base, (uint32_t)(nt - 1) * xs_step + SOP);
-  const __amdgpu_buffer_rsrc_t wsr = wave_rsrc(p.wsc + n0 * NB, (uint32_t)(nt - 1) * ws_step + SOP);
+    xr = wave_rsrc(p.x + m0 * xrow, (uint32_t)rows_x * (uint32_t)xrow);
+    wr = wave_rsrc(p.w + n0 * wrow, (uint32_t)rows_w * (uint32_t)wrow);
+    // rows without exponents: any bytes (not read from LDS)
+    xsr = wave_rsrc(p.xsc ? p.xsc + m0 * NB : p.wsc + n0 * NB, (uint32_t)(nt - 1) * xs_step + SOP);
+    wsr = wave_rsrc(p.wsc + n0 * NB, (uint32_t)(nt - 1) * ws_step + SOP);
+  };
 
   auto load_a = [&](int h, int t) {
     unsigned char *dst = lds + (t & 1) * BUF + h * AH + wave * 1024;
@@ -640,6 +662,19 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
       MX_DMA(wsr, dst + SOP + wave * 256, 4, (unsigned)(wave * 256 + lane * 4), sw);
     }
   };
+  // stream order of the DMAs: per K tile t  B1(t+1) | A1(t+1) | B0(t+2) | S(t+2) A0(t+2); CNT are those
+  // issued after the half-tile that the next phase reads.  A tile of y starts with the DMAs that the
+  // phases before its first K tile would have issued.
+  auto start_tile = [&]() {
+    load_b(0, 0);
+    load_s(0, 0);
+    load_a(0, 0);
+    load_b(1, 0);
+    load_a(1, 0);
+    load_b(0, 1);
+    load_s(1, 1);
+    load_a(0, 1);
+  };
 
   // ---- fragments.  E2M1 operand, step s: block 2 fq + s (E4M3 form: block fq of 4); E4M3 operand:
   // columns 16 fq .. and 64 + 16 fq ..
@@ -667,106 +702,125 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
     return *reinterpret_cast<const uint16_t *>(base + row * NB + 2 * fq);
   };
 
-  f32x4 acc[8][4];
+  const bool vec = (p.N * sizeof(T)) % 16 == 0 && ((uintptr_t)p.y & 15) == 0;
+  int id = blockIdx.x;
+  if (!next_tile(id)) return;  // the whole workgroup, before any barrier
+  set_tile();
+  start_tile();
+  for (bool more = true; more;) {
+    f32x4 acc[8][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    wait_vm<CNT>();
+    __builtin_amdgcn_s_barrier();
+    if (grp == 1) __builtin_amdgcn_s_barrier();  // one barrier behind
 
-  // stream order of the DMAs: per K tile t  B1(t+1) | A1(t+1) | B0(t+2) | S(t+2) A0(t+2); CNT are those
-  // issued after the half-tile that the next phase reads
-  load_b(0, 0);
-  load_s(0, 0);
-  load_a(0, 0);
-  load_b(1, 0);
-  load_a(1, 0);
-  load_b(0, 1);
-  load_s(1, 1);
-  load_a(0, 1);
-  wait_vm<CNT>();
-  __builtin_amdgcn_s_barrier();
-  if (grp == 1) __builtin_amdgcn_s_barrier();  // one barrier behind
-
-  i32x8 af[4][NS], b0f[2][NS], b1f[2][NS];
-  int sa[4], sb0[2], sb1[2];
-  int slot = 0;
-  for (int t = 0; t < nt; ++t) {
-    const unsigned char *cur = lds + (t & 1) * BUF;
-    const unsigned char *sx = sring + slot * SBUF, *sw = sx + SOP;
-    const int slot2 = slot == 0 ? 2 : slot - 1;  // (t + 2) % 3
-    // rows without exponents: 2^0, past K 2^-127
-    const int unit = F8 && !p.xsc ? ((t == nt - 1 && (nt - 1) * BK + 32 * fq >= p.K) ? 0 : 127) : 0;
+    i32x8 af[4][NS], b0f[2][NS], b1f[2][NS];
+    int sa[4], sb0[2], sb1[2];
+    int slot = 0;
+    for (int t = 0; t < nt; ++t) {
+      const unsigned char *cur = lds + (t & 1) * BUF;
+      const unsigned char *sx = sring + slot * SBUF, *sw = sx + SOP;
+      const int slot2 = slot == 0 ? 2 : slot - 1;  // (t + 2) % 3
+      // rows without exponents: 2^0, past K 2^-127
+      const int unit = F8 && !p.xsc ? ((t == nt - 1 && (nt - 1) * BK + 32 * fq >= p.K) ? 0 : 127) : 0;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int mq = (q == 0 || q == 1) ? 0 : 1;
-      const int nq = (q == 1 || q == 2) ? 1 : 0;
-      if (q == 0 || q == 2) {
+      for (int q = 0; q < 4; ++q) {
+        const int mq = (q == 0 || q == 1) ? 0 : 1;
+        const int nq = (q == 1 || q == 2) ? 1 : 0;
+        if (q == 0 || q == 2) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 4; ++i) {
 #pragma unroll
-          for (int s = 0; s < NS; ++s) af[i][s] = read_a(cur, 4 * mq + i, s);
-          sa[i] = F8 && !p.xsc ? unit : read_s(sx, grp * 128 + 16 * (4 * mq + i) + fr);
+            for (int s = 0; s < NS; ++s) af[i][s] = read_a(cur, 4 * mq + i, s);
+            sa[i] = F8 && !p.xsc ? unit : read_s(sx, grp * 128 + 16 * (4 * mq + i) + fr);
+          }
         }
-      }
-      if (q == 0) {
+        if (q == 0) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+          for (int j = 0; j < 2; ++j) {
 #pragma unroll
-          for (int s = 0; s < NS; ++s) b0f[j][s] = read_b(cur, j, s);
-          sb0[j] = read_s(sw, wn * 64 + 16 * j + fr);
+            for (int s = 0; s < NS; ++s) b0f[j][s] = read_b(cur, j, s);
+            sb0[j] = read_s(sw, wn * 64 + 16 * j + fr);
+          }
         }
-      }
-      if (q == 1) {
+        if (q == 1) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+          for (int j = 0; j < 2; ++j) {
 #pragma unroll
-          for (int s = 0; s < NS; ++s) b1f[j][s] = read_b(cur, 2 + j, s);
-          sb1[j] = read_s(sw, wn * 64 + 16 * (2 + j) + fr);
+            for (int s = 0; s < NS; ++s) b1f[j][s] = read_b(cur, 2 + j, s);
+            sb1[j] = read_s(sw, wn * 64 + 16 * (2 + j) + fr);
+          }
         }
+        if (q == 0) load_b(1, t + 1);
+        if (q == 1) load_a(1, t + 1);
+        if (q == 2) load_b(0, t + 2);
+        if (q == 3) {
+          load_s(t + 2, slot2);
+          load_a(0, t + 2);
+        }
+        wait_vm<CNT>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[4 * mq + i][2 * nq + j] =
+                  pp_mma<F8>(nq ? b1f[j][s] : b0f[j][s], af[i][s], acc[4 * mq + i][2 * nq + j], s, nq ? sb1[j] : sb0[j], sa[i]);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_s_barrier();
       }
-      if (q == 0) load_b(1, t + 1);
-      if (q == 1) load_a(1, t + 1);
-      if (q == 2) load_b(0, t + 2);
-      if (q == 3) {
-        load_s(t + 2, slot2);
-        load_a(0, t + 2);
-      }
-      wait_vm<CNT>();
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            acc[4 * mq + i][2 * nq + j] =
-                pp_mma<F8>(nq ? b1f[j][s] : b0f[j][s], af[i][s], acc[4 * mq + i][2 * nq + j], s, nq ? sb1[j] : sb0[j], sa[i]);
-      __builtin_amdgcn_s_setprio(0);
-      __builtin_amdgcn_s_barrier();
+      slot = slot == 2 ? 0 : slot + 1;
     }
-    slot = slot == 2 ? 0 : slot + 1;
-  }
-  if (grp == 0) __builtin_amdgcn_s_barrier();  // balance the stagger
-  wait_vm<0>();  // the re-loads past the end land before the workgroup's LDS is given away
+    if (grp == 0) __builtin_amdgcn_s_barrier();  // balance the stagger: every wave is done with the buffers
+    wait_vm<0>();                                // this tile's re-loads past the end have landed ...
+    __builtin_amdgcn_s_barrier();                // ... every wave's: the next tile's DMAs may begin
 
-  // ---- lane: y[m][n .. n + 3], m = 16 i + fr, n = 16 j + 4 fq of the wave's 128 x 64
+    const int64_t m0 = (int64_t)tm * kPpTile + grp * 128, n0 = (int64_t)tn * kPpTile + wn * 64;
+    id += gridDim.x;
+    more = next_tile(id);
+    if (more) {
+      set_tile();
+      start_tile();  // in flight under the epilogue
+    }
+
+    // ---- y of the wave's 128 x 64: a lane holds y[m][n .. n + 3], m = 16 i + fr, n = 16 j + 4 fq; through
+    // LDS, 8 rows at a time, so that 8 lanes store a row's 64 columns
+    const int orow = lane >> 3, ocol = 8 * (lane & 7);
+    const int64_t n = n0 + ocol;
+    float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (p.bias) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t m = m0 + grp * 128 + 16 * i + fr;
-    if (m >= p.M) continue;
-    const float f = p.xf ? p.xf[m * p.xf_stride] : 1.f;
-    T *y = reinterpret_cast<T *>(p.y) + m * p.N;
+      for (int k = 0; k < 8; ++k) {
+        const int64_t nk = n + k < p.N ? n + k : p.N - 1;
+        bias[k] = p.bias_f32 ? reinterpret_cast<const float *>(p.bias)[nk] : Elem<T>::ld(reinterpret_cast<const T *>(p.bias)[nk]);
+      }
+    }
+    float f0 = 1.f, f1 = 1.f;  // the factors of rows lane and 64 + lane
+    if (p.xf) {
+      const int64_t r0 = m0 + lane < p.M ? m0 + lane : p.M - 1, r1 = m0 + 64 + lane < p.M ? m0 + 64 + lane : p.M - 1;
+      f0 = p.xf[r0 * p.xf_stride], f1 = p.xf[r1 * p.xf_stride];
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = n0 + wn * 64 + 16 * j + 4 * fq;
+    for (int i = 0; i < 16; ++i) {
+      if ((fr >> 3) == (i & 1)) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (n + k < p.N) {
-          float o = acc[i][j][k] * f;
-          if (p.bias) o += p.bias_f32 ? reinterpret_cast<const float *>(p.bias)[n + k] : Elem<T>::ld(reinterpret_cast<const T *>(p.bias)[n + k]);
-          y[n + k] = Elem<T>::st(o);
-        }
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4 *>(ostage + (fr & 7) * OP + 16 * j + 4 * fq) = acc[i >> 1][j];
+      }
+      __builtin_amdgcn_wave_barrier();
+      const int64_t m = m0 + 8 * i + orow;
+      float v[8];
+      const f32x4 lo = *reinterpret_cast<const f32x4 *>(ostage + orow * OP + ocol), hi = *reinterpret_cast<const f32x4 *>(ostage + orow * OP + ocol + 4);
+      const float f = __shfl(i < 8 ? f0 : f1, (8 * i + orow) & 63, 64);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = (k < 4 ? lo[k] : hi[k - 4]) * f + bias[k];
+      if (m < p.M) pp_store8<T>(reinterpret_cast<T *>(p.y) + m * p.N, v, n, p.N, vec);
+      __builtin_amdgcn_wave_barrier();
     }
   }
 }
@@ -831,8 +885,10 @@ template <bool F8> int launch_tile_scales(const uint8_t *s, int rows, int K, uin
 }
 template <typename T, bool F8> int launch_pp(PpArgs a, hipStream_t stream) {
   a.tiles_m = (a.M + kPpTile - 1) / kPpTile, a.tiles_n = (a.N + kPpTile - 1) / kPpTile;
-  const int64_t units = (int64_t)((a.tiles_m + 7) / 8) * ((a.tiles_n + 3) / 4);
-  mx_pp_kernel<T, F8><<<(unsigned)((units + 7) / 8 * 8 * 32), kPpThreads, 0, stream>>>(a);
+  // one workgroup a CU (its LDS), each going through several tiles of y
+  const int64_t order = ((int64_t)((a.tiles_m + 7) / 8) * ((a.tiles_n + 3) / 4) + 7) / 8 * 8 * 32;
+  const int64_t cus = (host_num_cus() + 7) / 8 * 8;
+  mx_pp_kernel<T, F8><<<(unsigned)(order < cus ? order : cus), kPpThreads, 0, stream>>>(a);
   return host_check_launch();
 }
 
