@@ -489,7 +489,8 @@ int mtq_rms_norm_quantize(const void *x, int64_t x_stride, const void *residual,
 /* y[M][N] = xq[M][K] . W[N][K]^T + bias, W as MTQ_MXFP4 (MXFP4QTensor's bytes and scales), fp32
  * sums, one rounding to y_dtype.  x_dtype >= 0: x is [M][K] of that dtype (row stride x_stride) and
  * is quantised to `kind` on the way (amax for MTQ_FP8_TENSOR); x_dtype < 0: x and x_scale are the
- * quantised rows.  w (and a quantised x) 16-byte aligned.  bias: y_dtype or fp32, or NULL.  ws:
+ * quantised rows.  w (and a quantised x) 16-byte aligned, their scales 4-byte aligned; M, N <=
+ * 2^24, K <= 2^22.  bias: y_dtype or fp32, or NULL.  ws:
  * mtq_mx_linear_workspace_bytes bytes, 16-byte aligned, contents overwritten. */
 size_t mtq_mx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int kind, int x_dtype);
 int mtq_mx_linear(const void *x, int64_t x_stride, int x_dtype, const void *x_scale, int kind,

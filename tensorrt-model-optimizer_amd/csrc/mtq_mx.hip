@@ -350,6 +350,94 @@ int launch_quantize(const T *x, int64_t xs, int64_t rows, int64_t cols, int kind
   return host_check_launch();
 }
 
+// 4 consecutive columns of a row of y: v * f + bias, rounded once
+template <typename T>
+__device__ __forceinline__ void out4(T *y, const f32x4 &v, float f, const void *bias, int bias_f32, int64_t n, int N, bool vec) {
+  float o[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    o[k] = v[k] * f;
+    if (bias && n + k < N) o[k] += bias_f32 ? reinterpret_cast<const float *>(bias)[n + k] : Elem<T>::ld(reinterpret_cast<const T *>(bias)[n + k]);
+  }
+  if (vec) {  // N % 4 == 0, y aligned: the 4 columns are all in or all out
+    struct alignas(4 * sizeof(T)) Pack {
+      T e[4];
+    } pk;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) pk.e[k] = Elem<T>::st(o[k]);
+    if (n < N) *reinterpret_cast<Pack *>(y + n) = pk;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n + k < N) y[n + k] = Elem<T>::st(o[k]);
+  }
+}
+
+// v_cvt_scalef32_pk_fp4_{bf16,f16} into byte SEL of a dword of codes
+template <typename T> struct Fp4Pair;
+template <> struct Fp4Pair<__bf16> {
+  typedef bf16x2_t v2;
+  template <int SEL> static __device__ __forceinline__ uint32_t cvt(uint32_t w, v2 p, float s) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, p, s, SEL);
+  }
+};
+template <> struct Fp4Pair<_Float16> {
+  typedef f16x2_t v2;
+  template <int SEL> static __device__ __forceinline__ uint32_t cvt(uint32_t w, v2 p, float s) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, p, s, SEL);
+  }
+};
+
+// 32 values of one lane in 16 packed 16-bit pairs -> its block's E2M1 codes and exponent byte: the
+// largest magnitude from packed integer maxima of the bit patterns (NaN patterns sort above infinity),
+// the codes from v_cvt_scalef32_pk_fp4_{bf16,f16}; a block with a NaN or an exponent outside -100 .. 100
+// takes the fp32 forms
+template <typename T> __device__ __forceinline__ void block_codes(const u32x4 (&x)[4], u32x4 &codes, int &exponent) {
+  u16x2_t mx = {0, 0};
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mx = __builtin_elementwise_max(mx, __builtin_bit_cast(u16x2_t, x[t][j] & 0x7fff7fffu));
+  const uint32_t mb = mx.x > mx.y ? mx.x : mx.y;
+  float m = mb == Fp4Native<T>::kInfBits ? 3.402823466e38f : half_bits_to_float<T>(mb);
+  const bool nan = mb > Fp4Native<T>::kInfBits;
+  if (nan) {
+    m = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m = fmaxf(m, mx_abs(half_bits_to_float<T>(x[t][j] & 0xffffu)));
+        m = fmaxf(m, mx_abs(half_bits_to_float<T>(x[t][j] >> 16)));
+      }
+  }
+  float scale, un;
+  e8m0_scale(m, 6.0f, scale, un);
+  exponent = (int)((__float_as_uint(un) >> 23) & 0xff);
+  if (!nan && un >= 0x1p-100f && un <= 0x1p100f) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      uint32_t w = 0;
+      typename Fp4Pair<T>::v2 p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = __builtin_bit_cast(typename Fp4Pair<T>::v2, (uint32_t)x[t][j]);
+      w = Fp4Pair<T>::template cvt<0>(w, p[0], un);
+      w = Fp4Pair<T>::template cvt<1>(w, p[1], un);
+      w = Fp4Pair<T>::template cvt<2>(w, p[2], un);
+      w = Fp4Pair<T>::template cvt<3>(w, p[3], un);
+      codes[t] = w;
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[2 * j] = half_bits_to_float<T>(x[t][j] & 0xffffu), v[2 * j + 1] = half_bits_to_float<T>(x[t][j] >> 16);
+      codes[t] = e2m1_codes8(v, un);
+    }
+  }
+}
+
 // ---- y = xq . W^T for few rows -------------------------------------------------------------------
 // v_mfma_scale_f32_16x16x128_f8f6f4, first operand 16 rows of W, second 16 rows of xq: lane
 // (r = lane & 15, g = lane >> 4) gives row r's block g of a 128-column step (E2M1: 16 bytes) and that
@@ -357,10 +445,11 @@ int launch_quantize(const T *x, int64_t xs, int64_t rows, int64_t cols, int kind
 // (the layout was read off the instruction on the card), its lane's byte still being block g's.  The
 // result holds y^T: lane (r, g) has row r of xq and 4 consecutive rows 4 g .. of W.
 //
-// The call is bound by reading W once (17/32 byte per weight), so a workgroup is 8 waves that split K
-// over the same 16 * NT rows of W, every wave streaming its part straight into the operand registers
-// (nothing of W is shared, so LDS would only add a trip), and the 8 partial tiles meet in LDS at the end,
-// summed in wave order.
+// The call is bound by reading W once (17/32 byte per weight), so a workgroup is WAVES waves that split
+// K over the same 16 * NT rows of W, every wave streaming its part straight into the operand registers
+// (nothing of W is shared, so LDS would only add a trip), and the partial tiles meet in LDS at the end,
+// summed in wave order.  A wave takes 512 columns at a time: 4 NT loads of codes, one 16-byte load of
+// exponents a row, all in flight together; the other waves of the SIMD cover the rest.
 struct SkinnyArgs {
   const void *x;             // xq, or the 16-bit activations (FUSED)
   const uint8_t *xsc;        // exponent bytes [M, K / 32] (MX formats)
@@ -369,22 +458,26 @@ struct SkinnyArgs {
   const void *bias;
   void *y;
   int64_t xs;                // row stride of the 16-bit activations
-  int M, N, K;
+  int M, N, K, tiles_n;
   int xf_stride;             // 1: a factor per row, 0: one
   int bias_f32;
 };
 
 enum { kOpFp4 = 0, kOpFp8 = 1, kOpFused = 2 };
-constexpr int kSkinnyWaves = 8;
 
-template <typename T, int OP, int MT, int NT>
-__global__ __launch_bounds__(64 * kSkinnyWaves) void mx_skinny_kernel(SkinnyArgs a) {
-  constexpr int CH = MT * NT < 4 ? MT * NT : 4;  // tiles joined at a time
-  __shared__ f32x4 red[kSkinnyWaves][CH][64];
+__device__ __forceinline__ u32x4 load16_any(const uint8_t *p) {  // any alignment
+  u32x4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+
+template <typename T, int OP, int NT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void mx_skinny_kernel(SkinnyArgs a) {
+  __shared__ f32x4 red[WAVES][NT][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
-  const int nb = a.K / 32, steps = (nb + 3) / 4;
-  const int s0 = (int)((int64_t)steps * wave / kSkinnyWaves), s1 = (int)((int64_t)steps * (wave + 1) / kSkinnyWaves);
+  const int n0 = (blockIdx.x % a.tiles_n) * 16 * NT, m0 = (blockIdx.x / a.tiles_n) * 16;
+  const int nb = a.K / 32, batches = (nb + 15) / 16;
+  const int b0 = (int)((int64_t)batches * wave / WAVES), b1 = (int)((int64_t)batches * (wave + 1) / WAVES);
   const uint8_t *wp[NT], *wsp[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
@@ -392,107 +485,114 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void mx_skinny_kernel(SkinnyArgs
     wp[j] = a.w + (int64_t)n * (a.K / 2);
     wsp[j] = a.wsc + (int64_t)n * nb;
   }
-  int xrow[MT];
+  const int64_t xm = m0 + r < a.M ? m0 + r : a.M - 1;
+  const uint8_t *const xp = reinterpret_cast<const uint8_t *>(a.x) + xm * (OP == kOpFused ? a.xs * 2 : OP == kOpFp4 ? a.K / 2 : a.K);
+  const uint8_t *const xsp = a.xsc + xm * nb;
+  f32x4 acc[NT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) xrow[i] = m0 + 16 * i + r < a.M ? m0 + 16 * i + r : a.M - 1;
-  f32x4 acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int s = s0; s < s1; ++s) {
-    const int b = 4 * s + g;
-    const bool in = b < nb;  // the last step of a K that 128 does not divide
-    const int bc = in ? b : 0;
-    i32x8 wf[NT];
-    int ws[NT];
+  constexpr int XV = OP == kOpFused ? 4 : OP == kOpFp8 ? 2 : 1;
+  constexpr bool XS = OP != kOpFused;
+  struct Batch {
+    u32x4 w[NT][4], ws[NT], x[4][XV], xs;
+  } st;
+  auto load = [&](int b, Batch &d) {
+    const int blk0 = 16 * b + g;
+    if (16 * b + 16 <= nb) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      u32x4 d = *reinterpret_cast<const u32x4 *>(wp[j] + (int64_t)bc * 16);
-      ws[j] = wsp[j][bc];
-      if (!in) d = u32x4{0, 0, 0, 0};  // zero codes: whatever the other operand holds there is lost
-      if (!in) ws[j] = 127;
-      wf[j] = i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, 0, 0, 0, 0};
-    }
+      for (int j = 0; j < NT; ++j) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      i32x8 xf;
-      int xs = 127;
-      if constexpr (OP == kOpFused) {
-        const T *xp = reinterpret_cast<const T *>(a.x) + xrow[i] * a.xs + (int64_t)bc * 32;
-        float v[4][8];
-        float m = 0.f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          load8<T, true>(xp, 8 * t, 0, v[t]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) m = fmaxf(m, mx_abs(v[t][j]));
-        }
-        float sc, un;
-        e8m0_scale(m, 6.0f, sc, un);
-        xs = (int)((__float_as_uint(un) >> 23) & 0xff);
-        xf = i32x8{(int)e2m1_codes8(v[0], un), (int)e2m1_codes8(v[1], un), (int)e2m1_codes8(v[2], un),
-                   (int)e2m1_codes8(v[3], un), 0, 0, 0, 0};
-      } else if constexpr (OP == kOpFp4) {
-        const uint8_t *xp = reinterpret_cast<const uint8_t *>(a.x) + (int64_t)xrow[i] * (a.K / 2);
-        const u32x4 d = *reinterpret_cast<const u32x4 *>(xp + (int64_t)bc * 16);
-        xs = a.xsc[(int64_t)xrow[i] * nb + bc];
-        xf = i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, 0, 0, 0, 0};
-      } else {
-        const uint8_t *xp = reinterpret_cast<const uint8_t *>(a.x) + (int64_t)xrow[i] * a.K;
-        const int k0 = 128 * s + 16 * g, k1 = k0 + 64;  // 16 columns each; past K: columns 0 .. 15
-        const u32x4 d = *reinterpret_cast<const u32x4 *>(xp + (k0 < a.K ? k0 : 0));
-        const u32x4 e = *reinterpret_cast<const u32x4 *>(xp + (k1 < a.K ? k1 : 0));
-        if (a.xsc) xs = a.xsc[(int64_t)xrow[i] * nb + bc];
-        xf = i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, (int)e.x, (int)e.y, (int)e.z, (int)e.w};
+        for (int u = 0; u < 4; ++u) d.w[j][u] = *reinterpret_cast<const u32x4 *>(wp[j] + (int64_t)(blk0 + 4 * u) * 16);
+        d.ws[j] = load16_any(wsp[j] + 16 * b);
       }
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], xf, acc[i][j], 4, OP == kOpFp8 ? 0 : 4, 0, ws[j],
-                                                                     0, xs);
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int t = 0; t < XV; ++t)
+          d.x[u][t] = *reinterpret_cast<const u32x4 *>(
+              OP == kOpFp8 ? xp + 512 * (int64_t)b + 128 * u + 64 * t + 16 * g
+                           : xp + (int64_t)(blk0 + 4 * u) * (OP == kOpFused ? 64 : 16) + 16 * t);
+      if constexpr (XS) {
+        d.xs = u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+        if (a.xsc) d.xs = load16_any(xsp + 16 * b);
+      }
+    } else {  // the end of a K that 512 does not divide: what lies past it becomes zero codes of W
+      const uint32_t sh = 8 * g;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int blk = blk0 + 4 * u, bc = blk < nb ? blk : 0;
+        const bool in = blk < nb;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const u32x4 v = *reinterpret_cast<const u32x4 *>(wp[j] + (int64_t)bc * 16);
+          d.w[j][u] = in ? v : u32x4{0, 0, 0, 0};
+          d.ws[j][u] = (uint32_t)(in ? wsp[j][bc] : 127) << sh;
+        }
+#pragma unroll
+        for (int t = 0; t < XV; ++t) {
+          const int k = 512 * b + 128 * u + 64 * t + 16 * g;
+          d.x[u][t] = *reinterpret_cast<const u32x4 *>(OP == kOpFp8 ? xp + (k < a.K ? k : 0)
+                                                                    : xp + (int64_t)bc * (OP == kOpFused ? 64 : 16) + 16 * t);
+        }
+        if constexpr (XS) d.xs[u] = (uint32_t)(a.xsc ? xsp[bc] : 127) << sh;
+      }
     }
+  };
+  auto use = [&](const Batch &d) {
+    const uint32_t sh = 8 * g;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      i32x8 xf;
+      int xs;
+      if constexpr (OP == kOpFused) {
+        u32x4 c;
+        block_codes<T>(d.x[u], c, xs);
+        xf = i32x8{(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0};
+      } else {
+        xs = (int)(d.xs[u] >> sh);
+        if constexpr (OP == kOpFp4)
+          xf = i32x8{(int)d.x[u][0].x, (int)d.x[u][0].y, (int)d.x[u][0].z, (int)d.x[u][0].w, 0, 0, 0, 0};
+        else
+          xf = i32x8{(int)d.x[u][0].x, (int)d.x[u][0].y, (int)d.x[u][0].z, (int)d.x[u][0].w,
+                     (int)d.x[u][XV - 1].x, (int)d.x[u][XV - 1].y, (int)d.x[u][XV - 1].z, (int)d.x[u][XV - 1].w};
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const i32x8 wf = {(int)d.w[j][u].x, (int)d.w[j][u].y, (int)d.w[j][u].z, (int)d.w[j][u].w, 0, 0, 0, 0};
+        acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[j], 4, OP == kOpFp8 ? 0 : 4, 0, (int)(d.ws[j][u] >> sh), 0, xs);
+      }
+    }
+  };
+  for (int b = b0; b < b1; ++b) {
+    load(b, st);
+    use(st);
   }
 
 #pragma unroll
-  for (int c = 0; c < MT * NT; c += CH) {
-    if (c) __syncthreads();
+  for (int j = 0; j < NT; ++j) red[wave][j][lane] = acc[j];
+  __syncthreads();
+  if (wave < NT) {
+    const int m = m0 + r, n = n0 + 16 * wave + 4 * g;
+    f32x4 v = red[0][wave][lane];
 #pragma unroll
-    for (int t = 0; t < CH; ++t) red[wave][t][lane] = acc[(c + t) / NT][(c + t) % NT];
-    __syncthreads();
-    if (tid < 64 * CH) {
-      const int t = wave, m = m0 + 16 * ((c + t) / NT) + r, n = n0 + 16 * ((c + t) % NT) + 4 * g;
-      f32x4 v = red[0][t][lane];
-#pragma unroll
-      for (int w = 1; w < kSkinnyWaves; ++w) v += red[w][t][lane];
-      if (m < a.M) {
-        const float f = a.xf ? a.xf[(int64_t)m * a.xf_stride] : 1.f;
-        T *y = reinterpret_cast<T *>(a.y) + (int64_t)m * a.N;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (n + k < a.N) {
-            float o = v[k] * f;
-            if (a.bias) o += a.bias_f32 ? reinterpret_cast<const float *>(a.bias)[n + k] : Elem<T>::ld(reinterpret_cast<const T *>(a.bias)[n + k]);
-            y[n + k] = Elem<T>::st(o);
-          }
-      }
+    for (int w = 1; w < WAVES; ++w) v += red[w][wave][lane];
+    if (m < a.M) {
+      const float f = a.xf ? a.xf[(int64_t)m * a.xf_stride] : 1.f;
+      out4<T>(reinterpret_cast<T *>(a.y) + (int64_t)m * a.N, v, f, a.bias, a.bias_f32, n, a.N, a.N % 4 == 0 && ((uintptr_t)a.y & 15) == 0);
     }
   }
 }
 
-template <typename T, int OP> int launch_skinny(const SkinnyArgs &a, hipStream_t stream) {
-  // rows of W a wave takes: more of them share one read of xq (worth it once there are workgroups
-  // enough to fill the card)
-  const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-  const int tiles = (a.N + 15) / 16;
-  const dim3 g((unsigned)tiles, (unsigned)((a.M + 16 * mt - 1) / (16 * mt)));
-  if (mt == 1)
-    mx_skinny_kernel<T, OP, 1, 1><<<g, 64 * kSkinnyWaves, 0, stream>>>(a);
-  else if constexpr (OP != kOpFused) {
-    if (mt == 2)
-      mx_skinny_kernel<T, OP, 2, 1><<<g, 64 * kSkinnyWaves, 0, stream>>>(a);
-    else
-      mx_skinny_kernel<T, OP, 4, 1><<<g, 64 * kSkinnyWaves, 0, stream>>>(a);
+template <typename T, int OP> int launch_skinny(SkinnyArgs a, hipStream_t stream) {
+  // two tiles of W share a read (and FUSED: the quantisation) of xq where that leaves a workgroup for every CU
+  const int64_t gm = (a.M + 15) / 16;
+  if (a.N >= 32 * host_num_cus()) {
+    a.tiles_n = (a.N + 31) / 32;
+    mx_skinny_kernel<T, OP, 2, 8><<<(unsigned)(gm * a.tiles_n), 64 * 8, 0, stream>>>(a);
+  } else {
+    a.tiles_n = (a.N + 15) / 16;
+    mx_skinny_kernel<T, OP, 1, 8><<<(unsigned)(gm * a.tiles_n), 64 * 8, 0, stream>>>(a);
   }
   return host_check_launch();
 }
@@ -825,6 +925,206 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
   }
 }
 
+// ---- y = xq . W^T in between ---------------------------------------------------------------------
+// Too many rows to stream W past registers, too few tiles of 256 x 256 to fill the card: BM x BN tiles
+// (64 or 128), 4 waves of (BM / 2) x (BN / 2), K tiles as above in a ring of STAGES in LDS, filled by
+// DMA STAGES - 1 ahead, one barrier a K tile (a stage is refilled after the barrier behind its last
+// read).  Where there are still fewer tiles than CUs, K is cut into splits whose fp32 tiles a second
+// small kernel adds in order.  Exponents: [rows][stride], stride a multiple of 4, zero past K.
+struct MidArgs {
+  const uint8_t *x, *w, *xsc, *wsc;
+  const float *xf;
+  const void *bias;
+  void *y;
+  float *part;  // [splits][M][N]
+  int M, N, K, tiles_m, tiles_n, xs_stride, ws_stride, xf_stride, bias_f32, splits;
+};
+
+template <typename T, bool F8, int BM, int BN, int STAGES>
+__global__ __launch_bounds__(256, 2) void mx_mid_kernel(MidArgs p) {
+  constexpr int BK = pp_bk(F8), NB = BK / 32, WR = BK / 2;  // K tile, its blocks, bytes of a W row in it
+  constexpr int AB = BM * 128, BB = BN * WR, SA = BM * NB, SB = BN * NB;
+  constexpr int AU = AB / 4096, BU = BB / 4096;          // 16-byte DMAs a wave
+  constexpr int SI = (SA + SB + 1023) / 1024;            // 4-byte DMAs a wave (the last ones may be idle copies)
+  constexpr int SBYTES = SI * 1024;
+  constexpr int STAGE = AB + BB + SBYTES, CNT = (STAGES - 2) * (AU + BU + SI);
+  constexpr int NS = F8 ? 1 : 2, MI = BM / 32, NJ = BN / 32;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[STAGES * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1, fr = lane & 15, fq = lane >> 4;
+
+  // tiles of one column of W on one XCD, row tiles fastest: W's panel is read from HBM once
+  const int per = p.tiles_m * p.tiles_n, split = blockIdx.x / per, rest = blockIdx.x - split * per;
+  const int q8 = per / 8, r8 = per % 8, xcd = rest % 8;
+  const int li = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + rest / 8;
+  const int tn = li / p.tiles_m, tm = li - tn * p.tiles_m;
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int xrow = F8 ? p.K : p.K / 2, wrow = p.K / 2;
+  const int nt_all = (p.K + BK - 1) / BK;
+  const int t0 = (int)((int64_t)nt_all * split / p.splits), t1 = (int)((int64_t)nt_all * (split + 1) / p.splits);
+  const int rows_x = (int)(p.M - m0 < BM ? p.M - m0 : BM), rows_w = (int)(p.N - n0 < BN ? p.N - n0 : BN);
+
+  // ---- DMA sources.  Operand rows of 128 bytes: LDS row u * 32 + wave * 8 + lane / 8, chunk slot lane % 8; of 64
+  // bytes: u * 64 + wave * 16 + lane / 4, slot lane % 4.  Rows past the matrix re-read its last one.
+  const int a_chunk = (lane & 7) ^ (((wave * 8 + (lane >> 3)) >> 1) & 7);
+  const int b_chunk = F8 ? (lane & 3) ^ ((lane >> 4) & 3) : a_chunk;
+  unsigned a_off[AU], b_off[BU], s_off[SI];
+#pragma unroll
+  for (int u = 0; u < AU; ++u) {
+    const int row = u * 32 + wave * 8 + (lane >> 3);
+    a_off[u] = (unsigned)(row < rows_x ? row : rows_x - 1) * (unsigned)xrow + a_chunk * 16;
+  }
+#pragma unroll
+  for (int u = 0; u < BU; ++u) {
+    const int row = F8 ? u * 64 + wave * 16 + (lane >> 2) : u * 32 + wave * 8 + (lane >> 3);
+    b_off[u] = (unsigned)(row < rows_w ? row : rows_w - 1) * (unsigned)wrow + b_chunk * 16;
+  }
+  // exponents: dword d of [xq rows][NB] then [W rows][NB]; a wave-sized piece is one operand's
+  bool s_x[SI];
+#pragma unroll
+  for (int u = 0; u < SI; ++u) {
+    int d = (u * 4 + wave) * 64 + lane;
+    s_x[u] = p.xsc && (u * 4 + wave) * 256 < SA;
+    if ((u * 4 + wave) * 256 >= SA) d -= SA / 4;
+    const int rows = s_x[u] ? rows_x : rows_w;
+    int row = d / (NB / 4);
+    row = row < rows ? row : rows - 1;
+    s_off[u] = (unsigned)row * (unsigned)(s_x[u] ? p.xs_stride : p.ws_stride) + 4 * (d % (NB / 4));
+  }
+  const int k_last = (nt_all - 1) * BK;
+  const unsigned a_tail = k_last + a_chunk * (F8 ? 16 : 32) < p.K ? 0 : a_chunk * 16;
+  const unsigned b_tail = k_last + b_chunk * 32 < p.K ? 0 : b_chunk * 16;
+  const __amdgpu_buffer_rsrc_t xr = wave_rsrc(p.x + m0 * xrow, (uint32_t)rows_x * (uint32_t)xrow);
+  const __amdgpu_buffer_rsrc_t wr = wave_rsrc(p.w + n0 * wrow, (uint32_t)rows_w * (uint32_t)wrow);
+  const __amdgpu_buffer_rsrc_t xsr = wave_rsrc(p.xsc ? p.xsc + m0 * p.xs_stride : p.wsc + n0 * p.ws_stride,
+                                               p.xsc ? (uint32_t)rows_x * p.xs_stride : (uint32_t)rows_w * p.ws_stride);
+  const __amdgpu_buffer_rsrc_t wsr = wave_rsrc(p.wsc + n0 * p.ws_stride, (uint32_t)rows_w * p.ws_stride);
+  auto load = [&](int t, int slot) {
+    unsigned char *dst = lds + slot * STAGE;
+    const int tt = t < t1 ? t : t1 - 1;  // past the end: harmless re-loads
+    const uint32_t sa = __builtin_amdgcn_readfirstlane((uint32_t)tt * 128), sb = __builtin_amdgcn_readfirstlane((uint32_t)tt * WR);
+    const uint32_t ss = __builtin_amdgcn_readfirstlane((uint32_t)tt * NB);
+    const bool last = tt == nt_all - 1;
+#pragma unroll
+    for (int u = 0; u < AU; ++u) MX_DMA(xr, dst + u * 4096 + wave * 1024, 16, a_off[u] - (last ? a_tail : 0), sa);
+#pragma unroll
+    for (int u = 0; u < BU; ++u) MX_DMA(wr, dst + AB + u * 4096 + wave * 1024, 16, b_off[u] - (last ? b_tail : 0), sb);
+#pragma unroll
+    for (int u = 0; u < SI; ++u) {
+      if (s_x[u])
+        MX_DMA(xsr, dst + AB + BB + (u * 4 + wave) * 256, 4, s_off[u], ss);
+      else
+        MX_DMA(wsr, dst + AB + BB + (u * 4 + wave) * 256, 4, s_off[u], ss);
+    }
+  };
+
+  const int sw8 = (fr >> 1) & 7, sw4 = (fr >> 2) & 3;
+  auto ld4 = [&](const unsigned char *q) -> i32x8 {
+    const u32x4 d = *reinterpret_cast<const u32x4 *>(q);
+    return i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, 0, 0, 0, 0};
+  };
+  f32x4 acc[MI][NJ];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (t0 < t1) {
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) load(t0 + s, s);
+    int slot = 0;
+    for (int t = t0; t < t1; ++t) {
+      wait_vm<CNT>();                 // this wave's part of stage t has landed ...
+      __builtin_amdgcn_s_barrier();   // ... every wave's; and stage t - 1 has been read by all
+      load(t + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+      const unsigned char *st = lds + slot * STAGE, *sx = st + AB + BB, *sw = sx + SA;
+      const int unit = F8 && !p.xsc ? ((t == nt_all - 1 && k_last + 32 * fq >= p.K) ? 0 : 127) : 0;
+      i32x8 bf[NJ][NS];
+      int sb[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int row = wn * (BN / 2) + 16 * j + fr;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) bf[j][s] = ld4(st + AB + row * WR + (F8 ? (fq ^ sw4) << 4 : ((2 * fq + s) ^ sw8) << 4));
+        if constexpr (F8)
+          sb[j] = sw[row * NB + fq];
+        else
+          sb[j] = *reinterpret_cast<const uint16_t *>(sw + row * NB + 2 * fq);
+      }
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int row = wm * (BM / 2) + 16 * i + fr;
+        i32x8 af[NS];
+        int sa;
+        if constexpr (F8) {
+          const u32x4 d = *reinterpret_cast<const u32x4 *>(st + row * 128 + ((fq ^ sw8) << 4));
+          const u32x4 e = *reinterpret_cast<const u32x4 *>(st + row * 128 + (((4 + fq) ^ sw8) << 4));
+          af[0] = i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, (int)e.x, (int)e.y, (int)e.z, (int)e.w};
+          sa = p.xsc ? sx[row * NB + fq] : unit;
+        } else {
+#pragma unroll
+          for (int s = 0; s < NS; ++s) af[s] = ld4(st + row * 128 + (((2 * fq + s) ^ sw8) << 4));
+          sa = *reinterpret_cast<const uint16_t *>(sx + row * NB + 2 * fq);
+        }
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[i][j] = pp_mma<F8>(bf[j][s], af[s], acc[i][j], s, sb[j], sa);
+      }
+      slot = slot == STAGES - 1 ? 0 : slot + 1;
+    }
+    wait_vm<0>();  // the re-loads past the end land before the workgroup's LDS is given away
+  }
+
+  const bool vec = p.N % 4 == 0 && ((uintptr_t)p.y & 15) == 0;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int64_t m = m0 + wm * (BM / 2) + 16 * i + fr;
+    if (m >= p.M) continue;
+    const float f = p.xf ? p.xf[m * p.xf_stride] : 1.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int64_t n = n0 + wn * (BN / 2) + 16 * j + 4 * fq;
+      if (p.splits > 1)
+        out4<float>(p.part + ((int64_t)split * p.M + m) * p.N, acc[i][j], 1.f, nullptr, 0, n, p.N, p.N % 4 == 0);
+      else
+        out4<T>(reinterpret_cast<T *>(p.y) + m * p.N, acc[i][j], f, p.bias, p.bias_f32, n, p.N, vec);
+    }
+  }
+}
+
+template <typename T> __global__ __launch_bounds__(256) void mx_join_kernel(MidArgs p) {
+  const int64_t groups = (p.N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / groups, n = 4 * (i - m * groups);
+  if (m >= p.M) return;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  const int64_t step = (int64_t)p.M * p.N;
+  const float *q = p.part + m * p.N + n;
+  if (p.N % 4 == 0) {
+    for (int s = 0; s < p.splits; ++s) v += *reinterpret_cast<const f32x4 *>(q + s * step);
+  } else {
+    for (int s = 0; s < p.splits; ++s)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (n + k < p.N) v[k] += q[s * step + k];
+  }
+  out4<T>(reinterpret_cast<T *>(p.y) + m * p.N, v, p.xf ? p.xf[m * p.xf_stride] : 1.f, p.bias, p.bias_f32, n, p.N,
+          p.N % 4 == 0 && ((uintptr_t)p.y & 15) == 0);
+}
+
+// exponents [rows][nb] -> [rows][stride], zero past nb
+__global__ __launch_bounds__(256) void mx_pad_scales_kernel(const uint8_t *__restrict__ s, int64_t rows, int nb, int stride,
+                                                            uint8_t *__restrict__ o) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = stride / 4, row = i / per;
+  const int b = 4 * (int)(i - row * per);
+  if (row >= rows) return;
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (b + j < nb) w |= (uint32_t)s[row * nb + b + j] << (8 * j);
+  *reinterpret_cast<uint32_t *>(o + row * stride + b) = w;
+}
+
 // exponents [rows][nb] -> [K tile][rows padded to 256][NB], 0 past the matrix
 template <int NB>
 __global__ __launch_bounds__(256) void mx_tile_scales_kernel(const uint8_t *__restrict__ s, int rows, int nb, int pad, int nt,
@@ -853,14 +1153,35 @@ bool is_mx(int kind) { return kind == MTQ_MXFP4 || kind == MTQ_MXFP8; }
 // up to this many rows a wave quantises its part of x in its own registers (mx_skinny_kernel FUSED)
 constexpr int kFusedRows = 16;
 // rows up to which the weight-streaming kernel is taken
-constexpr int kSkinnyRows = 64;
-bool use_pp(int64_t M, int64_t N, int64_t K) {
-  // 32-bit offsets inside a 256-row panel and inside the tiled exponents
+constexpr int kSkinnyRows = 16;  // = kFusedRows: one 16-row operand
+
+// which kernel, and its tile
+struct LinearPlan {
+  enum { kSkinny, kMid, kPp } form;
+  int bm, bn, splits;
+};
+LinearPlan linear_plan(int64_t M, int64_t N, int64_t K, int kind) {
+  LinearPlan p{LinearPlan::kSkinny, 0, 0, 1};
+  // 32-bit offsets inside a panel of 256 rows and inside the tiled exponents
   const int64_t pad = (M > N ? M : N) + kPpTile;
-  return M > kSkinnyRows && K <= (1 << 22) && pad * (K / 32 + 8) < (1ll << 31);
+  if (M <= kSkinnyRows || pad * (K / 32 + 8) >= (1ll << 31)) return p;
+  const int64_t cus = host_num_cus();
+  auto tiles = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  if (M > 128 && tiles(256, 256) * 4 >= cus * 3) {
+    p.form = LinearPlan::kPp;
+    return p;
+  }
+  p.form = LinearPlan::kMid;
+  p.bm = p.bn = M > 64 && tiles(128, 128) >= cus ? 128 : 64;
+  const int bk = pp_bk(kind != MTQ_MXFP4);
+  const int64_t nt = (K + bk - 1) / bk, have = tiles(p.bm, p.bn);
+  int64_t splits = have >= 2 * cus ? 1 : (2 * cus + have - 1) / have;
+  if (splits > nt / 4) splits = nt / 4;  // a split of fewer than 4 K tiles is mostly its start
+  p.splits = (int)(splits < 1 ? 1 : splits > 16 ? 16 : splits);
+  return p;
 }
 struct LinearWs {
-  size_t q, scale, xt, wt, bytes;  // offsets: codes and scales of x, both operands' tiled exponents
+  size_t q, scale, xt, wt, part, bytes;  // offsets: codes and scales of x, both operands' exponents laid out anew, splits
 };
 LinearWs linear_ws(int64_t M, int64_t N, int64_t K, int kind, bool quantise) {
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
@@ -868,14 +1189,33 @@ LinearWs linear_ws(int64_t M, int64_t N, int64_t K, int kind, bool quantise) {
   w.q = 0;
   w.scale = quantise ? up((size_t)M * (kind == MTQ_MXFP4 ? K / 2 : K)) : 0;
   w.xt = w.scale + (quantise ? up(is_mx(kind) ? (size_t)M * (K / 32) : kind == MTQ_FP8_TOKEN ? 4 * (size_t)M : 4) : 0);
-  w.wt = w.bytes = w.xt;
-  if (use_pp(M, N, K)) {
-    const int bk = pp_bk(kind != MTQ_MXFP4);
-    const size_t nt = (size_t)((K + bk - 1) / bk);
-    w.wt = w.xt + (is_mx(kind) ? nt * up(M) * (bk / 32) : 0);
-    w.bytes = w.wt + nt * up(N) * (bk / 32);
+  w.wt = w.part = w.bytes = w.xt;
+  const LinearPlan p = linear_plan(M, N, K, kind);
+  const int bk = pp_bk(kind != MTQ_MXFP4);
+  const size_t nt = (size_t)((K + bk - 1) / bk), per = nt * (bk / 32);
+  if (p.form == LinearPlan::kPp) {
+    w.wt = w.xt + (is_mx(kind) ? up(M) * per : 0);
+    w.part = w.bytes = w.wt + up(N) * per;
+  } else if (p.form == LinearPlan::kMid) {
+    if (K % bk) {  // rows of exponents padded to whole K tiles
+      w.wt = w.xt + (is_mx(kind) ? up((size_t)M * per) : 0);
+      w.part = w.wt + up((size_t)N * per);
+    }
+    w.bytes = w.part + (p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0);
   }
   return w;
+}
+template <typename T, bool F8> int launch_mid(MidArgs a, const LinearPlan &p, hipStream_t stream) {
+  a.tiles_m = (a.M + p.bm - 1) / p.bm, a.tiles_n = (a.N + p.bn - 1) / p.bn, a.splits = p.splits;
+  const unsigned g = (unsigned)((int64_t)a.tiles_m * a.tiles_n * a.splits);
+  if (p.bm == 128)
+    mx_mid_kernel<T, F8, 128, 128, 2><<<g, 256, 0, stream>>>(a);
+  else
+    mx_mid_kernel<T, F8, 64, 64, 4><<<g, 256, 0, stream>>>(a);
+  int st = host_check_launch();
+  if (st != MTQ_OK || a.splits == 1) return st;
+  mx_join_kernel<T><<<(unsigned)(((int64_t)a.M * ((a.N + 3) / 4) + 255) / 256), 256, 0, stream>>>(a);
+  return host_check_launch();
 }
 template <bool F8> int launch_tile_scales(const uint8_t *s, int rows, int K, uint8_t *o, hipStream_t stream) {
   constexpr int BK = pp_bk(F8);
@@ -951,10 +1291,10 @@ int mtq_mx_linear(const void *x, int64_t x_stride, int x_dtype, const void *x_sc
   if (y_dtype != MTQ_BF16 && y_dtype != MTQ_F16 && y_dtype != MTQ_F32) return MTQ_ERR_DTYPE;
   if (x_dtype >= 0 && x_dtype != MTQ_BF16 && x_dtype != MTQ_F16 && x_dtype != MTQ_F32) return MTQ_ERR_DTYPE;
   if (bias && bias_dtype != y_dtype && bias_dtype != MTQ_F32) return MTQ_ERR_DTYPE;
-  if (M < 0 || N < 1 || K < 32 || K % 32 || M > (1 << 24) || N > (1 << 24) || K > (1 << 24)) return MTQ_ERR_INVALID_ARG;
+  if (M < 0 || N < 1 || K < 32 || K % 32 || M > (1 << 24) || N > (1 << 24) || K > (1 << 22)) return MTQ_ERR_INVALID_ARG;
   if (M == 0) return MTQ_OK;
-  if (!x || !w || !w_scale || !y || !al16(w)) return MTQ_ERR_INVALID_ARG;
-  if (x_dtype < 0 ? !x_scale || !al16(x) : (M > 1 && x_stride < K) || (kind == MTQ_FP8_TENSOR && !amax)) return MTQ_ERR_INVALID_ARG;
+  if (!x || !w || !w_scale || !y || !al16(w) || (uintptr_t)w_scale % 4) return MTQ_ERR_INVALID_ARG;
+  if (x_dtype < 0 ? !x_scale || !al16(x) || (uintptr_t)x_scale % 4 : (M > 1 && x_stride < K) || (kind == MTQ_FP8_TENSOR && !amax)) return MTQ_ERR_INVALID_ARG;
   SkinnyArgs a{};
   a.w = w, a.wsc = w_scale, a.bias = bias, a.y = y, a.M = (int)M, a.N = (int)N, a.K = (int)K;
   a.bias_f32 = bias && bias_dtype == MTQ_F32;
@@ -980,17 +1320,37 @@ int mtq_mx_linear(const void *x, int64_t x_stride, int x_dtype, const void *x_sc
     a.xf = (const float *)x_scale;
     a.xf_stride = kind == MTQ_FP8_TOKEN;
   }
-  if (use_pp(M, N, K)) {
+  const LinearPlan plan = linear_plan(M, N, K, kind);
+  if (plan.form != LinearPlan::kSkinny) {
     const bool f8 = kind != MTQ_MXFP4;
-    uint8_t *xt = is_mx(kind) ? (uint8_t *)ws + o.xt : nullptr, *wt = (uint8_t *)ws + o.wt;
+    const int bk = pp_bk(f8), nb = (int)(K / 32), per = (int)((K + bk - 1) / bk * (bk / 32));
+    const uint8_t *xt = a.xsc, *wt = w_scale;
     int st = MTQ_OK;
-    if (xt) st = f8 ? launch_tile_scales<true>(a.xsc, a.M, a.K, xt, stream) : launch_tile_scales<false>(a.xsc, a.M, a.K, xt, stream);
-    if (st == MTQ_OK) st = f8 ? launch_tile_scales<true>(w_scale, a.N, a.K, wt, stream) : launch_tile_scales<false>(w_scale, a.N, a.K, wt, stream);
+    auto lay = [&](const uint8_t *&s, int64_t rows, size_t off) {
+      if (!s || st != MTQ_OK) return;
+      uint8_t *d = (uint8_t *)ws + off;
+      if (plan.form == LinearPlan::kPp) {
+        st = f8 ? launch_tile_scales<true>(s, (int)rows, a.K, d, stream) : launch_tile_scales<false>(s, (int)rows, a.K, d, stream);
+      } else if (K % bk) {
+        mx_pad_scales_kernel<<<(unsigned)((rows * (per / 4) + 255) / 256), 256, 0, stream>>>(s, rows, nb, per, d);
+        st = host_check_launch();
+      } else {
+        return;  // as they are (4-byte aligned: checked)
+      }
+      s = d;
+    };
+    lay(xt, M, o.xt);
+    lay(wt, N, o.wt);
     if (st != MTQ_OK) return st;
-    const PpArgs p{(const uint8_t *)x, w, xt, wt, a.xf, bias, y, a.M, a.N, a.K, 0, 0, a.xf_stride, a.bias_f32};
     auto go = [&](auto t) {
       using T = decltype(t);
-      return f8 ? launch_pp<T, true>(p, stream) : launch_pp<T, false>(p, stream);
+      if (plan.form == LinearPlan::kPp) {
+        const PpArgs p{(const uint8_t *)x, w, xt, wt, a.xf, bias, y, a.M, a.N, a.K, 0, 0, a.xf_stride, a.bias_f32};
+        return f8 ? launch_pp<T, true>(p, stream) : launch_pp<T, false>(p, stream);
+      }
+      const MidArgs p{(const uint8_t *)x, w, xt, wt, a.xf, bias, y, (float *)((uint8_t *)ws + o.part), a.M, a.N, a.K, 0, 0, per, per,
+                      a.xf_stride, a.bias_f32, 1};
+      return f8 ? launch_mid<T, true>(p, plan, stream) : launch_mid<T, false>(p, plan, stream);
     };
     return y_dtype == MTQ_BF16 ? go(__bf16{}) : y_dtype == MTQ_F16 ? go(_Float16{}) : go(float{});
   }

@@ -1303,6 +1303,7 @@ at::Tensor mx_linear(const at::Tensor &x, const c10::optional<at::Tensor> &x_sca
                           x_scale->device() == x.device(),
                       what, ": x_scale does not fit the format");
     xs = x_scale->contiguous();
+    if ((uintptr_t)xs.data_ptr() % 4) xs = xs.clone();
   } else {
     check_float_rows(x, what);
   }
@@ -1323,7 +1324,7 @@ at::Tensor mx_linear(const at::Tensor &x, const c10::optional<at::Tensor> &x_sca
     at::Tensor c = t.contiguous();
     return (uintptr_t)c.data_ptr() % 16 ? c.clone() : c;
   };
-  const at::Tensor v = packed ? dense16(x) : as_rows(x), wc = dense16(w), wsc = w_scale.contiguous();
+  const at::Tensor v = packed ? dense16(x) : as_rows(x), wc = dense16(w), wsc = dense16(w_scale);
   const int xd = packed ? -1 : dtype_code(x.scalar_type());
   const size_t nb = mtq_mx_linear_workspace_bytes(M, N, K, kind, xd);
   at::Tensor ws = nb ? at::empty({(int64_t)nb}, x.options().dtype(at::kByte)) : at::Tensor();
