@@ -282,6 +282,47 @@ template <typename T> int launch_norm_k(const NormArgs &a, int kind, bool vec, i
   }
 }
 
+// v_cvt_scalef32_pk_fp4_{bf16,f16} into byte SEL of a dword of codes
+template <typename T> struct Fp4Pair;
+template <> struct Fp4Pair<__bf16> {
+  typedef bf16x2_t v2;
+  template <int SEL> static __device__ __forceinline__ uint32_t cvt(uint32_t w, v2 p, float s) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, p, s, SEL);
+  }
+};
+template <> struct Fp4Pair<_Float16> {
+  typedef f16x2_t v2;
+  template <int SEL> static __device__ __forceinline__ uint32_t cvt(uint32_t w, v2 p, float s) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, p, s, SEL);
+  }
+};
+
+// 8 packed 16-bit values of one lane, 4 lanes a block: MXFP4 codes as block_codes() below makes them
+template <typename T>
+__device__ __forceinline__ void mxfp4_store8_packed(const u32x4 &x, int64_t col, uint8_t *q, uint8_t *sc, bool live) {
+  u16x2_t mx = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) mx = __builtin_elementwise_max(mx, __builtin_bit_cast(u16x2_t, x[j] & 0x7fff7fffu));
+  const uint32_t mb = group_max_u32<4>(mx.x > mx.y ? mx.x : mx.y);
+  float un, scale;
+  e8m0_scale(mb >= Fp4Native<T>::kInfBits ? 3.402823466e38f : half_bits_to_float<T>(mb), 6.0f, scale, un);
+  if (mb <= Fp4Native<T>::kInfBits && un >= 0x1p-100f && un <= 0x1p100f) {  // uniform over the block's lanes
+    if (!live) return;
+    uint32_t w = 0;
+    w = Fp4Pair<T>::template cvt<0>(w, __builtin_bit_cast(typename Fp4Pair<T>::v2, (uint32_t)x[0]), un);
+    w = Fp4Pair<T>::template cvt<1>(w, __builtin_bit_cast(typename Fp4Pair<T>::v2, (uint32_t)x[1]), un);
+    w = Fp4Pair<T>::template cvt<2>(w, __builtin_bit_cast(typename Fp4Pair<T>::v2, (uint32_t)x[2]), un);
+    w = Fp4Pair<T>::template cvt<3>(w, __builtin_bit_cast(typename Fp4Pair<T>::v2, (uint32_t)x[3]), un);
+    *reinterpret_cast<uint32_t *>(q + col / 2) = w;
+    if ((col & 31) == 0) sc[col / 32] = (uint8_t)((__float_as_uint(un) >> 23) & 0xff);
+  } else {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[2 * j] = half_bits_to_float<T>(x[j] & 0xffffu), v[2 * j + 1] = half_bits_to_float<T>(x[j] >> 16);
+    mx_store8<MTQ_MXFP4>(v, col, q, sc, live);
+  }
+}
+
 // ---- quantising rows ---------------------------------------------------------------------------
 // MX and per-tensor FP8: 8 values a lane over all rows (a block's 4 lanes are neighbours).
 template <typename T, int KIND, bool VEC>
@@ -292,6 +333,12 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ 
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t row = i / gpr, col = (i - row * gpr) * 8;
   const bool live = row < rows;
+  if constexpr (KIND == MTQ_MXFP4 && VEC && sizeof(T) == 2) {
+    u32x4 w = {0, 0, 0, 0};
+    if (live) w = *reinterpret_cast<const u32x4 *>(x + row * xs + col);
+    mxfp4_store8_packed<T>(w, col, q + row * (cols / 2), reinterpret_cast<uint8_t *>(scale) + row * (cols / 32), live);
+    return;
+  }
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (live) load8<T, VEC>(x + row * xs, col, cols, v);
   if constexpr (KIND == MTQ_FP8_TENSOR) {
@@ -352,41 +399,24 @@ int launch_quantize(const T *x, int64_t xs, int64_t rows, int64_t cols, int kind
 
 // 4 consecutive columns of a row of y: v * f + bias, rounded once
 template <typename T>
-__device__ __forceinline__ void out4(T *y, const f32x4 &v, float f, const void *bias, int bias_f32, int64_t n, int N, bool vec) {
+__device__ __forceinline__ void out4(T *y, const f32x4 &v, float f, const void *bias, int bias_f32, int64_t n, int N) {
   float o[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     o[k] = v[k] * f;
     if (bias && n + k < N) o[k] += bias_f32 ? reinterpret_cast<const float *>(bias)[n + k] : Elem<T>::ld(reinterpret_cast<const T *>(bias)[n + k]);
   }
-  if (vec) {  // N % 4 == 0, y aligned: the 4 columns are all in or all out
-    struct alignas(4 * sizeof(T)) Pack {
-      T e[4];
-    } pk;
+  if (n + 4 <= N) {  // one store, of any alignment (rows of an odd N)
+    T e[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) pk.e[k] = Elem<T>::st(o[k]);
-    if (n < N) *reinterpret_cast<Pack *>(y + n) = pk;
+    for (int k = 0; k < 4; ++k) e[k] = Elem<T>::st(o[k]);
+    __builtin_memcpy(y + n, e, sizeof(e));
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (n + k < N) y[n + k] = Elem<T>::st(o[k]);
   }
 }
-
-// v_cvt_scalef32_pk_fp4_{bf16,f16} into byte SEL of a dword of codes
-template <typename T> struct Fp4Pair;
-template <> struct Fp4Pair<__bf16> {
-  typedef bf16x2_t v2;
-  template <int SEL> static __device__ __forceinline__ uint32_t cvt(uint32_t w, v2 p, float s) {
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, p, s, SEL);
-  }
-};
-template <> struct Fp4Pair<_Float16> {
-  typedef f16x2_t v2;
-  template <int SEL> static __device__ __forceinline__ uint32_t cvt(uint32_t w, v2 p, float s) {
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, p, s, SEL);
-  }
-};
 
 // 32 values of one lane in 16 packed 16-bit pairs -> its block's E2M1 codes and exponent byte: the
 // largest magnitude from packed integer maxima of the bit patterns (NaN patterns sort above infinity),
@@ -472,7 +502,7 @@ __device__ __forceinline__ u32x4 load16_any(const uint8_t *p) {  // any alignmen
 }
 
 template <typename T, int OP, int NT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void mx_skinny_kernel(SkinnyArgs a) {
+__global__ __launch_bounds__(64 * WAVES, OP == kOpFused && NT == 2 ? 2 : 4) void mx_skinny_kernel(SkinnyArgs a) {
   __shared__ f32x4 red[WAVES][NT][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
   const int n0 = (blockIdx.x % a.tiles_n) * 16 * NT, m0 = (blockIdx.x / a.tiles_n) * 16;
@@ -579,7 +609,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void mx_skinny_kernel(SkinnyArgs a) 
     for (int w = 1; w < WAVES; ++w) v += red[w][wave][lane];
     if (m < a.M) {
       const float f = a.xf ? a.xf[(int64_t)m * a.xf_stride] : 1.f;
-      out4<T>(reinterpret_cast<T *>(a.y) + (int64_t)m * a.N, v, f, a.bias, a.bias_f32, n, a.N, a.N % 4 == 0 && ((uintptr_t)a.y & 15) == 0);
+      out4<T>(reinterpret_cast<T *>(a.y) + (int64_t)m * a.N, v, f, a.bias, a.bias_f32, n, a.N);
     }
   }
 }
@@ -647,15 +677,12 @@ template <bool F8> __device__ __forceinline__ f32x4 pp_mma(const i32x8 &w, const
 }
 
 // one lane's 8 values of a row of y
-template <typename T> __device__ __forceinline__ void pp_store8(T *y, const float (&v)[8], int64_t n, int N, bool vec) {
-  if (vec && n + 8 <= N) {
+template <typename T> __device__ __forceinline__ void pp_store8(T *y, const float (&v)[8], int64_t n, int N) {
+  if (n + 8 <= N) {  // one store (fp32: two), of any alignment (rows of an odd N)
+    T e[8];
 #pragma unroll
-    for (int k = 0; k < 8; k += Vec<T>::N) {
-      Vec<T> o;
-#pragma unroll
-      for (int e = 0; e < Vec<T>::N; ++e) o.e[e] = Elem<T>::st(v[k + e]);
-      stg_vec(y + n + k, o);
-    }
+    for (int k = 0; k < 8; ++k) e[k] = Elem<T>::st(v[k]);
+    __builtin_memcpy(y + n, e, sizeof(e));
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
@@ -802,7 +829,6 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
     return *reinterpret_cast<const uint16_t *>(base + row * NB + 2 * fq);
   };
 
-  const bool vec = (p.N * sizeof(T)) % 16 == 0 && ((uintptr_t)p.y & 15) == 0;
   int id = blockIdx.x;
   if (!next_tile(id)) return;  // the whole workgroup, before any barrier
   set_tile();
@@ -919,7 +945,7 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
       const float f = __shfl(i < 8 ? f0 : f1, (8 * i + orow) & 63, 64);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = (k < 4 ? lo[k] : hi[k - 4]) * f + bias[k];
-      if (m < p.M) pp_store8<T>(reinterpret_cast<T *>(p.y) + m * p.N, v, n, p.N, vec);
+      if (m < p.M) pp_store8<T>(reinterpret_cast<T *>(p.y) + m * p.N, v, n, p.N);
       __builtin_amdgcn_wave_barrier();
     }
   }
@@ -1077,7 +1103,6 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MidArgs p) {
     wait_vm<0>();  // the re-loads past the end land before the workgroup's LDS is given away
   }
 
-  const bool vec = p.N % 4 == 0 && ((uintptr_t)p.y & 15) == 0;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int64_t m = m0 + wm * (BM / 2) + 16 * i + fr;
@@ -1087,9 +1112,9 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MidArgs p) {
     for (int j = 0; j < NJ; ++j) {
       const int64_t n = n0 + wn * (BN / 2) + 16 * j + 4 * fq;
       if (p.splits > 1)
-        out4<float>(p.part + ((int64_t)split * p.M + m) * p.N, acc[i][j], 1.f, nullptr, 0, n, p.N, p.N % 4 == 0);
+        out4<float>(p.part + ((int64_t)split * p.M + m) * p.N, acc[i][j], 1.f, nullptr, 0, n, p.N);
       else
-        out4<T>(reinterpret_cast<T *>(p.y) + m * p.N, acc[i][j], f, p.bias, p.bias_f32, n, p.N, vec);
+        out4<T>(reinterpret_cast<T *>(p.y) + m * p.N, acc[i][j], f, p.bias, p.bias_f32, n, p.N);
     }
   }
 }
@@ -1108,8 +1133,7 @@ template <typename T> __global__ __launch_bounds__(256) void mx_join_kernel(MidA
       for (int k = 0; k < 4; ++k)
         if (n + k < p.N) v[k] += q[s * step + k];
   }
-  out4<T>(reinterpret_cast<T *>(p.y) + m * p.N, v, p.xf ? p.xf[m * p.xf_stride] : 1.f, p.bias, p.bias_f32, n, p.N,
-          p.N % 4 == 0 && ((uintptr_t)p.y & 15) == 0);
+  out4<T>(reinterpret_cast<T *>(p.y) + m * p.N, v, p.xf ? p.xf[m * p.xf_stride] : 1.f, p.bias, p.bias_f32, n, p.N);
 }
 
 // exponents [rows][nb] -> [rows][stride], zero past nb
@@ -1172,7 +1196,8 @@ LinearPlan linear_plan(int64_t M, int64_t N, int64_t K, int kind) {
     return p;
   }
   p.form = LinearPlan::kMid;
-  p.bm = p.bn = M > 64 && tiles(128, 128) >= cus ? 128 : 64;
+  p.bm = M > 64 && tiles(128, 128) >= cus ? 128 : 64;
+  p.bn = p.bm == 128 || tiles(64, 128) * 4 >= cus * 3 ? 128 : 64;
   const int bk = pp_bk(kind != MTQ_MXFP4);
   const int64_t nt = (K + bk - 1) / bk, have = tiles(p.bm, p.bn);
   int64_t splits = have >= 2 * cus ? 1 : (2 * cus + have - 1) / have;
@@ -1209,7 +1234,9 @@ template <typename T, bool F8> int launch_mid(MidArgs a, const LinearPlan &p, hi
   a.tiles_m = (a.M + p.bm - 1) / p.bm, a.tiles_n = (a.N + p.bn - 1) / p.bn, a.splits = p.splits;
   const unsigned g = (unsigned)((int64_t)a.tiles_m * a.tiles_n * a.splits);
   if (p.bm == 128)
-    mx_mid_kernel<T, F8, 128, 128, 2><<<g, 256, 0, stream>>>(a);
+    mx_mid_kernel<T, F8, 128, 128, F8 ? 3 : 2><<<g, 256, 0, stream>>>(a);
+  else if (p.bn == 128)
+    mx_mid_kernel<T, F8, 64, 128, F8 ? 4 : 3><<<g, 256, 0, stream>>>(a);
   else
     mx_mid_kernel<T, F8, 64, 64, 4><<<g, 256, 0, stream>>>(a);
   int st = host_check_launch();
