@@ -502,7 +502,7 @@ __device__ __forceinline__ u32x4 load16_any(const uint8_t *p) {  // any alignmen
 }
 
 template <typename T, int OP, int NT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, OP == kOpFused && NT == 2 ? 2 : 4) void mx_skinny_kernel(SkinnyArgs a) {
+__global__ __launch_bounds__(64 * WAVES, NT == 4 ? 2 : 4) void mx_skinny_kernel(SkinnyArgs a) {
   __shared__ f32x4 red[WAVES][NT][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
   const int n0 = (blockIdx.x % a.tiles_n) * 16 * NT, m0 = (blockIdx.x / a.tiles_n) * 16;
@@ -615,15 +615,18 @@ __global__ __launch_bounds__(64 * WAVES, OP == kOpFused && NT == 2 ? 2 : 4) void
 }
 
 template <typename T, int OP> int launch_skinny(SkinnyArgs a, hipStream_t stream) {
-  // two tiles of W share a read (and FUSED: the quantisation) of xq where that leaves a workgroup for every CU
-  const int64_t gm = (a.M + 15) / 16;
-  if (a.N >= 32 * host_num_cus()) {
-    a.tiles_n = (a.N + 31) / 32;
-    mx_skinny_kernel<T, OP, 2, 8><<<(unsigned)(gm * a.tiles_n), 64 * 8, 0, stream>>>(a);
-  } else {
-    a.tiles_n = (a.N + 15) / 16;
-    mx_skinny_kernel<T, OP, 1, 8><<<(unsigned)(gm * a.tiles_n), 64 * 8, 0, stream>>>(a);
+  // tiles of W that share a read of xq: four where that leaves a workgroup for nearly every CU (16 rows of
+  // E4M3 against 28672 x 8192: 33 us, two 40, one 49), one where there are too few of them
+  const int64_t gm = (a.M + 15) / 16, cus = host_num_cus();
+  if constexpr (OP != kOpFused) {
+    if (a.N >= 48 * cus) {
+      a.tiles_n = (a.N + 63) / 64;
+      mx_skinny_kernel<T, OP, 4, 4><<<(unsigned)(gm * a.tiles_n), 64 * 4, 0, stream>>>(a);
+      return host_check_launch();
+    }
   }
+  a.tiles_n = (a.N + 15) / 16;
+  mx_skinny_kernel<T, OP, 1, 8><<<(unsigned)(gm * a.tiles_n), 64 * 8, 0, stream>>>(a);
   return host_check_launch();
 }
 
@@ -638,10 +641,11 @@ template <typename T, int OP> int launch_skinny(SkinnyArgs a, hipStream_t stream
 // behind waves 0-3, so that one wave of a SIMD reads LDS while the other multiplies.
 // The exponent bytes are laid out by K tile first ([K tile][row][BK / 32], zero past the matrix; one
 // small pass per operand), so a tile's are two DMAs a wave into a ring of three; a lane's exponents of
-// both 128-column steps are one 16-bit read, its blocks of a K tile being 2 g and 2 g + 1 (the
-// order in which the columns of a K tile are multiplied is free).
-// LDS rows are 16-byte chunks stored at chunk ^ (row bits) (the XOR is applied to the global
-// address): conflict-free fragment reads.
+// both 128-column steps are one 16-bit read (bytes 2 g + s for its block 4 s + g).
+// LDS rows are 16-byte chunks stored at chunk ^ f(row) (the XOR is applied to the global address),
+// f = row / 2 for 128-byte rows and -(row / 4) for 64-byte ones: a 128-bit read serves lanes 0-3, 12-15
+// and 20-27 together (then the others of 0-31), whose 16 chunks then fall on different banks
+// (SQ_LDS_BANK_CONFLICT 39 % -> 5 % of the LDS cycles against blocks 2 g + s, 266 -> 260 us).
 // Columns past K (K % BK != 0): chunks there are read from the row's first chunk of the tile, and
 // their exponents are 2^-127 on both sides, so what they add vanishes (below 2^-230).
 struct PpArgs {
@@ -711,7 +715,7 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
   const int xpad = p.tiles_m * kPpTile, wpad = p.tiles_n * kPpTile;  // rows of the tiled exponents
   const int xs_step = (p.xsc ? xpad : wpad) * NB, ws_step = wpad * NB;
   const int a_chunk = (lane & 7) ^ (((wave * 8 + (lane >> 3)) >> 1) & 7);
-  const int b_chunk = F8 ? (lane & 3) ^ ((lane >> 4) & 3) : a_chunk;
+  const int b_chunk = F8 ? (lane & 3) ^ (-(lane >> 4) & 3) : a_chunk;
   // what to step back by where the chunk lies past K in the last tile (a chunk: 16 columns of E4M3, 32 of E2M1)
   const unsigned a_tail = (nt - 1) * BK + a_chunk * (F8 ? 16 : 32) < p.K ? 0 : a_chunk * 16;
   const unsigned b_tail = (nt - 1) * BK + b_chunk * 32 < p.K ? 0 : b_chunk * 16;
@@ -803,9 +807,9 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
     load_a(0, 1);
   };
 
-  // ---- fragments.  E2M1 operand, step s: block 2 fq + s (E4M3 form: block fq of 4); E4M3 operand:
+  // ---- fragments.  E2M1 operand, step s: block 4 s + fq (E4M3 form: block fq of 4); E4M3 operand:
   // columns 16 fq .. and 64 + 16 fq ..
-  const int sw8 = (lane >> 1) & 7, sw4 = (lane >> 2) & 3;
+  const int sw8 = (lane >> 1) & 7, sw4 = -(fr >> 2) & 3;
   auto ld4 = [&](const unsigned char *q) -> i32x8 {
     const u32x4 d = *reinterpret_cast<const u32x4 *>(q);
     return i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, 0, 0, 0, 0};
@@ -817,12 +821,12 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
       const u32x4 e = *reinterpret_cast<const u32x4 *>(row + (((4 + fq) ^ sw8) << 4));
       return i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, (int)e.x, (int)e.y, (int)e.z, (int)e.w};
     } else {
-      return ld4(row + (((2 * fq + s) ^ sw8) << 4));
+      return ld4(row + (((4 * s + fq) ^ sw8) << 4));
     }
   };
   auto read_b = [&](const unsigned char *buf, int j, int s) -> i32x8 {
     const unsigned char *row = buf + 2 * AH + (j >> 1) * BH + (wn * 32 + (j & 1) * 16 + fr) * (BK / 2);
-    return ld4(row + (F8 ? (fq ^ sw4) << 4 : ((2 * fq + s) ^ sw8) << 4));
+    return ld4(row + (F8 ? (fq ^ sw4) << 4 : ((4 * s + fq) ^ sw8) << 4));
   };
   auto read_s = [&](const unsigned char *base, int row) -> int {
     if constexpr (F8) return base[row * NB + fq];
@@ -994,7 +998,7 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MidArgs p) {
   // ---- DMA sources.  Operand rows of 128 bytes: LDS row u * 32 + wave * 8 + lane / 8, chunk slot lane % 8; of 64
   // bytes: u * 64 + wave * 16 + lane / 4, slot lane % 4.  Rows past the matrix re-read its last one.
   const int a_chunk = (lane & 7) ^ (((wave * 8 + (lane >> 3)) >> 1) & 7);
-  const int b_chunk = F8 ? (lane & 3) ^ ((lane >> 4) & 3) : a_chunk;
+  const int b_chunk = F8 ? (lane & 3) ^ (-(lane >> 4) & 3) : a_chunk;
   unsigned a_off[AU], b_off[BU], s_off[SI];
 #pragma unroll
   for (int u = 0; u < AU; ++u) {
@@ -1045,7 +1049,7 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MidArgs p) {
     }
   };
 
-  const int sw8 = (fr >> 1) & 7, sw4 = (fr >> 2) & 3;
+  const int sw8 = (fr >> 1) & 7, sw4 = -(fr >> 2) & 3;
   auto ld4 = [&](const unsigned char *q) -> i32x8 {
     const u32x4 d = *reinterpret_cast<const u32x4 *>(q);
     return i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, 0, 0, 0, 0};
@@ -1067,36 +1071,45 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MidArgs p) {
       const unsigned char *st = lds + slot * STAGE, *sx = st + AB + BB, *sw = sx + SA;
       const int unit = F8 && !p.xsc ? ((t == nt_all - 1 && k_last + 32 * fq >= p.K) ? 0 : 127) : 0;
       i32x8 bf[NJ][NS];
-      int sb[NJ];
+      int sb[NJ][NS];
+      // exponent byte of block 4 s + fq in a lane's lowest byte
+      auto read_s = [&](const unsigned char *row, int (&e)[NS]) {
+        if constexpr (F8) {
+          e[0] = row[fq];
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2 *>(row);
+          e[0] = (int)(v.x >> (8 * fq)), e[1] = (int)(v.y >> (8 * fq));
+        }
+      };
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int row = wn * (BN / 2) + 16 * j + fr;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) bf[j][s] = ld4(st + AB + row * WR + (F8 ? (fq ^ sw4) << 4 : ((2 * fq + s) ^ sw8) << 4));
-        if constexpr (F8)
-          sb[j] = sw[row * NB + fq];
-        else
-          sb[j] = *reinterpret_cast<const uint16_t *>(sw + row * NB + 2 * fq);
+        for (int s = 0; s < NS; ++s) bf[j][s] = ld4(st + AB + row * WR + (F8 ? (fq ^ sw4) << 4 : ((4 * s + fq) ^ sw8) << 4));
+        read_s(sw + row * NB, sb[j]);
       }
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int row = wm * (BM / 2) + 16 * i + fr;
         i32x8 af[NS];
-        int sa;
+        int sa[NS];
         if constexpr (F8) {
           const u32x4 d = *reinterpret_cast<const u32x4 *>(st + row * 128 + ((fq ^ sw8) << 4));
           const u32x4 e = *reinterpret_cast<const u32x4 *>(st + row * 128 + (((4 + fq) ^ sw8) << 4));
           af[0] = i32x8{(int)d.x, (int)d.y, (int)d.z, (int)d.w, (int)e.x, (int)e.y, (int)e.z, (int)e.w};
-          sa = p.xsc ? sx[row * NB + fq] : unit;
+          if (p.xsc)
+            read_s(sx + row * NB, sa);
+          else
+            sa[0] = unit;
         } else {
 #pragma unroll
-          for (int s = 0; s < NS; ++s) af[s] = ld4(st + row * 128 + (((2 * fq + s) ^ sw8) << 4));
-          sa = *reinterpret_cast<const uint16_t *>(sx + row * NB + 2 * fq);
+          for (int s = 0; s < NS; ++s) af[s] = ld4(st + row * 128 + (((4 * s + fq) ^ sw8) << 4));
+          read_s(sx + row * NB, sa);
         }
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) acc[i][j] = pp_mma<F8>(bf[j][s], af[s], acc[i][j], s, sb[j], sa);
+          for (int j = 0; j < NJ; ++j) acc[i][j] = pp_mma<F8>(bf[j][s], af[s], acc[i][j], 0, sb[j][s], sa[s]);
       }
       slot = slot == STAGES - 1 ? 0 : slot + 1;
     }
@@ -1163,7 +1176,8 @@ __global__ __launch_bounds__(256) void mx_tile_scales_kernel(const uint8_t *__re
     w[k] = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int b = t * NB + 4 * k + j;
+      // E2M1: a lane's two blocks 4 s + g of a K tile next to each other
+      const int at = 4 * k + j, b = t * NB + (NB == 8 ? (at >> 1) + 4 * (at & 1) : at);
       if (row < rows && b < nb) w[k] |= (uint32_t)s[row * nb + b] << (8 * j);
     }
   }
@@ -1174,10 +1188,13 @@ __global__ __launch_bounds__(256) void mx_tile_scales_kernel(const uint8_t *__re
 
 bool is_mx(int kind) { return kind == MTQ_MXFP4 || kind == MTQ_MXFP8; }
 
-// up to this many rows a wave quantises its part of x in its own registers (mx_skinny_kernel FUSED)
-constexpr int kFusedRows = 16;
 // rows up to which the weight-streaming kernel is taken
-constexpr int kSkinnyRows = 16;  // = kFusedRows: one 16-row operand
+constexpr int kSkinnyRows = 16;  // one 16-row operand
+// MXFP4 rows of at most 8 tokens against at most 16 MiB of W: quantised by every workgroup for itself, in
+// registers (kOpFused); else once, by a launch of its own.  us, fused / in two launches:
+// 4096 x 4096: 1 row 6.0 / 7.6, 8 rows 6.9 / 7.2, 16 rows 8.1 / 7.4; 14336 x 4096: 1 row 11.9 / 10.1
+constexpr int kFusedRows = 8;
+constexpr int64_t kFusedWeights = 1 << 25;
 
 // which kernel, and its tile
 struct LinearPlan {
@@ -1200,7 +1217,7 @@ LinearPlan linear_plan(int64_t M, int64_t N, int64_t K, int kind) {
   p.bn = p.bm == 128 || tiles(64, 128) * 4 >= cus * 3 ? 128 : 64;
   const int bk = pp_bk(kind != MTQ_MXFP4);
   const int64_t nt = (K + bk - 1) / bk, have = tiles(p.bm, p.bn);
-  int64_t splits = have >= 2 * cus ? 1 : (2 * cus + have - 1) / have;
+  int64_t splits = have * 4 >= 3 * cus ? 1 : (2 * cus + have - 1) / have;
   if (splits > nt / 4) splits = nt / 4;  // a split of fewer than 4 K tiles is mostly its start
   p.splits = (int)(splits < 1 ? 1 : splits > 16 ? 16 : splits);
   return p;
@@ -1238,7 +1255,7 @@ template <typename T, bool F8> int launch_mid(MidArgs a, const LinearPlan &p, hi
   else if (p.bn == 128)
     mx_mid_kernel<T, F8, 64, 128, F8 ? 4 : 3><<<g, 256, 0, stream>>>(a);
   else
-    mx_mid_kernel<T, F8, 64, 64, 4><<<g, 256, 0, stream>>>(a);
+    mx_mid_kernel<T, F8, 64, 64, 3><<<g, 256, 0, stream>>>(a);
   int st = host_check_launch();
   if (st != MTQ_OK || a.splits == 1) return st;
   mx_join_kernel<T><<<(unsigned)(((int64_t)a.M * ((a.N + 3) / 4) + 255) / 256), 256, 0, stream>>>(a);
@@ -1326,7 +1343,7 @@ int mtq_mx_linear(const void *x, int64_t x_stride, int x_dtype, const void *x_sc
   a.w = w, a.wsc = w_scale, a.bias = bias, a.y = y, a.M = (int)M, a.N = (int)N, a.K = (int)K;
   a.bias_f32 = bias && bias_dtype == MTQ_F32;
   const bool vec = x_dtype >= 0 && x_dtype != MTQ_F32 && al16(x) && (M == 1 || x_stride % 8 == 0);
-  const bool fused = vec && kind == MTQ_MXFP4 && M <= kFusedRows && x_dtype == y_dtype;
+  const bool fused = vec && kind == MTQ_MXFP4 && M <= kFusedRows && N * K <= kFusedWeights && x_dtype == y_dtype;
   if (fused) {
     a.x = x, a.xs = x_stride;
     return y_dtype == MTQ_BF16 ? launch_skinny<__bf16, kOpFused>(a, stream) : launch_skinny<_Float16, kOpFused>(a, stream);
