@@ -1077,8 +1077,7 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MidArgs p) {
         if constexpr (F8) {
           e[0] = row[fq];
         } else {
-          const uint2 v = *reinterpret_cast<const uint2 *>(row);
-          e[0] = (int)(v.x >> (8 * fq)), e[1] = (int)(v.y >> (8 * fq));
+          e[0] = row[fq], e[1] = row[4 + fq];
         }
       };
 #pragma unroll
@@ -1251,7 +1250,7 @@ template <typename T, bool F8> int launch_mid(MidArgs a, const LinearPlan &p, hi
   a.tiles_m = (a.M + p.bm - 1) / p.bm, a.tiles_n = (a.N + p.bn - 1) / p.bn, a.splits = p.splits;
   const unsigned g = (unsigned)((int64_t)a.tiles_m * a.tiles_n * a.splits);
   if (p.bm == 128)
-    mx_mid_kernel<T, F8, 128, 128, F8 ? 3 : 2><<<g, 256, 0, stream>>>(a);
+    mx_mid_kernel<T, F8, 128, 128, 2><<<g, 256, 0, stream>>>(a);
   else if (p.bn == 128)
     mx_mid_kernel<T, F8, 64, 128, F8 ? 4 : 3><<<g, 256, 0, stream>>>(a);
   else
