@@ -289,7 +289,7 @@ __device__ __forceinline__ float sum_g(float v) {
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_decode_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(AttnArgs a) {
   constexpr int NF = D / 32;                // fragments of a row in the contraction over head_dim
   constexpr int NB = D / 16;                // 16-column blocks of the output
   constexpr int VP = 2 * D + 32;            // V row pitch in LDS
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(256) void attn_decode_kernel(AttnArgs a) {
     int e = (int)(__float_as_uint(m) >> 23) - 127;   // m >= 0
     e = m == 0.f || e == 128 ? 0 : e < -100 ? -100 : e;  // inf: left as it is
     const float up = pow2f(14 - e < 127 ? 14 - e : 127);
-    qscale = a.sm_log2 * global_scale_of(c.amax[0]) * (1.0f / up);
+    qscale = fmaxf(a.sm_log2 * global_scale_of(c.amax[0]) * (1.0f / up), 1e-37f);  // > 0: scores of -inf stay -inf
 #pragma unroll
     for (int f = 0; f < NF; ++f)
 #pragma unroll
@@ -508,6 +508,281 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   }
 }
 
+// ---- attention of prompts ------------------------------------------------------------------------
+// The same sums where every KV head has rows by the hundred: bound by the matrix cores and, nearly as
+// much, by the exponentials (16 of 64 lanes a cycle), so both have to run at once.  A workgroup is 4 waves
+// of 64 rows (two column blocks of v_mfma_f32_32x32x16_f16) on one KV head, one wave a SIMD with all its
+// registers; 64 keys at a time are turned into fp16 by the whole workgroup and put into one of three LDS
+// stages (each key's codes are unpacked once per 256 rows).  64 rows a wave halve the LDS reads per MFMA
+// against 32: at 32 they take as many cycles as the MFMAs.
+// The loop over 32-key tiles is pipelined in registers: the step of tile j multiplies K of tile j + 1
+// and V of tile j - 1 while the softmax of tile j runs, three chains without a dependency between them.
+// The running maximum moves (and O is rescaled) only where a tile exceeds it by 2^8: weights then reach
+// 2^(8 + kPromptShift), inside fp16.
+constexpr float kPromptShift = 6.0f, kPromptSlack = 8.0f;
+
+__device__ __forceinline__ float xmax32(float v) {  // v and its lane ^ 32 partner
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xadd32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f2v __attribute__((ext_vector_type(2)));
+
+// key (of a 32-key tile) of score register j in half hi
+__device__ __forceinline__ int crow(int j, int hi) { return (j & 3) + 8 * (j >> 2) + 4 * hi; }
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 1) void attn_prompt_kernel(AttnArgs a) {
+  constexpr int KP = 2 * D + 16, VP = 2 * D + 64;  // row pitches: conflict-free b128 reads / transposed reads
+  constexpr int KIMG = 64 * KP, VIMG = 64 * VP, STAGE = KIMG + VIMG;
+  constexpr int QS = D / 16, DB = D / 32, NW = D / 32;  // steps over head_dim, output blocks, code dwords a lane
+  __shared__ __attribute__((aligned(16))) unsigned char lds[3 * STAGE];
+  const Cache &c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 31, hi = lane >> 5;
+  // the tiles of one (sequence, KV head) on one XCD, longest first
+  const int xcd = blockIdx.x % 8, li = blockIdx.x / 8;
+  const int pair = (li / a.tiles) * 8 + xcd, tile = a.tiles - 1 - li % a.tiles;
+  if (pair >= a.batch * c.hkv) return;
+  const int b = pair / c.hkv, kvh = pair - b * c.hkv;
+  const int lq = c.len_q[b], off = c.len_k[b] - lq, cap = c.table_cols << c.shift;
+  const int lk = c.len_k[b] < cap ? c.len_k[b] : cap;
+  const int nrows = lq > 0 ? lq * a.group : 0;
+  if (256 * tile >= nrows) return;  // the whole workgroup
+  const int last_tok = (256 * tile + 255 < nrows ? 256 * tile + 255 : nrows - 1) / a.group;
+  int kv_end = a.causal ? off + last_tok + 1 : lk;
+  kv_end = kv_end < lk ? kv_end : lk;
+  const int stages = kv_end > 0 ? (kv_end + 63) / 64 : 0;
+
+  // ---- this lane's two rows of q
+  h8 qf[2][QS];
+  float qs[2];
+  int see[2], wmin = 0x7fffffff;  // keys a row sees; keys below wmin need no mask in any of the wave's rows
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = 256 * tile + 64 * wave + 32 * r + fr, rtok = row / a.group, head = kvh * a.group + row % a.group;
+    const int64_t qrow = (int64_t)c.start[b] + rtok;
+    const bool ok = row < nrows && qrow >= 0 && qrow < a.rows;
+    see[r] = ok ? (a.causal ? (off + rtok + 1 < lk ? off + rtok + 1 : lk) : lk) : 0;
+    wmin = ok && see[r] < wmin ? see[r] : wmin;
+    const T *qp = reinterpret_cast<const T *>(a.q) + (ok ? qrow : 0) * a.qt + head * a.qh + 8 * hi;
+    Vec<T> x[QS];
+    float m = 0.f;
+#pragma unroll
+    for (int s = 0; s < QS; ++s) {
+      x[s].raw = make_uint4(0, 0, 0, 0);
+      if (ok) x[s] = ldg_vec(qp + 16 * s);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max_skip_nan(m, Elem<T>::ld(x[s].e[j]));
+    }
+    m = xmax32(m);
+    int e = (int)(__float_as_uint(m) >> 23) - 127;
+    e = m == 0.f || e == 128 ? 0 : e < -100 ? -100 : e;
+    const float up = pow2f(14 - e < 127 ? 14 - e : 127);
+    qs[r] = fmaxf(a.sm_log2 * global_scale_of(c.amax[0]) * (1.0f / up), 1e-37f);
+#pragma unroll
+    for (int s = 0; s < QS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) qf[r][s][j] = (_Float16)(Elem<T>::ld(x[s].e[j]) * up);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const int v = __shfl_xor(wmin, o, 64);
+    wmin = v < wmin ? v : wmin;
+  }
+  wmin = __builtin_amdgcn_readfirstlane(wmin);
+
+  f32x16 acc[2][DB];
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[r][d][e] = 0.f;
+  float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
+
+  // ---- staging: lane -> key tid / 4 of the stage, quarter tid % 4 of its columns
+  const int skey = tid >> 2, sg = tid & 3;
+  uint32_t kw[NW], vw[NW], ksc = 0, vsc = 0;
+  bool vok = false;
+  int pages = 0;  // of the stage in the registers: bit u: keys 16 u .. 16 u + 15 have a page
+  auto gload = [&](int t) {
+    const int key = 64 * t + skey;
+    pages = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) pages |= (page_of(c, b, 64 * t + 16 * u) >= 0 ? 1 : 0) << u;
+    pages = __builtin_amdgcn_readfirstlane(pages);
+    const int page = page_of(c, b, key);  // the 16 keys of a group: one page
+    const int64_t pg = page >= 0 ? page : 0;
+    const int at = key & ((1 << c.shift) - 1);
+    load_codes<D>(c.data[0] + kvh * c.d_head[0] + sg * (D / 8) + pg * c.d_page[0] + at * c.d_tok[0],
+                  c.scale[0] + kvh * c.s_head[0] + sg * (D / 64) + pg * c.s_page[0] + at * c.s_tok[0], kw, ksc);
+    load_codes<D>(c.data[1] + kvh * c.d_head[1] + sg * (D / 8) + pg * c.d_page[1] + at * c.d_tok[1],
+                  c.scale[1] + kvh * c.s_head[1] + sg * (D / 64) + pg * c.s_page[1] + at * c.s_tok[1], vw, vsc);
+    vok = page >= 0 && key < lk;
+  };
+  auto swrite = [&](int slot) {
+    h8 f[NW];
+    unsigned char *kb = lds + slot * STAGE + skey * KP + sg * (D / 2), *vb = lds + slot * STAGE + KIMG + skey * VP + sg * (D / 2);
+    dequant<D>(kw, ksc, true, f);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) *reinterpret_cast<h8 *>(kb + 16 * i) = f[i];
+    dequant<D>(vw, vsc, vok, f);  // keys of no token of this sequence: zeros (0 * NaN is NaN)
+#pragma unroll
+    for (int i = 0; i < NW; ++i) *reinterpret_cast<h8 *>(vb + 16 * i) = f[i];
+  };
+  // S^T of a tile for both column blocks
+  auto score = [&](const unsigned char *K, f32x16 (&s)[2]) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[r][e] = 0.f;
+#pragma unroll
+    for (int st = 0; st < QS; ++st) {
+      const h8 kf = *reinterpret_cast<const h8 *>(K + fr * KP + (16 * st + 8 * hi) * 2);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) s[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[r][st], s[r], 0, 0, 0);
+    }
+  };
+  const int trq = (lane & 15) >> 2, trp = lane & 3, trg = lane >> 4;
+  const int tr_off = (4 * (trg >> 1) + trq) * VP + (16 * (trg & 1) + 4 * trp) * 2;
+  auto pv = [&](const unsigned char *V, const h8 (&p)[2][2]) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const unsigned char *base = V + tr_off + 16 * g * VP + 64 * d;
+        const h4 lo = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)base));
+        const h4 up = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(base + 8 * VP)));
+        const h8 vf = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
+#pragma unroll
+        for (int r = 0; r < 2; ++r) acc[r][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[r][g], acc[r][d], 0, 0, 0);
+      }
+  };
+  // the softmax of one tile; returns whether some row's maximum moved (corr: what O and l of before are worth)
+  auto soft = [&](const f32x16 (&s)[2], h8 (&p)[2][2], float (&corr)[2]) -> bool {
+    bool moved = false;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float mx = s[r][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[r][e]);
+      mx = xmax32(mx) * qs[r];
+      const bool up = mx > m[r] + kPromptSlack;
+      corr[r] = up ? __builtin_amdgcn_exp2f(m[r] - mx) : 1.f;  // m = -inf: 0
+      moved |= up;
+      m[r] = up ? mx : m[r];
+      const float mu = (m[r] == kNegInf ? 0.f : m[r]) - kPromptShift;
+      float ls = 0.f;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][8 * g + i], qs[r], -mu));
+          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][8 * g + i + 1], qs[r], -mu));
+          ls += e0;
+          ls += e1;
+          const h2 h = __builtin_convertvector((f2v{e0, e1}), h2);
+          p[r][g][i] = h.x;
+          p[r][g][i + 1] = h.y;
+        }
+      l[r] = l[r] * corr[r] + ls;  // this lane's keys only; joined at the end
+    }
+    return moved;
+  };
+  auto mask = [&](f32x16 (&s)[2], int kv0, int pg) {
+    if (kv0 + 32 <= wmin && pg == 3) return;  // wave-uniform
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int k = crow(e, hi);
+        s[r][e] = kv0 + k < see[r] && (pg >> (k >> 4) & 1) ? s[r][e] : kNegInf;
+      }
+  };
+
+  if (stages > 0) {
+    // V of "tile -1" is multiplied by weights of zero: it has to be finite
+    for (int i = tid; i < VIMG / 16; i += 256) *reinterpret_cast<uint4 *>(lds + 2 * STAGE + KIMG + 16 * i) = make_uint4(0, 0, 0, 0);
+    gload(0);
+    int pg0 = pages;
+    swrite(0);
+    gload(1 < stages ? 1 : 0);
+    int pg1 = pages;
+    __syncthreads();
+    f32x16 sc[2], sn[2];
+    score(lds, sc);
+    h8 pp[2][2], pc[2][2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pp[r][g][i] = (_Float16)0.f;
+    int slot = 0;
+    float corr[2];
+    auto rescale = [&](bool moved) {
+      if (__builtin_amdgcn_ballot_w64(moved)) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[r][d][e] *= corr[r];
+      }
+    };
+    for (int t = 0; t < stages; ++t) {
+      const int nx = slot == 2 ? 0 : slot + 1, pv_slot = slot == 0 ? 2 : slot - 1;
+      const unsigned char *Kc = lds + slot * STAGE, *Vc = Kc + KIMG, *Vp = lds + pv_slot * STAGE + KIMG + 32 * VP;
+      // tile 2 t: scores of 2 t + 1, V of 2 t - 1
+      mask(sc, 64 * t, pg0 & 3);
+      swrite(nx);                                   // stage t + 1 (read by none before the barrier below)
+      gload(t + 2 < stages ? t + 2 : stages - 1);   // in flight under the rest of this stage
+      const int pg2 = pages;
+      score(Kc + 32 * KP, sn);
+      bool moved = soft(sc, pc, corr);
+      pv(Vp, pp);
+      rescale(moved);
+      __syncthreads();
+      // tile 2 t + 1: scores of 2 t + 2, V of 2 t
+      mask(sn, 64 * t + 32, pg0 >> 2);
+      score(lds + nx * STAGE, sc);
+      moved = soft(sn, pp, corr);
+      pv(Vc, pc);
+      rescale(moved);
+      slot = nx;
+      pg0 = pg1, pg1 = pg2;
+    }
+    pv(lds + (slot == 0 ? 2 : slot - 1) * STAGE + KIMG + 32 * VP, pp);
+  }
+
+  // ---- o = acc gv / l: lane holds columns 32 d + crow(e, hi) of its rows
+  const float gv = global_scale_of(c.amax[1]);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const float ls = xadd32(l[r]);
+    const int row = 256 * tile + 64 * wave + 32 * r + fr;
+    const int64_t orow = (int64_t)c.start[b] + row / a.group;
+    if (row >= nrows || orow < 0 || orow >= a.rows) continue;
+    const float inv = gv / ls;
+    T *op = reinterpret_cast<T *>(a.o) + orow * a.ot + (kvh * a.group + row % a.group) * a.oh;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        struct alignas(4 * sizeof(T)) Pack {
+          T h[4];
+        } pk;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pk.h[i] = Elem<T>::st(ls == 0.f ? 0.f : acc[r][d][4 * e4 + i] * inv);
+        *reinterpret_cast<Pack *>(op + 32 * d + 8 * e4 + 4 * hi) = pk;
+      }
+  }
+}
+
 bool make_cache(const mtq_kv_cache *k, const int32_t *table, int64_t table_stride, int table_cols, const int32_t *start,
                 const int32_t *len_q, const int32_t *len_k, int batch, Cache &c) {
   if (!k || !table || !start || !len_q || !len_k || batch < 1 || table_cols < 1 || (batch > 1 && table_stride < table_cols)) return false;
@@ -568,9 +843,18 @@ int rows_call(bool append, const mtq_kv_cache *cache, void *k, void *v, const in
 // keys of a split: enough workgroups to fill the card, at least 128 keys (one 32-key step a wave)
 struct Plan {
   int tiles, chunk, splits;
+  bool prompt;
 };
-Plan attn_plan(int batch, int hkv, int group, int max_len_q, int max_len_k) {
+// rows of a KV head from which the prompt kernel is taken
+constexpr int kPromptRows = 128;
+Plan attn_plan(int batch, int hkv, int group, int head_dim, int max_len_q, int max_len_k) {
   Plan p;
+  const int64_t rows = (int64_t)max_len_q * group;
+  p.prompt = rows >= kPromptRows && head_dim <= 128;  // head_dim 256: its three stages do not fit LDS
+  if (p.prompt) {
+    p.tiles = (int)((rows + 255) / 256), p.splits = 1, p.chunk = max_len_k;
+    return p;
+  }
   p.tiles = (int)(((int64_t)max_len_q * group + 15) / 16);
   const int64_t wgs = (int64_t)batch * hkv * p.tiles, want = 8 * 256;
   int64_t splits = (want + wgs - 1) / wgs;
@@ -605,7 +889,7 @@ int mtq_kv_read(const mtq_kv_cache *cache, void *k, void *v, const int64_t *stri
 
 size_t mtq_kv_attention_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim, int max_len_q, int max_len_k) {
   if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_len_q < 1 || head_dim < 1) return 0;
-  const Plan p = attn_plan(batch, num_kv_heads, num_q_heads / num_kv_heads, max_len_q, max_len_k);
+  const Plan p = attn_plan(batch, num_kv_heads, num_q_heads / num_kv_heads, head_dim, max_len_q, max_len_k);
   return p.splits > 1 ? (size_t)p.splits * batch * num_kv_heads * p.tiles * 16 * (head_dim + 4) * sizeof(float) : 0;
 }
 
@@ -622,13 +906,14 @@ int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const in
   if (num_q_heads < 1 || num_q_heads % a.c.hkv) return MTQ_ERR_INVALID_ARG;
   for (int i = 0; i < 4; ++i)
     if (strides[i] < 0 || strides[i] % 8) return MTQ_ERR_INVALID_ARG;
-  if (!al16p(q) || !al16p(o) || !(softmax_scale == softmax_scale)) return MTQ_ERR_INVALID_ARG;
+  if (!al16p(q) || !al16p(o) || !(softmax_scale > 0.0 && softmax_scale < 3.4e38)) return MTQ_ERR_INVALID_ARG;
   const int64_t cap = (int64_t)table_cols * cache->page_size;
   if (max_len_k > cap) max_len_k = (int)cap;
   a.group = num_q_heads / a.c.hkv;
   if ((int64_t)max_len_q * a.group > INT32_MAX - 16) return MTQ_ERR_INVALID_ARG;
-  const Plan p = attn_plan(batch, a.c.hkv, a.group, max_len_q, max_len_k);
-  if ((int64_t)p.tiles * a.c.hkv > 65535) return MTQ_ERR_INVALID_ARG;
+  const Plan p = attn_plan(batch, a.c.hkv, a.group, a.c.head_dim, max_len_q, max_len_k);
+  const int64_t pg = ((int64_t)batch * a.c.hkv + 7) / 8 * 8 * p.tiles;  // the prompt kernel's grid
+  if (p.prompt ? pg > INT32_MAX : (int64_t)p.tiles * a.c.hkv > 65535) return MTQ_ERR_INVALID_ARG;
   const size_t need = mtq_kv_attention_workspace_bytes(batch, num_q_heads, a.c.hkv, a.c.head_dim, max_len_q, max_len_k);
   if (need && (!ws || ws_bytes < need || !al16p(ws))) return MTQ_ERR_INVALID_ARG;
   a.q = q, a.o = o, a.part = (float *)ws;
@@ -640,6 +925,12 @@ int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const in
   auto go = [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
+    if constexpr (D <= 128) {
+      if (p.prompt) {
+        attn_prompt_kernel<T, D><<<(unsigned)pg, 256, 0, stream>>>(a);
+        return host_check_launch();
+      }
+    }
     attn_decode_kernel<T, D><<<g, 256, 0, stream>>>(a);
     const int st = host_check_launch();
     if (st != MTQ_OK || p.splits == 1) return st;
