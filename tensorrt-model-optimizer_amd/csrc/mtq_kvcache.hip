@@ -233,11 +233,16 @@ struct AttnArgs {
   Cache c;
   const void *q;
   void *o;
-  float *part;  // [splits][batch][hkv][tiles][16][D + 2] (o, m, l) of each split
+  float *part;  // the splits' rows: o, m, l
   int64_t qt, qh, ot, oh, rows;
-  int group, causal, splits, chunk, tiles, batch;
+  int group, causal, splits, chunk, tiles, part_tiles, batch;  // tiles: of the kernel's rows, part_tiles: of 16
   float sm_log2;  // softmax_scale * log2(e)
 };
+
+// where a row of a split's results lies: [splits][batch][hkv][16-row tiles][16][D + 4]
+template <int D> __device__ __forceinline__ int64_t part_row(const AttnArgs &a, int split, int b, int kvh, int row) {
+  return (((((int64_t)split * a.batch + b) * a.c.hkv + kvh) * a.part_tiles + (row >> 4)) * 16 + (row & 15)) * (D + 4);
+}
 
 // fp16 values of a lane's D / 4 codes times their block scales; ok false: zeros
 template <int D>
@@ -454,7 +459,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
       o += *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(lds) + (w * 16 + r) * (D + 4) + d4) * f;
     }
     if (a.splits > 1) {
-      float *pp = a.part + ((((int64_t)split * a.batch + b) * c.hkv + kvh) * a.tiles + tile) * 16 * (D + 4) + r * (D + 4);
+      float *pp = a.part + part_row<D>(a, split, b, kvh, rr);
       *reinterpret_cast<f32x4 *>(pp + d4) = o;
       if (d4 == 0) pp[D] = mm, pp[D + 1] = ls;
     } else {
@@ -472,7 +477,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const Cache &c = a.c;
-  const int kvh = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles, b = blockIdx.z;
+  const int kvh = blockIdx.y / a.part_tiles, tile = blockIdx.y % a.part_tiles, b = blockIdx.z;
   const int lq = c.len_q[b];
   int lk = c.len_k[b];
   const int cap = c.table_cols << c.shift, off = lk - lq;
@@ -485,12 +490,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   int n = kv_end > 0 ? (kv_end + a.chunk - 1) / a.chunk : 1;
   n = n < a.splits ? n : a.splits;
   const float gv = global_scale_of(c.amax[1]);
-  const int64_t step = (int64_t)a.batch * c.hkv * a.tiles * 16 * (D + 4);
+  const int64_t step = (int64_t)a.batch * c.hkv * a.part_tiles * 16 * (D + 4);
   for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
     const int r = i / (D / 4), d4 = 4 * (i % (D / 4)), rr = 16 * tile + r;
     const int64_t orow = (int64_t)c.start[b] + rr / a.group;
     if (rr >= nrows || orow < 0 || orow >= a.rows) continue;
-    const float *pp = a.part + (((int64_t)b * c.hkv + kvh) * a.tiles + tile) * 16 * (D + 4) + r * (D + 4);
+    const float *pp = a.part + part_row<D>(a, 0, b, kvh, rr);
     float mm = kNegInf;
     for (int s = 0; s < n; ++s) mm = fmaxf(mm, pp[s * step + D]);
     const float mu = mm == kNegInf ? 0.f : mm;
@@ -510,11 +515,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 // ---- attention of prompts ------------------------------------------------------------------------
 // The same sums where every KV head has rows by the hundred: bound by the matrix cores and, nearly as
-// much, by the exponentials (16 of 64 lanes a cycle), so both have to run at once.  A workgroup is 4 waves
-// of 64 rows (two column blocks of v_mfma_f32_32x32x16_f16) on one KV head, one wave a SIMD with all its
-// registers; 64 keys at a time are turned into fp16 by the whole workgroup and put into one of three LDS
-// stages (each key's codes are unpacked once per 256 rows).  64 rows a wave halve the LDS reads per MFMA
-// against 32: at 32 they take as many cycles as the MFMAs.
+// much, by the exponentials (a quarter of the VALU's rate) and by LDS (K and V of a 32 x 32 tile of scores
+// are 16 KiB of fragments: 128 cycles of LDS beside 512 of one SIMD's matrix core, four SIMDs at once).  A
+// workgroup is 8 waves of 32 rows (v_mfma_f32_32x32x16_f16) on one KV head, two waves a SIMD; 64 keys at
+// a time are turned into fp16 by the whole workgroup, once per 256 rows, into one of three LDS stages.
+// (64 rows a wave, one wave a SIMD, half the LDS reads: 546 us against 409 for chunks of 500 to 1024
+// tokens behind contexts of up to 8192, 4 sequences, 32 / 8 heads: nothing of its one wave overlaps.)
 // The loop over 32-key tiles is pipelined in registers: the step of tile j multiplies K of tile j + 1
 // and V of tile j - 1 while the softmax of tile j runs, three chains without a dependency between them.
 // The running maximum moves (and O is rescaled) only where a tile exceeds it by 2^8: weights then reach
@@ -536,7 +542,7 @@ typedef float f2v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ int crow(int j, int hi) { return (j & 3) + 8 * (j >> 2) + 4 * hi; }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, 1) void attn_prompt_kernel(AttnArgs a) {
+__global__ __launch_bounds__(512, 2) void attn_prompt_kernel(AttnArgs a) {
   constexpr int KP = 2 * D + 16, VP = 2 * D + 64;  // row pitches: conflict-free b128 reads / transposed reads
   constexpr int KIMG = 64 * KP, VIMG = 64 * VP, STAGE = KIMG + VIMG;
   constexpr int QS = D / 16, DB = D / 32, NW = D / 32;  // steps over head_dim, output blocks, code dwords a lane
@@ -555,19 +561,22 @@ __global__ __launch_bounds__(256, 1) void attn_prompt_kernel(AttnArgs a) {
   const int last_tok = (256 * tile + 255 < nrows ? 256 * tile + 255 : nrows - 1) / a.group;
   int kv_end = a.causal ? off + last_tok + 1 : lk;
   kv_end = kv_end < lk ? kv_end : lk;
-  const int stages = kv_end > 0 ? (kv_end + 63) / 64 : 0;
+  // this split's stages of 64 keys (the last split takes what is left); the join knows the splits there are
+  const int split = blockIdx.y, t0 = split * (a.chunk / 64);
+  if (split > 0 && 64 * t0 >= kv_end) return;
+  int stages = kv_end > 0 ? (kv_end + 63) / 64 : 0;
+  if (split + 1 < a.splits && t0 + a.chunk / 64 < stages) stages = t0 + a.chunk / 64;
 
-  // ---- this lane's two rows of q
-  h8 qf[2][QS];
-  float qs[2];
-  int see[2], wmin = 0x7fffffff;  // keys a row sees; keys below wmin need no mask in any of the wave's rows
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = 256 * tile + 64 * wave + 32 * r + fr, rtok = row / a.group, head = kvh * a.group + row % a.group;
+  // ---- this lane's row of q
+  h8 qf[QS];
+  float qs;
+  int see, wmin = 0x7fffffff;  // keys a row sees; keys below wmin need no mask in any of the wave's rows
+  {
+    const int row = 256 * tile + 32 * wave + fr, rtok = row / a.group, head = kvh * a.group + row % a.group;
     const int64_t qrow = (int64_t)c.start[b] + rtok;
     const bool ok = row < nrows && qrow >= 0 && qrow < a.rows;
-    see[r] = ok ? (a.causal ? (off + rtok + 1 < lk ? off + rtok + 1 : lk) : lk) : 0;
-    wmin = ok && see[r] < wmin ? see[r] : wmin;
+    see = ok ? (a.causal ? (off + rtok + 1 < lk ? off + rtok + 1 : lk) : lk) : 0;
+    wmin = ok && see < wmin ? see : wmin;
     const T *qp = reinterpret_cast<const T *>(a.q) + (ok ? qrow : 0) * a.qt + head * a.qh + 8 * hi;
     Vec<T> x[QS];
     float m = 0.f;
@@ -582,11 +591,11 @@ __global__ __launch_bounds__(256, 1) void attn_prompt_kernel(AttnArgs a) {
     int e = (int)(__float_as_uint(m) >> 23) - 127;
     e = m == 0.f || e == 128 ? 0 : e < -100 ? -100 : e;
     const float up = pow2f(14 - e < 127 ? 14 - e : 127);
-    qs[r] = fmaxf(a.sm_log2 * global_scale_of(c.amax[0]) * (1.0f / up), 1e-37f);
+    qs = fmaxf(a.sm_log2 * global_scale_of(c.amax[0]) * (1.0f / up), 1e-37f);
 #pragma unroll
     for (int s = 0; s < QS; ++s)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) qf[r][s][j] = (_Float16)(Elem<T>::ld(x[s].e[j]) * up);
+      for (int j = 0; j < 8; ++j) qf[s][j] = (_Float16)(Elem<T>::ld(x[s].e[j]) * up);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -595,61 +604,52 @@ __global__ __launch_bounds__(256, 1) void attn_prompt_kernel(AttnArgs a) {
   }
   wmin = __builtin_amdgcn_readfirstlane(wmin);
 
-  f32x16 acc[2][DB];
+  f32x16 acc[DB];
 #pragma unroll
-  for (int r = 0; r < 2; ++r)
+  for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[r][d][e] = 0.f;
-  float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
+    for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+  float m = kNegInf, l = 0.f;
 
-  // ---- staging: lane -> key tid / 4 of the stage, quarter tid % 4 of its columns
-  const int skey = tid >> 2, sg = tid & 3;
-  uint32_t kw[NW], vw[NW], ksc = 0, vsc = 0;
-  bool vok = false;
+  // ---- staging: the first 256 lanes unpack K, the others V; lane -> key of the stage, quarter of its columns
+  const int skey = (tid & 255) >> 2, sg = tid & 3, skv = wave >> 2;
+  uint32_t cw[NW], csc = 0;
+  bool cok = false;
   int pages = 0;  // of the stage in the registers: bit u: keys 16 u .. 16 u + 15 have a page
+  const int64_t d_page = skv ? c.d_page[1] : c.d_page[0], d_tok = skv ? c.d_tok[1] : c.d_tok[0];
+  const int64_t s_page = skv ? c.s_page[1] : c.s_page[0], s_tok = skv ? c.s_tok[1] : c.s_tok[0];
+  const uint8_t *const dbase = (skv ? c.data[1] + kvh * c.d_head[1] : c.data[0] + kvh * c.d_head[0]) + sg * (D / 8);
+  const uint8_t *const sbase = (skv ? c.scale[1] + kvh * c.s_head[1] : c.scale[0] + kvh * c.s_head[0]) + sg * (D / 64);
   auto gload = [&](int t) {
-    const int key = 64 * t + skey;
     pages = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) pages |= (page_of(c, b, 64 * t + 16 * u) >= 0 ? 1 : 0) << u;
     pages = __builtin_amdgcn_readfirstlane(pages);
-    const int page = page_of(c, b, key);  // the 16 keys of a group: one page
+    const int key = 64 * t + skey, page = page_of(c, b, key), at = key & ((1 << c.shift) - 1);
     const int64_t pg = page >= 0 ? page : 0;
-    const int at = key & ((1 << c.shift) - 1);
-    load_codes<D>(c.data[0] + kvh * c.d_head[0] + sg * (D / 8) + pg * c.d_page[0] + at * c.d_tok[0],
-                  c.scale[0] + kvh * c.s_head[0] + sg * (D / 64) + pg * c.s_page[0] + at * c.s_tok[0], kw, ksc);
-    load_codes<D>(c.data[1] + kvh * c.d_head[1] + sg * (D / 8) + pg * c.d_page[1] + at * c.d_tok[1],
-                  c.scale[1] + kvh * c.s_head[1] + sg * (D / 64) + pg * c.s_page[1] + at * c.s_tok[1], vw, vsc);
-    vok = page >= 0 && key < lk;
+    load_codes<D>(dbase + pg * d_page + at * d_tok, sbase + pg * s_page + at * s_tok, cw, csc);
+    cok = skv == 0 || (page >= 0 && key < lk);  // V of no token of this sequence: zeros (0 * NaN is NaN)
   };
   auto swrite = [&](int slot) {
     h8 f[NW];
-    unsigned char *kb = lds + slot * STAGE + skey * KP + sg * (D / 2), *vb = lds + slot * STAGE + KIMG + skey * VP + sg * (D / 2);
-    dequant<D>(kw, ksc, true, f);
+    dequant<D>(cw, csc, cok, f);
+    unsigned char *o = lds + slot * STAGE + (skv ? KIMG + skey * VP : skey * KP) + sg * (D / 2);
 #pragma unroll
-    for (int i = 0; i < NW; ++i) *reinterpret_cast<h8 *>(kb + 16 * i) = f[i];
-    dequant<D>(vw, vsc, vok, f);  // keys of no token of this sequence: zeros (0 * NaN is NaN)
-#pragma unroll
-    for (int i = 0; i < NW; ++i) *reinterpret_cast<h8 *>(vb + 16 * i) = f[i];
+    for (int i = 0; i < NW; ++i) *reinterpret_cast<h8 *>(o + 16 * i) = f[i];
   };
-  // S^T of a tile for both column blocks
-  auto score = [&](const unsigned char *K, f32x16 (&s)[2]) {
+  // S^T of a tile
+  auto score = [&](const unsigned char *K, f32x16 &s) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[r][e] = 0.f;
+    for (int e = 0; e < 16; ++e) s[e] = 0.f;
 #pragma unroll
     for (int st = 0; st < QS; ++st) {
       const h8 kf = *reinterpret_cast<const h8 *>(K + fr * KP + (16 * st + 8 * hi) * 2);
-#pragma unroll
-      for (int r = 0; r < 2; ++r) s[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[r][st], s[r], 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[st], s, 0, 0, 0);
     }
   };
   const int trq = (lane & 15) >> 2, trp = lane & 3, trg = lane >> 4;
   const int tr_off = (4 * (trg >> 1) + trq) * VP + (16 * (trg & 1) + 4 * trp) * 2;
-  auto pv = [&](const unsigned char *V, const h8 (&p)[2][2]) {
+  auto pv = [&](const unsigned char *V, const h8 (&p)[2]) {
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -658,83 +658,71 @@ __global__ __launch_bounds__(256, 1) void attn_prompt_kernel(AttnArgs a) {
         const h4 lo = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)base));
         const h4 up = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(base + 8 * VP)));
         const h8 vf = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
-#pragma unroll
-        for (int r = 0; r < 2; ++r) acc[r][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[r][g], acc[r][d], 0, 0, 0);
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[g], acc[d], 0, 0, 0);
       }
   };
   // the softmax of one tile; returns whether some row's maximum moved (corr: what O and l of before are worth)
-  auto soft = [&](const f32x16 (&s)[2], h8 (&p)[2][2], float (&corr)[2]) -> bool {
-    bool moved = false;
+  auto soft = [&](const f32x16 &s, h8 (&p)[2], float &corr) -> bool {
+    float mx = s[0];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float mx = s[r][0];
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+    mx = xmax32(mx) * qs;
+    const bool up = mx > m + kPromptSlack;
+    corr = up ? __builtin_amdgcn_exp2f(m - mx) : 1.f;  // m = -inf: 0
+    m = up ? mx : m;
+    const float mu = (m == kNegInf ? 0.f : m) - kPromptShift;
+    float ls = 0.f;
 #pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[r][e]);
-      mx = xmax32(mx) * qs[r];
-      const bool up = mx > m[r] + kPromptSlack;
-      corr[r] = up ? __builtin_amdgcn_exp2f(m[r] - mx) : 1.f;  // m = -inf: 0
-      moved |= up;
-      m[r] = up ? mx : m[r];
-      const float mu = (m[r] == kNegInf ? 0.f : m[r]) - kPromptShift;
-      float ls = 0.f;
+    for (int g = 0; g < 2; ++g)
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][8 * g + i], qs[r], -mu));
-          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][8 * g + i + 1], qs[r], -mu));
-          ls += e0;
-          ls += e1;
-          const h2 h = __builtin_convertvector((f2v{e0, e1}), h2);
-          p[r][g][i] = h.x;
-          p[r][g][i + 1] = h.y;
-        }
-      l[r] = l[r] * corr[r] + ls;  // this lane's keys only; joined at the end
-    }
-    return moved;
+      for (int i = 0; i < 8; i += 2) {
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * g + i], qs, -mu));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * g + i + 1], qs, -mu));
+        ls += e0;
+        ls += e1;
+        const h2 h = __builtin_convertvector((f2v{e0, e1}), h2);
+        p[g][i] = h.x;
+        p[g][i + 1] = h.y;
+      }
+    l = l * corr + ls;  // this lane's keys only; joined at the end
+    return up;
   };
-  auto mask = [&](f32x16 (&s)[2], int kv0, int pg) {
+  auto mask = [&](f32x16 &s, int kv0, int pg) {
     if (kv0 + 32 <= wmin && pg == 3) return;  // wave-uniform
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int k = crow(e, hi);
-        s[r][e] = kv0 + k < see[r] && (pg >> (k >> 4) & 1) ? s[r][e] : kNegInf;
-      }
+    for (int e = 0; e < 16; ++e) {
+      const int k = crow(e, hi);
+      s[e] = kv0 + k < see && (pg >> (k >> 4) & 1) ? s[e] : kNegInf;
+    }
   };
 
-  if (stages > 0) {
+  if (t0 < stages) {
     // V of "tile -1" is multiplied by weights of zero: it has to be finite
-    for (int i = tid; i < VIMG / 16; i += 256) *reinterpret_cast<uint4 *>(lds + 2 * STAGE + KIMG + 16 * i) = make_uint4(0, 0, 0, 0);
-    gload(0);
+    for (int i = tid; i < VIMG / 16; i += 512) *reinterpret_cast<uint4 *>(lds + 2 * STAGE + KIMG + 16 * i) = make_uint4(0, 0, 0, 0);
+    gload(t0);
     int pg0 = pages;
     swrite(0);
-    gload(1 < stages ? 1 : 0);
+    gload(t0 + 1 < stages ? t0 + 1 : t0);
     int pg1 = pages;
     __syncthreads();
-    f32x16 sc[2], sn[2];
+    f32x16 sc, sn;
     score(lds, sc);
-    h8 pp[2][2], pc[2][2];
+    h8 pp[2], pc[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int g = 0; g < 2; ++g)
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pp[r][g][i] = (_Float16)0.f;
+      for (int i = 0; i < 8; ++i) pp[g][i] = (_Float16)0.f;
     int slot = 0;
-    float corr[2];
+    float corr;
     auto rescale = [&](bool moved) {
       if (__builtin_amdgcn_ballot_w64(moved)) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-          for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[r][d][e] *= corr[r];
+          for (int e = 0; e < 16; ++e) acc[d][e] *= corr;
       }
     };
-    for (int t = 0; t < stages; ++t) {
+    for (int t = t0; t < stages; ++t) {
       const int nx = slot == 2 ? 0 : slot + 1, pv_slot = slot == 0 ? 2 : slot - 1;
       const unsigned char *Kc = lds + slot * STAGE, *Vc = Kc + KIMG, *Vp = lds + pv_slot * STAGE + KIMG + 32 * VP;
       // tile 2 t: scores of 2 t + 1, V of 2 t - 1
@@ -759,28 +747,35 @@ __global__ __launch_bounds__(256, 1) void attn_prompt_kernel(AttnArgs a) {
     pv(lds + (slot == 0 ? 2 : slot - 1) * STAGE + KIMG + 32 * VP, pp);
   }
 
-  // ---- o = acc gv / l: lane holds columns 32 d + crow(e, hi) of its rows
-  const float gv = global_scale_of(c.amax[1]);
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const float ls = xadd32(l[r]);
-    const int row = 256 * tile + 64 * wave + 32 * r + fr;
-    const int64_t orow = (int64_t)c.start[b] + row / a.group;
-    if (row >= nrows || orow < 0 || orow >= a.rows) continue;
-    const float inv = gv / ls;
-    T *op = reinterpret_cast<T *>(a.o) + orow * a.ot + (kvh * a.group + row % a.group) * a.oh;
+  // ---- o = acc gv / l: lane holds columns 32 d + crow(e, hi) of its row
+  const float ls = xadd32(l);
+  const int row = 256 * tile + 32 * wave + fr;
+  if (row >= nrows) return;
+  if (a.splits > 1) {
+    float *pp = a.part + part_row<D>(a, split, b, kvh, row);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
-        struct alignas(4 * sizeof(T)) Pack {
-          T h[4];
-        } pk;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pk.h[i] = Elem<T>::st(ls == 0.f ? 0.f : acc[r][d][4 * e4 + i] * inv);
-        *reinterpret_cast<Pack *>(op + 32 * d + 8 * e4 + 4 * hi) = pk;
-      }
+      for (int e4 = 0; e4 < 4; ++e4)
+        *reinterpret_cast<f32x4 *>(pp + 32 * d + 8 * e4 + 4 * hi) = f32x4{acc[d][4 * e4], acc[d][4 * e4 + 1], acc[d][4 * e4 + 2], acc[d][4 * e4 + 3]};
+    if (hi == 0) pp[D] = m, pp[D + 1] = ls;
+    return;
   }
+  const int64_t orow = (int64_t)c.start[b] + row / a.group;
+  if (orow < 0 || orow >= a.rows) return;
+  const float inv = global_scale_of(c.amax[1]) / ls;
+  T *op = reinterpret_cast<T *>(a.o) + orow * a.ot + (kvh * a.group + row % a.group) * a.oh;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      struct alignas(4 * sizeof(T)) Pack {
+        T h[4];
+      } pk;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pk.h[i] = Elem<T>::st(ls == 0.f ? 0.f : acc[d][4 * e4 + i] * inv);
+      *reinterpret_cast<Pack *>(op + 32 * d + 8 * e4 + 4 * hi) = pk;
+    }
 }
 
 bool make_cache(const mtq_kv_cache *k, const int32_t *table, int64_t table_stride, int table_cols, const int32_t *start,
@@ -842,28 +837,29 @@ int rows_call(bool append, const mtq_kv_cache *cache, void *k, void *v, const in
 
 // keys of a split: enough workgroups to fill the card, at least 128 keys (one 32-key step a wave)
 struct Plan {
-  int tiles, chunk, splits;
+  int tiles, part_tiles, chunk, splits;
   bool prompt;
 };
 // rows of a KV head from which the prompt kernel is taken
 constexpr int kPromptRows = 128;
+
+// Splits of the keys: enough workgroups to fill the card (decode: 8 a CU, a split at least 128 keys, one
+// 32-key step a wave; prompts: one a CU, at least 512 keys)
 Plan attn_plan(int batch, int hkv, int group, int head_dim, int max_len_q, int max_len_k) {
   Plan p;
   const int64_t rows = (int64_t)max_len_q * group;
   p.prompt = rows >= kPromptRows && head_dim <= 128;  // head_dim 256: its three stages do not fit LDS
-  if (p.prompt) {
-    p.tiles = (int)((rows + 255) / 256), p.splits = 1, p.chunk = max_len_k;
-    return p;
-  }
-  p.tiles = (int)(((int64_t)max_len_q * group + 15) / 16);
-  const int64_t wgs = (int64_t)batch * hkv * p.tiles, want = 8 * 256;
-  int64_t splits = (want + wgs - 1) / wgs;
-  const int64_t most = (max_len_k + 127) / 128;
+  p.part_tiles = (int)((rows + 15) / 16);
+  p.tiles = p.prompt ? (int)((rows + 255) / 256) : p.part_tiles;
+  const int64_t wgs = (int64_t)batch * hkv * p.tiles, cus = host_num_cus();
+  const int least = p.prompt ? 512 : 128;
+  int64_t splits = p.prompt ? cus / wgs : (8 * cus + wgs - 1) / wgs;
+  const int64_t most = (max_len_k + least - 1) / least;
   splits = splits < most ? splits : most;
   splits = splits < 1 ? 1 : splits > 256 ? 256 : splits;
   int64_t chunk = (max_len_k + splits - 1) / splits;
   chunk = (chunk + 127) / 128 * 128;
-  p.chunk = (int)(chunk < 128 ? 128 : chunk);
+  p.chunk = (int)(chunk < least ? least : chunk);
   p.splits = (max_len_k + p.chunk - 1) / p.chunk;
   if (p.splits < 1) p.splits = 1;
   return p;
@@ -890,7 +886,7 @@ int mtq_kv_read(const mtq_kv_cache *cache, void *k, void *v, const int64_t *stri
 size_t mtq_kv_attention_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim, int max_len_q, int max_len_k) {
   if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_len_q < 1 || head_dim < 1) return 0;
   const Plan p = attn_plan(batch, num_kv_heads, num_q_heads / num_kv_heads, head_dim, max_len_q, max_len_k);
-  return p.splits > 1 ? (size_t)p.splits * batch * num_kv_heads * p.tiles * 16 * (head_dim + 4) * sizeof(float) : 0;
+  return p.splits > 1 ? (size_t)p.splits * batch * num_kv_heads * p.part_tiles * 16 * (head_dim + 4) * sizeof(float) : 0;
 }
 
 int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const int64_t *strides, int64_t rows, int num_q_heads,
@@ -914,24 +910,26 @@ int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const in
   const Plan p = attn_plan(batch, a.c.hkv, a.group, a.c.head_dim, max_len_q, max_len_k);
   const int64_t pg = ((int64_t)batch * a.c.hkv + 7) / 8 * 8 * p.tiles;  // the prompt kernel's grid
   if (p.prompt ? pg > INT32_MAX : (int64_t)p.tiles * a.c.hkv > 65535) return MTQ_ERR_INVALID_ARG;
+  if (p.splits > 1 && (int64_t)p.part_tiles * a.c.hkv > 65535) return MTQ_ERR_INVALID_ARG;
   const size_t need = mtq_kv_attention_workspace_bytes(batch, num_q_heads, a.c.hkv, a.c.head_dim, max_len_q, max_len_k);
   if (need && (!ws || ws_bytes < need || !al16p(ws))) return MTQ_ERR_INVALID_ARG;
   a.q = q, a.o = o, a.part = (float *)ws;
   a.qt = strides[0], a.qh = strides[1], a.ot = strides[2], a.oh = strides[3], a.rows = rows;
   a.causal = is_causal ? 1 : 0;
-  a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles, a.batch = batch;
+  a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles, a.part_tiles = p.part_tiles, a.batch = batch;
   a.sm_log2 = (float)(softmax_scale * 1.44269504088896);
-  const dim3 g((unsigned)p.splits, (unsigned)(p.tiles * a.c.hkv), (unsigned)batch), gj(1, g.y, g.z);
+  const dim3 g((unsigned)p.splits, (unsigned)(p.tiles * a.c.hkv), (unsigned)batch), gj(1, (unsigned)(p.part_tiles * a.c.hkv), (unsigned)batch);
   auto go = [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
     if constexpr (D <= 128) {
-      if (p.prompt) {
-        attn_prompt_kernel<T, D><<<(unsigned)pg, 256, 0, stream>>>(a);
-        return host_check_launch();
-      }
+      if (p.prompt)
+        attn_prompt_kernel<T, D><<<dim3((unsigned)pg, (unsigned)p.splits), 512, 0, stream>>>(a);
+      else
+        attn_decode_kernel<T, D><<<g, 256, 0, stream>>>(a);
+    } else {
+      attn_decode_kernel<T, D><<<g, 256, 0, stream>>>(a);
     }
-    attn_decode_kernel<T, D><<<g, 256, 0, stream>>>(a);
     const int st = host_check_launch();
     if (st != MTQ_OK || p.splits == 1) return st;
     attn_join_kernel<T, D><<<gj, 256, 0, stream>>>(a);
