@@ -54,13 +54,16 @@ __device__ __forceinline__ float global_scale_of(const float *amax) {
   return gs > 0.f ? gs : 1e-12f;
 }
 
-// the page of position pos, -1 where there is none
-__device__ __forceinline__ int page_of(const Cache &c, int b, int pos) {
+// the page of position pos, -1 where there is none: the table's entry, which is loaded without a branch
+// (page_entry) so that a loop can have it in flight, and what it says (page_at)
+__device__ __forceinline__ int page_entry(const Cache &c, int b, int pos) {
   const int slot = pos >> c.shift;
-  if (pos < 0 || slot >= c.table_cols) return -1;
-  const int page = c.table[(int64_t)b * c.table_stride + slot];
-  return page >= 0 && page < c.num_pages ? page : -1;
+  return c.table[(int64_t)b * c.table_stride + ((uint32_t)slot < (uint32_t)c.table_cols ? slot : 0)];
 }
+__device__ __forceinline__ int page_at(const Cache &c, int pos, int entry) {
+  return (uint32_t)(pos >> c.shift) < (uint32_t)c.table_cols && (uint32_t)entry < (uint32_t)c.num_pages ? entry : -1;
+}
+__device__ __forceinline__ int page_of(const Cache &c, int b, int pos) { return page_at(c, pos, page_entry(c, b, pos)); }
 
 // ---- rows into pages and back -------------------------------------------------------------------
 // A lane takes one block: 16 columns of one row.  Bound by HBM (32 + 9 bytes a block); consecutive
@@ -360,18 +363,44 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
   const uint8_t *kd = c.data[0] + kvh * c.d_head[0] + g * (D / 8), *ks = c.scale[0] + kvh * c.s_head[0] + g * (D / 64);
   const uint8_t *vd = c.data[1] + kvh * c.d_head[1] + g * (D / 8), *vs = c.scale[1] + kvh * c.s_head[1] + g * (D / 64);
 
-  for (int kv = t0 + 32 * wave; kv < t1; kv += 128) {
+  // 32 keys' codes; those of the wave's next 32 keys and the pages of the 32 after them are in flight while
+  // these are used
+  struct Codes {
     uint32_t kw[2][NF], vw[2][NF], ksc[2], vsc[2];
     bool has[2];
+  };
+  auto entries = [&](int kv, int (&e)[2]) {  // 16 keys: one page
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {  // 16 keys: one page
-      const int page = __builtin_amdgcn_readfirstlane(page_of(c, b, kv + 16 * u));
-      has[u] = page >= 0;
-      const int64_t pg = has[u] ? page : 0;
+    for (int u = 0; u < 2; ++u) e[u] = page_entry(c, b, __builtin_amdgcn_readfirstlane(kv + 16 * u));
+  };
+  auto fetch = [&](int kv, const int (&e)[2], Codes &d) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int page = page_at(c, kv + 16 * u, e[u]);
+      d.has[u] = page >= 0;
+      const int64_t pg = d.has[u] ? page : 0;
       const int at = ((kv + 16 * u) & ((1 << c.shift) - 1)) + t;
-      load_codes<D>(kd + pg * c.d_page[0] + at * c.d_tok[0], ks + pg * c.s_page[0] + at * c.s_tok[0], kw[u], ksc[u]);
-      load_codes<D>(vd + pg * c.d_page[1] + at * c.d_tok[1], vs + pg * c.s_page[1] + at * c.s_tok[1], vw[u], vsc[u]);
+      load_codes<D>(kd + pg * c.d_page[0] + at * c.d_tok[0], ks + pg * c.s_page[0] + at * c.s_tok[0], d.kw[u], d.ksc[u]);
+      load_codes<D>(vd + pg * c.d_page[1] + at * c.d_tok[1], vs + pg * c.s_page[1] + at * c.s_tok[1], d.vw[u], d.vsc[u]);
     }
+  };
+  Codes nxt;
+  int ent[2];
+  const int kv_first = t0 + 32 * wave;
+  if (kv_first < t1) {
+    entries(kv_first, ent);
+    fetch(kv_first, ent, nxt);
+    entries(kv_first + 128, ent);
+  }
+  for (int kv = kv_first; kv < t1; kv += 128) {
+    const Codes now = nxt;
+    fetch(kv + 128, ent, nxt);  // past the end: keys of any page, not used
+    entries(kv + 256, ent);
+    const auto &kw = now.kw;
+    const auto &vw = now.vw;
+    const auto &ksc = now.ksc;
+    const auto &vsc = now.vsc;
+    const auto &has = now.has;
     // ---- scores
     f32x4 s[2];
 #pragma unroll
@@ -473,44 +502,46 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
   }
 }
 
-// the splits of a row, in order
+// the splits of a row, in order: a workgroup a row, D / 4 lanes for its columns, 1024 / D splits at a time
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  constexpr int LN = D / 4, NG = 256 / LN;
+  __shared__ f32x4 ob[NG][LN];
+  __shared__ float lb[NG];
   const Cache &c = a.c;
-  const int kvh = blockIdx.y / a.part_tiles, tile = blockIdx.y % a.part_tiles, b = blockIdx.z;
-  const int lq = c.len_q[b];
-  int lk = c.len_k[b];
-  const int cap = c.table_cols << c.shift, off = lk - lq;
-  lk = lk < cap ? lk : cap;
-  const int nrows = lq > 0 ? lq * a.group : 0;
-  if (16 * tile >= nrows) return;
-  const int last_tok = (16 * tile + 15 < nrows ? 16 * tile + 15 : nrows - 1) / a.group;
-  int kv_end = a.causal ? off + last_tok + 1 : lk;
+  const int kvh = blockIdx.y, row = blockIdx.x, b = blockIdx.z, grp = threadIdx.x / LN, d4 = 4 * (threadIdx.x % LN);
+  const int lq = c.len_q[b], off = c.len_k[b] - lq, cap = c.table_cols << c.shift;
+  const int lk = c.len_k[b] < cap ? c.len_k[b] : cap;
+  if (row >= (lq > 0 ? lq * a.group : 0)) return;
+  const int64_t orow = (int64_t)c.start[b] + row / a.group;
+  if (orow < 0 || orow >= a.rows) return;
+  int kv_end = a.causal ? off + row / a.group + 1 : lk;
   kv_end = kv_end < lk ? kv_end : lk;
   int n = kv_end > 0 ? (kv_end + a.chunk - 1) / a.chunk : 1;
   n = n < a.splits ? n : a.splits;
-  const float gv = global_scale_of(c.amax[1]);
   const int64_t step = (int64_t)a.batch * c.hkv * a.part_tiles * 16 * (D + 4);
-  for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
-    const int r = i / (D / 4), d4 = 4 * (i % (D / 4)), rr = 16 * tile + r;
-    const int64_t orow = (int64_t)c.start[b] + rr / a.group;
-    if (rr >= nrows || orow < 0 || orow >= a.rows) continue;
-    const float *pp = a.part + part_row<D>(a, 0, b, kvh, rr);
-    float mm = kNegInf;
-    for (int s = 0; s < n; ++s) mm = fmaxf(mm, pp[s * step + D]);
-    const float mu = mm == kNegInf ? 0.f : mm;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float ls = 0.f;
-    for (int s = 0; s < n; ++s) {
-      const float f = __builtin_amdgcn_exp2f(pp[s * step + D] - mu);
-      ls += pp[s * step + D + 1] * f;
-      o += *reinterpret_cast<const f32x4 *>(pp + s * step + d4) * f;
-    }
-    const float inv = gv / ls;
-    T *op = reinterpret_cast<T *>(a.o) + orow * a.ot + (kvh * a.group + rr % a.group) * a.oh + d4;
+  const float *pp = a.part + part_row<D>(a, 0, b, kvh, row);
+  float m = kNegInf;
+  for (int s = threadIdx.x % 64; s < n; s += 64) m = fmaxf(m, pp[s * step + D]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) op[j] = Elem<T>::st(ls == 0.f ? 0.f : o[j] * inv);
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  const float mu = m == kNegInf ? 0.f : m;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  for (int s = grp; s < n; s += NG) {
+    const float f = __builtin_amdgcn_exp2f(pp[s * step + D] - mu);
+    l += pp[s * step + D + 1] * f;
+    o += *reinterpret_cast<const f32x4 *>(pp + s * step + d4) * f;
   }
+  ob[grp][threadIdx.x % LN] = o;
+  if (d4 == 0) lb[grp] = l;
+  __syncthreads();
+  if (grp) return;
+  for (int g = 1; g < NG; ++g) o += ob[g][threadIdx.x], l += lb[g];
+  const float inv = global_scale_of(c.amax[1]) / l;
+  T *op = reinterpret_cast<T *>(a.o) + orow * a.ot + (kvh * a.group + row % a.group) * a.oh + d4;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) op[j] = Elem<T>::st(l == 0.f ? 0.f : o[j] * inv);
 }
 
 // ---- attention of prompts ------------------------------------------------------------------------
@@ -620,12 +651,19 @@ __global__ __launch_bounds__(512, 2) void attn_prompt_kernel(AttnArgs a) {
   const int64_t s_page = skv ? c.s_page[1] : c.s_page[0], s_tok = skv ? c.s_tok[1] : c.s_tok[0];
   const uint8_t *const dbase = (skv ? c.data[1] + kvh * c.d_head[1] : c.data[0] + kvh * c.d_head[0]) + sg * (D / 8);
   const uint8_t *const sbase = (skv ? c.scale[1] + kvh * c.s_head[1] : c.scale[0] + kvh * c.s_head[0]) + sg * (D / 64);
-  auto gload = [&](int t) {
+  struct Entries {
+    int group[4], mine;
+  };
+  auto entries = [&](int t, Entries &e) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) e.group[u] = page_entry(c, b, 64 * t + 16 * u);
+    e.mine = page_entry(c, b, 64 * t + skey);
+  };
+  auto gload = [&](int t, const Entries &e) {
     pages = 0;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) pages |= (page_of(c, b, 64 * t + 16 * u) >= 0 ? 1 : 0) << u;
-    pages = __builtin_amdgcn_readfirstlane(pages);
-    const int key = 64 * t + skey, page = page_of(c, b, key), at = key & ((1 << c.shift) - 1);
+    for (int u = 0; u < 4; ++u) pages |= (page_at(c, 64 * t + 16 * u, e.group[u]) >= 0 ? 1 : 0) << u;
+    const int key = 64 * t + skey, page = page_at(c, key, e.mine), at = key & ((1 << c.shift) - 1);
     const int64_t pg = page >= 0 ? page : 0;
     load_codes<D>(dbase + pg * d_page + at * d_tok, sbase + pg * s_page + at * s_tok, cw, csc);
     cok = skv == 0 || (page >= 0 && key < lk);  // V of no token of this sequence: zeros (0 * NaN is NaN)
@@ -699,10 +737,14 @@ __global__ __launch_bounds__(512, 2) void attn_prompt_kernel(AttnArgs a) {
   if (t0 < stages) {
     // V of "tile -1" is multiplied by weights of zero: it has to be finite
     for (int i = tid; i < VIMG / 16; i += 512) *reinterpret_cast<uint4 *>(lds + 2 * STAGE + KIMG + 16 * i) = make_uint4(0, 0, 0, 0);
-    gload(t0);
+    Entries ent;
+    entries(t0, ent);
+    gload(t0, ent);
+    entries(t0 + 1, ent);
     int pg0 = pages;
     swrite(0);
-    gload(t0 + 1 < stages ? t0 + 1 : t0);
+    gload(t0 + 1, ent);  // past the end: keys of any page, not used
+    entries(t0 + 2, ent);
     int pg1 = pages;
     __syncthreads();
     f32x16 sc, sn;
@@ -728,7 +770,8 @@ __global__ __launch_bounds__(512, 2) void attn_prompt_kernel(AttnArgs a) {
       // tile 2 t: scores of 2 t + 1, V of 2 t - 1
       mask(sc, 64 * t, pg0 & 3);
       swrite(nx);                                   // stage t + 1 (read by none before the barrier below)
-      gload(t + 2 < stages ? t + 2 : stages - 1);   // in flight under the rest of this stage
+      gload(t + 2, ent);                            // in flight under the rest of this stage
+      entries(t + 3, ent);
       const int pg2 = pages;
       score(Kc + 32 * KP, sn);
       bool moved = soft(sc, pc, corr);
@@ -910,7 +953,7 @@ int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const in
   const Plan p = attn_plan(batch, a.c.hkv, a.group, a.c.head_dim, max_len_q, max_len_k);
   const int64_t pg = ((int64_t)batch * a.c.hkv + 7) / 8 * 8 * p.tiles;  // the prompt kernel's grid
   if (p.prompt ? pg > INT32_MAX : (int64_t)p.tiles * a.c.hkv > 65535) return MTQ_ERR_INVALID_ARG;
-  if (p.splits > 1 && (int64_t)p.part_tiles * a.c.hkv > 65535) return MTQ_ERR_INVALID_ARG;
+  if (a.c.hkv > 65535) return MTQ_ERR_INVALID_ARG;
   const size_t need = mtq_kv_attention_workspace_bytes(batch, num_q_heads, a.c.hkv, a.c.head_dim, max_len_q, max_len_k);
   if (need && (!ws || ws_bytes < need || !al16p(ws))) return MTQ_ERR_INVALID_ARG;
   a.q = q, a.o = o, a.part = (float *)ws;
@@ -918,7 +961,7 @@ int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const in
   a.causal = is_causal ? 1 : 0;
   a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles, a.part_tiles = p.part_tiles, a.batch = batch;
   a.sm_log2 = (float)(softmax_scale * 1.44269504088896);
-  const dim3 g((unsigned)p.splits, (unsigned)(p.tiles * a.c.hkv), (unsigned)batch), gj(1, (unsigned)(p.part_tiles * a.c.hkv), (unsigned)batch);
+  const dim3 g((unsigned)p.splits, (unsigned)(p.tiles * a.c.hkv), (unsigned)batch), gj((unsigned)(max_len_q * a.group), (unsigned)a.c.hkv, (unsigned)batch);
   auto go = [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
