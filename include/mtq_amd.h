@@ -501,7 +501,7 @@ int mtq_mx_linear(const void *x, int64_t x_stride, int x_dtype, const void *x_sc
 /* ---- KV cache in 4 bits (NVFP4), in pages ------------------------------------------------------
  * Place (page, head, token) of K (index 0) or V (1): head_dim / 2 bytes of E2M1 codes at data +
  * page * data_strides[.][0] + head * [1] + token * [2] (bytes, multiples of 16) and head_dim / 16
- * E4M3 scales at scale + ... (multiples of head_dim / 16); amax: the tensor's fp32 amax on the
+ * E4M3 scales at scale + ... (multiples of head_dim / 16), token strides below 2^26; amax: the tensor's fp32 amax on the
  * device (global scale amax / 2688).  Values as mtq_nvfp4_fake_quant of the rows.  page_size: a
  * power of two in 16 .. 32768; head_dim 64, 128 or 256. */
 typedef struct {

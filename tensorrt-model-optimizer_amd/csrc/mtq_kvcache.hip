@@ -30,6 +30,7 @@ int host_num_cus();
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -37,7 +38,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 inline bool al16p(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-constexpr float kNegInf = -__builtin_inff(), kPShift = 12.0f;
+constexpr float kNegInf = -__builtin_inff();
+// probabilities are held as 2^kShift exp2(x - m), m at most kSlack below the largest x so far
+constexpr float kShift = 6.0f, kSlack = 8.0f;
 
 struct Cache {
   uint8_t *data[2], *scale[2];                        // K, V
@@ -225,8 +228,9 @@ __global__ __launch_bounds__(256) void cache_read_kernel(RowArgs a) {
 //   q: to fp16 with a power of two of its row that puts its largest value into [2^14, 2^15): 8
 //      (bf16) or 11 (fp16) bits stay exact down to 2^-28 of it.
 //   V: the same products, through LDS rows that ds_read_b64_tr_b16 reads transposed.
-//   P: fp16, 2^12 exp2(x - running maximum): off by 2^-12 of each weight, and a normal number down to
-//      2^-26 of the largest; the row sum carries the same 2^12.
+//   P: fp16, 2^6 exp2(x - m), off by 2^-12 of each weight and a normal number down to 2^-20 of the
+//      largest; the row sum carries the same 2^6.  m follows the running maximum only where a key exceeds it
+//      by 2^8 (weights then reach 2^14, inside fp16): most steps neither exchange maxima nor rescale O.
 // Sums and the accumulators are fp32.
 //
 // A wave takes 32 keys at a time, the waves of a workgroup every fourth 32 keys, and keep statistics
@@ -359,48 +363,49 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
 #pragma unroll
   for (int d = 0; d < NB; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = kNegInf, l = 0.f;
+  // keys below wmin need no mask in any of the wave's rows
+  int wmin = row_ok ? see : 0x7fffffff;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    const int v = __shfl_xor(wmin, o, 64);
+    wmin = v < wmin ? v : wmin;
+  }
+  wmin = __builtin_amdgcn_readfirstlane(wmin);
   unsigned char *const vb = lds + wave * kVBytes;
-  const uint8_t *kd = c.data[0] + kvh * c.d_head[0] + g * (D / 8), *ks = c.scale[0] + kvh * c.s_head[0] + g * (D / 64);
-  const uint8_t *vd = c.data[1] + kvh * c.d_head[1] + g * (D / 8), *vs = c.scale[1] + kvh * c.s_head[1] + g * (D / 64);
+  // a key's codes: the page's place (uniform) + a lane's offset in 16 keys (32 bits: token strides are below 2^26)
+  const uint32_t kdo = t * (uint32_t)c.d_tok[0] + g * (D / 8), kso = t * (uint32_t)c.s_tok[0] + g * (D / 64);
+  const uint32_t vdo = t * (uint32_t)c.d_tok[1] + g * (D / 8), vso = t * (uint32_t)c.s_tok[1] + g * (D / 64);
 
-  // 32 keys' codes; those of the wave's next 32 keys and the pages of the 32 after them are in flight while
-  // these are used
-  struct Codes {
-    uint32_t kw[2][NF], vw[2][NF], ksc[2], vsc[2];
-    bool has[2];
-  };
+  // 32 keys' codes: K's registers are loaded anew (the wave's next 32 keys) as soon as its fp16 products are
+  // made, V's as soon as its are; the pages of the 32 keys after those are in flight too
+  uint32_t kw[2][NF], vw[2][NF], ksc[2], vsc[2];
   auto entries = [&](int kv, int (&e)[2]) {  // 16 keys: one page
 #pragma unroll
     for (int u = 0; u < 2; ++u) e[u] = page_entry(c, b, __builtin_amdgcn_readfirstlane(kv + 16 * u));
   };
-  auto fetch = [&](int kv, const int (&e)[2], Codes &d) {
+  auto fetch = [&](int i, int kv, const int (&page)[2], uint32_t (&w)[2][NF], uint32_t (&sc)[2]) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int page = page_at(c, kv + 16 * u, e[u]);
-      d.has[u] = page >= 0;
-      const int64_t pg = d.has[u] ? page : 0;
-      const int at = ((kv + 16 * u) & ((1 << c.shift) - 1)) + t;
-      load_codes<D>(kd + pg * c.d_page[0] + at * c.d_tok[0], ks + pg * c.s_page[0] + at * c.s_tok[0], d.kw[u], d.ksc[u]);
-      load_codes<D>(vd + pg * c.d_page[1] + at * c.d_tok[1], vs + pg * c.s_page[1] + at * c.s_tok[1], d.vw[u], d.vsc[u]);
+      const int64_t pg = page[u] >= 0 ? page[u] : 0, at = (kv + 16 * u) & ((1 << c.shift) - 1);
+      load_codes<D>(c.data[i] + (kvh * c.d_head[i] + pg * c.d_page[i] + at * c.d_tok[i]) + (i ? vdo : kdo),
+                    c.scale[i] + (kvh * c.s_head[i] + pg * c.s_page[i] + at * c.s_tok[i]) + (i ? vso : kso), w[u], sc[u]);
     }
   };
-  Codes nxt;
-  int ent[2];
+  int ent[2], page[2] = {-1, -1};
   const int kv_first = t0 + 32 * wave;
   if (kv_first < t1) {
     entries(kv_first, ent);
-    fetch(kv_first, ent, nxt);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) page[u] = page_at(c, kv_first + 16 * u, ent[u]);
     entries(kv_first + 128, ent);
+    fetch(0, kv_first, page, kw, ksc);
+    fetch(1, kv_first, page, vw, vsc);
   }
   for (int kv = kv_first; kv < t1; kv += 128) {
-    const Codes now = nxt;
-    fetch(kv + 128, ent, nxt);  // past the end: keys of any page, not used
+    const bool has[2] = {page[0] >= 0, page[1] >= 0};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) page[u] = page_at(c, kv + 128 + 16 * u, ent[u]);
     entries(kv + 256, ent);
-    const auto &kw = now.kw;
-    const auto &vw = now.vw;
-    const auto &ksc = now.ksc;
-    const auto &vsc = now.vsc;
-    const auto &has = now.has;
     // ---- scores
     f32x4 s[2];
 #pragma unroll
@@ -411,6 +416,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
 #pragma unroll
       for (int f = 0; f < NF; ++f) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[f], qf[f], s[u], 0, 0, 0);
     }
+    fetch(0, kv + 128, page, kw, ksc);  // past the end: keys of any page, not used
     // ---- V to LDS (rows that hold no token of this sequence as zeros: 0 * NaN is NaN)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -420,32 +426,38 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
       for (int f = 0; f < NF; ++f)
         *reinterpret_cast<h8 *>(vb + (16 * u + t) * VP + g * (D / 2) + 16 * f) = vf[f];
     }
+    fetch(1, kv + 128, page, vw, vsc);
     // ---- softmax: keys kv + 16 u + 4 g + j
-    float x[2][4], mx = kNegInf;
+    if (kv + 32 > wmin || !has[0] || !has[1]) {  // wave-uniform
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[u][j] = has[u] && kv + 16 * u + 4 * g + j < see ? s[u][j] * qscale : kNegInf;
-        mx = fmaxf(mx, x[u][j]);
-      }
-    const float mn = fmaxf(m, max_g(mx));
-    const float mu = mn == kNegInf ? 0.f : mn;
-    const float corr = __builtin_amdgcn_exp2f(m - mu);
-    m = mn;
+        for (int j = 0; j < 4; ++j) s[u][j] = has[u] && kv + 16 * u + 4 * g + j < see ? s[u][j] : kNegInf;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[j >> 2][j & 3]);
+    mx *= qscale;
+    // the running maximum moves only where a key of the wave exceeds its row's by 2^kSlack
+    if (__builtin_amdgcn_ballot_w64(mx > m + kSlack)) {
+      const float mn = fmaxf(m, max_g(mx));
+      const float corr = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.f : mn));
+      m = mn;
+      l *= corr;
+#pragma unroll
+      for (int d = 0; d < NB; ++d) acc[d] *= corr;
+    }
+    const float mu = (m == kNegInf ? 0.f : m) - kShift;
     h8 p;
-    float ls = 0.f;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = __builtin_amdgcn_exp2f(x[u][j] - (mu - kPShift));
-        ls += e;
-        p[4 * u + j] = (_Float16)e;
-      }
-    l = l * corr + ls;  // this lane's keys only; joined at the end
-#pragma unroll
-    for (int d = 0; d < NB; ++d) acc[d] *= corr;
+    for (int j = 0; j < 8; j += 2) {
+      const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], qscale, -mu));
+      const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][(j & 3) + 1], qscale, -mu));
+      l += e0;  // this lane's keys only; joined at the end
+      l += e1;
+      const h2 h = __builtin_convertvector((f2v{e0, e1}), h2);
+      p[j] = h.x, p[j + 1] = h.y;
+    }
     // ---- O^T += V^T P^T
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -554,10 +566,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 // tokens behind contexts of up to 8192, 4 sequences, 32 / 8 heads: nothing of its one wave overlaps.)
 // The loop over 32-key tiles is pipelined in registers: the step of tile j multiplies K of tile j + 1
 // and V of tile j - 1 while the softmax of tile j runs, three chains without a dependency between them.
-// The running maximum moves (and O is rescaled) only where a tile exceeds it by 2^8: weights then reach
-// 2^(8 + kPromptShift), inside fp16.
-constexpr float kPromptShift = 6.0f, kPromptSlack = 8.0f;
-
 __device__ __forceinline__ float xmax32(float v) {  // v and its lane ^ 32 partner
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -567,7 +575,6 @@ __device__ __forceinline__ float xadd32(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f2v __attribute__((ext_vector_type(2)));
 
 // key (of a 32-key tile) of score register j in half hi
 __device__ __forceinline__ int crow(int j, int hi) { return (j & 3) + 8 * (j >> 2) + 4 * hi; }
@@ -705,10 +712,10 @@ __global__ __launch_bounds__(512, 2) void attn_prompt_kernel(AttnArgs a) {
 #pragma unroll
     for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
     mx = xmax32(mx) * qs;
-    const bool up = mx > m + kPromptSlack;
+    const bool up = mx > m + kSlack;
     corr = up ? __builtin_amdgcn_exp2f(m - mx) : 1.f;  // m = -inf: 0
     m = up ? mx : m;
-    const float mu = (m == kNegInf ? 0.f : m) - kPromptShift;
+    const float mu = (m == kNegInf ? 0.f : m) - kShift;
     float ls = 0.f;
 #pragma unroll
     for (int g = 0; g < 2; ++g)
@@ -838,6 +845,7 @@ bool make_cache(const mtq_kv_cache *k, const int32_t *table, int64_t table_strid
     if ((uintptr_t)c.data[i] % 16 || (uintptr_t)c.scale[i] % sb) return false;
     for (int j = 0; j < 3; ++j)
       if (k->data_strides[i][j] < 0 || k->data_strides[i][j] % 16 || k->scale_strides[i][j] < 0 || k->scale_strides[i][j] % sb) return false;
+    if (k->data_strides[i][2] >= (1 << 26) || k->scale_strides[i][2] >= (1 << 26)) return false;
   }
   c.table = table, c.start = start, c.len_q = len_q, c.len_k = len_k, c.table_stride = table_stride;
   c.table_cols = table_cols, c.num_pages = k->num_pages, c.hkv = k->num_kv_heads, c.head_dim = k->head_dim;
@@ -886,8 +894,8 @@ struct Plan {
 // rows of a KV head from which the prompt kernel is taken
 constexpr int kPromptRows = 128;
 
-// Splits of the keys: enough workgroups to fill the card (decode: 8 a CU, a split at least 128 keys, one
-// 32-key step a wave; prompts: one a CU, at least 512 keys)
+// Splits of the keys: enough workgroups to fill the card (decode: 6 a CU, a split at least 256 keys, two
+// 32-key steps a wave; prompts: one a CU, at least 512 keys)
 Plan attn_plan(int batch, int hkv, int group, int head_dim, int max_len_q, int max_len_k) {
   Plan p;
   const int64_t rows = (int64_t)max_len_q * group;
@@ -895,8 +903,8 @@ Plan attn_plan(int batch, int hkv, int group, int head_dim, int max_len_q, int m
   p.part_tiles = (int)((rows + 15) / 16);
   p.tiles = p.prompt ? (int)((rows + 255) / 256) : p.part_tiles;
   const int64_t wgs = (int64_t)batch * hkv * p.tiles, cus = host_num_cus();
-  const int least = p.prompt ? 512 : 128;
-  int64_t splits = p.prompt ? cus / wgs : (8 * cus + wgs - 1) / wgs;
+  const int least = p.prompt ? 512 : 256;
+  int64_t splits = p.prompt ? cus / wgs : (6 * cus + wgs - 1) / wgs;
   const int64_t most = (max_len_k + least - 1) / least;
   splits = splits < most ? splits : most;
   splits = splits < 1 ? 1 : splits > 256 ? 256 : splits;
