@@ -251,6 +251,17 @@ template <int D> __device__ __forceinline__ int64_t part_row(const AttnArgs &a, 
   return (((((int64_t)split * a.batch + b) * a.c.hkv + kvh) * a.part_tiles + (row >> 4)) * 16 + (row & 15)) * (D + 4);
 }
 
+// Weights are 2^(s qs - m) in one fused step, so that m, which is rounded, leaves the rounding of the largest
+// score in the exponent: the same for all keys, and below 1 while |s qs| < 2^24.  Rows that could get past
+// that (|s| <= D 2^15 2688, so real scores beyond 10^7) have their scores multiplied by pre before, where they
+// would be masked, and qs = 1: every product with m is then exact.
+template <int D> __device__ __forceinline__ bool split_scale(float &qs, float &pre) {
+  const bool far = qs * (float)(D * 2688) > 512.f;
+  pre = far ? qs : 1.f;
+  qs = far ? 1.f : qs;
+  return far;
+}
+
 // fp16 values of a lane's D / 4 codes times their block scales; ok false: zeros
 template <int D>
 __device__ __forceinline__ void dequant(const uint32_t (&w)[D / 32], uint32_t sc, bool ok, h8 (&f)[D / 32]) {
@@ -334,7 +345,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
   const bool row_ok = row < nrows && qrow >= 0 && qrow < a.rows;
   const int see = row_ok ? (a.causal ? (off + rtok + 1 < lk ? off + rtok + 1 : lk) : lk) : 0;  // keys it sees
   h8 qf[NF];
-  float qscale;
+  float qscale, pre;
+  bool far;
   {
     float v[NF][8];
     float m = 0.f;
@@ -353,6 +365,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
     e = m == 0.f || e == 128 ? 0 : e < -100 ? -100 : e;  // inf: left as it is
     const float up = pow2f(14 - e < 127 ? 14 - e : 127);
     qscale = fmaxf(a.sm_log2 * global_scale_of(c.amax[0]) * (1.0f / up), 1e-37f);  // > 0: scores of -inf stay -inf
+    far = split_scale<D>(qscale, pre);
 #pragma unroll
     for (int f = 0; f < NF; ++f)
 #pragma unroll
@@ -363,8 +376,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
 #pragma unroll
   for (int d = 0; d < NB; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = kNegInf, l = 0.f;
-  // keys below wmin need no mask in any of the wave's rows
-  int wmin = row_ok ? see : 0x7fffffff;
+  // keys below wmin need neither a mask nor pre in any of the wave's rows
+  int wmin = row_ok ? (far ? 0 : see) : 0x7fffffff;
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) {
     const int v = __shfl_xor(wmin, o, 64);
@@ -432,7 +445,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[u][j] = has[u] && kv + 16 * u + 4 * g + j < see ? s[u][j] : kNegInf;
+        for (int j = 0; j < 4; ++j) s[u][j] = has[u] && kv + 16 * u + 4 * g + j < see ? s[u][j] * pre : kNegInf;
     }
     float mx = s[0][0];
 #pragma unroll
@@ -607,14 +620,13 @@ __global__ __launch_bounds__(512, 2) void attn_prompt_kernel(AttnArgs a) {
 
   // ---- this lane's row of q
   h8 qf[QS];
-  float qs;
-  int see, wmin = 0x7fffffff;  // keys a row sees; keys below wmin need no mask in any of the wave's rows
+  float qs, pre;
+  int see, wmin = 0x7fffffff;  // keys a row sees; keys below wmin need neither a mask nor pre in any of the wave's rows
   {
     const int row = 256 * tile + 32 * wave + fr, rtok = row / a.group, head = kvh * a.group + row % a.group;
     const int64_t qrow = (int64_t)c.start[b] + rtok;
     const bool ok = row < nrows && qrow >= 0 && qrow < a.rows;
     see = ok ? (a.causal ? (off + rtok + 1 < lk ? off + rtok + 1 : lk) : lk) : 0;
-    wmin = ok && see < wmin ? see : wmin;
     const T *qp = reinterpret_cast<const T *>(a.q) + (ok ? qrow : 0) * a.qt + head * a.qh + 8 * hi;
     Vec<T> x[QS];
     float m = 0.f;
@@ -630,6 +642,8 @@ __global__ __launch_bounds__(512, 2) void attn_prompt_kernel(AttnArgs a) {
     e = m == 0.f || e == 128 ? 0 : e < -100 ? -100 : e;
     const float up = pow2f(14 - e < 127 ? 14 - e : 127);
     qs = fmaxf(a.sm_log2 * global_scale_of(c.amax[0]) * (1.0f / up), 1e-37f);
+    const bool far = split_scale<D>(qs, pre);
+    wmin = ok ? (far ? 0 : see) : wmin;
 #pragma unroll
     for (int s = 0; s < QS; ++s)
 #pragma unroll
@@ -737,7 +751,7 @@ __global__ __launch_bounds__(512, 2) void attn_prompt_kernel(AttnArgs a) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int k = crow(e, hi);
-      s[e] = kv0 + k < see && (pg >> (k >> 4) & 1) ? s[e] : kNegInf;
+      s[e] = kv0 + k < see && (pg >> (k >> 4) & 1) ? s[e] * pre : kNegInf;
     }
   };
 

@@ -111,7 +111,8 @@ def _restore_compressed(model: nn.Module, entry: dict) -> None:
     from ..quantization.compress import CompressConfig, compress_convert
     from ..quantization.qtensor import QTensorWrapper
 
-    cfg = CompressConfig(entry["config"].get("compress"), entry["config"].get("quant_gemm", True))
+    cfg = CompressConfig(entry["config"].get("compress"), entry["config"].get("quant_gemm", True),
+                         entry["config"].get("mx_gemm", False))
     compress_convert(model, cfg, skip_real_quantize_weight=True)
     meta = entry["metadata"]
     for name, m in model.named_modules():
