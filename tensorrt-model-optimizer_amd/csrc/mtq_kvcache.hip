@@ -69,148 +69,165 @@ __device__ __forceinline__ int page_at(const Cache &c, int pos, int entry) {
 __device__ __forceinline__ int page_of(const Cache &c, int b, int pos) { return page_at(c, pos, page_entry(c, b, pos)); }
 
 // ---- rows into pages and back -------------------------------------------------------------------
-// A lane takes one block: 16 columns of one row.  Bound by HBM (32 + 9 bytes a block); consecutive
-// lanes take consecutive blocks, so a wave reads 2 KiB and writes 512 + 64 bytes in one piece each.
+// A lane takes 8 columns of a row, two lanes a block, so that 16-bit rows move in whole 16-byte pieces of
+// neighbouring lanes.  A workgroup takes tokens of one head where the call has them (2^lt of them, then heads):
+// in the cache's layout these lie behind each other, 16 of them at head_dim 128 being 1 KiB of codes and a
+// line of scales, while k and v are met in pieces of a row (256 bytes there).  Bound by HBM (16 + 4.5 bytes a
+// lane): 3.4 TB/s each way at the size below.
 struct RowArgs {
   Cache c;
   void *x[2];             // k, v
   int64_t xt[2], xh[2];   // element strides (token, head)
   int64_t rows;
-  int max_len, tok_per_wg;
+  int lt, passes;
 };
+// Tokens of a lane in flight at once, and whether it loops over more.  us for the prompts of 7 sequences, 131 MB
+// at 8 heads of 128: 1 / 2 / 4 tokens: append 51 / 46 / 44, read 50 / 45 / 39; looping, with at most 48
+// workgroups a CU: append 38 / 39 / 45, read 46 / 46 / 43 (16 workgroups: over 50, the sequences are unequal)
+constexpr int kAppendAhead = 2, kReadAhead = 4, kAppendWgs = 48;
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load16(const T *p, float (&v)[16]) {
-  if constexpr (VEC) {
+// what a lane works on: false where there is none of it
+struct RowLane {
+  int kv, h, col, first, step, end;  // tokens first, first + step, .. below end
+};
+template <int AHEAD> __device__ __forceinline__ bool row_lane(const RowArgs &a, int lq, RowLane &r) {
+  const int ll = 28 - __builtin_clz(a.c.head_dim), lr = 8 - ll;  // 2^ll lanes a row, 2^lr rows a pass
+  const int row = threadIdx.x >> ll;
+  const int kvh = (blockIdx.z << (lr - a.lt)) + (row >> a.lt);
+  r.col = 8 * (threadIdx.x & ((1 << ll) - 1));
+  r.kv = kvh >= a.c.hkv ? 1 : 0;
+  r.h = kvh - r.kv * a.c.hkv;
+  r.step = 1 << a.lt;
+  r.first = (blockIdx.x * a.passes * AHEAD << a.lt) + (row & (r.step - 1));
+  const int end = (blockIdx.x + 1) * a.passes * AHEAD << a.lt;
+  r.end = end < lq ? end : lq;
+  return kvh < 2 * a.c.hkv;
+}
+
+template <typename T, bool VEC> struct Row8 {
+  static constexpr int NV = 8 / Vec<T>::N;
+  Vec<T> v[NV];
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < 16; i += Vec<T>::N) {
-      const Vec<T> a = ldg_vec(p + i);
+      for (int i = 0; i < NV; ++i) v[i] = ldg_vec(p + i * Vec<T>::N);
+    } else {
 #pragma unroll
-      for (int j = 0; j < Vec<T>::N; ++j) v[i + j] = Elem<T>::ld(a.e[j]);
+      for (int i = 0; i < 8; ++i) v[i / Vec<T>::N].e[i % Vec<T>::N] = p[i];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = Elem<T>::ld(p[i]);
   }
-}
-
-// places a lane's block: false where the block is none of a live token's
-struct Place {
-  int kv, h, blk, page, at;
-  int64_t row;
+  __device__ __forceinline__ void store(T *p) const {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) stg_vec(p + i * Vec<T>::N, v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = v[i / Vec<T>::N].e[i % Vec<T>::N];
+    }
+  }
+  __device__ __forceinline__ T &operator[](int i) { return v[i / Vec<T>::N].e[i % Vec<T>::N]; }
 };
-__device__ __forceinline__ bool place_block(const RowArgs &a, int b, int lq, int lk, int t0, int idx, Place &p) {
-  const int bpr = a.c.head_dim / 16, bpt = 2 * a.c.hkv * bpr;
-  const int t = idx / bpt;
-  int rem = idx - t * bpt;
-  p.kv = rem / (a.c.hkv * bpr);
-  rem -= p.kv * a.c.hkv * bpr;
-  p.h = rem / bpr;
-  p.blk = rem - p.h * bpr;
-  const int i = t0 + t;
-  if (t >= a.tok_per_wg || i >= lq) return false;
-  p.row = (int64_t)a.c.start[b] + i;
-  if (p.row < 0 || p.row >= a.rows) return false;
-  const int pos = lk - lq + i;
-  p.page = page_of(a.c, b, pos);
-  p.at = pos & ((1 << a.c.shift) - 1);
-  return true;
-}
 
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void cache_append_kernel(RowArgs a) {
-  const int b = blockIdx.y, lq = a.c.len_q[b], lk = a.c.len_k[b], t0 = blockIdx.x * a.tok_per_wg;
-  if (t0 >= lq) return;
-  const float gs[2] = {global_scale_of(a.c.amax[0]), global_scale_of(a.c.amax[1])};
-  const int n = a.tok_per_wg * 2 * a.c.hkv * (a.c.head_dim / 16);
-  for (int idx = threadIdx.x; idx < n; idx += 256) {
-    Place p;
-    if (!place_block(a, b, lq, lk, t0, idx, p) || p.page < 0) continue;
-    const int kv = p.kv;
-    float v[16];
-    load16<T, VEC>(reinterpret_cast<const T *>(kv ? a.x[1] : a.x[0]) + p.row * (kv ? a.xt[1] : a.xt[0]) +
-                       p.h * (kv ? a.xh[1] : a.xh[0]) + 16 * p.blk, v);
-    float m = 0.f;
+  const Cache &c = a.c;
+  const int b = blockIdx.y, lq = c.len_q[b], lk = c.len_k[b];
+  RowLane r;
+  if (!row_lane<kAppendAhead>(a, lq, r)) return;
+  const int64_t start = c.start[b];
+  const int kv = r.kv;
+  const float g = global_scale_of(kv ? c.amax[1] : c.amax[0]), six = 6.0f * g, rsix = 1.0f / six;
+  const T *x = reinterpret_cast<const T *>(kv ? a.x[1] : a.x[0]) + r.h * (kv ? a.xh[1] : a.xh[0]) + r.col;
+  uint8_t *d = (kv ? c.data[1] : c.data[0]) + r.h * (kv ? c.d_head[1] : c.d_head[0]) + (r.col >> 1);
+  uint8_t *s = (kv ? c.scale[1] : c.scale[0]) + r.h * (kv ? c.s_head[1] : c.s_head[0]) + (r.col >> 4);
+  const int64_t xt = kv ? a.xt[1] : a.xt[0], dp = kv ? c.d_page[1] : c.d_page[0], dt = kv ? c.d_tok[1] : c.d_tok[0];
+  const int64_t sp = kv ? c.s_page[1] : c.s_page[0], st = kv ? c.s_tok[1] : c.s_tok[0];
+  for (int i0 = r.first; i0 < r.end; i0 += kAppendAhead * r.step) {
+    Row8<T, VEC> in[kAppendAhead];
+    int page[kAppendAhead];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) m = max_skip_nan(m, v[j]);
-    const float g = kv ? gs[1] : gs[0], six = 6.0f * g;
-    float s8 = div_rn(m, six, 1.0f / six);
-    s8 = s8 < kE4M3Max ? s8 : kE4M3Max;
-    int sb = __builtin_amdgcn_cvt_pk_fp8_f32(s8, s8, 0, false) & 0xff;
-    const float q = __builtin_amdgcn_cvt_f32_fp8(sb, 0) * g;
-    uint32_t w[2] = {0, 0};
-    if (q >= 1e-5f) {
-      const float r = 1.0f / q;
-      float c[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float t = fminf(div_rn(fabsf(v[j]), q, r), 6.0f);  // inf and NaN: 6
-        c[j] = v[j] >= 0.f ? t : -t;
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float *e = c + 8 * k;
-        w[k] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[k], e[0], e[1], 1.0f, 0);
-        w[k] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[k], e[2], e[3], 1.0f, 1);
-        w[k] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[k], e[4], e[5], 1.0f, 2);
-        w[k] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[k], e[6], e[7], 1.0f, 3);
-      }
-    } else {
-      sb = 0;
+    for (int u = 0; u < kAppendAhead; ++u) {
+      const int i = i0 + u * r.step;
+      const int64_t row = start + i;
+      const bool ok = i < r.end && row >= 0 && row < a.rows;
+      if (ok) in[u].load(x + row * xt);
+      page[u] = ok ? page_of(c, b, lk - lq + i) : -1;
     }
-    uint8_t *d = (kv ? a.c.data[1] : a.c.data[0]) + p.page * (kv ? a.c.d_page[1] : a.c.d_page[0]) +
-                 p.h * (kv ? a.c.d_head[1] : a.c.d_head[0]) + p.at * (kv ? a.c.d_tok[1] : a.c.d_tok[0]);
-    uint8_t *s = (kv ? a.c.scale[1] : a.c.scale[0]) + p.page * (kv ? a.c.s_page[1] : a.c.s_page[0]) +
-                 p.h * (kv ? a.c.s_head[1] : a.c.s_head[0]) + p.at * (kv ? a.c.s_tok[1] : a.c.s_tok[0]);
-    *reinterpret_cast<uint2 *>(d + 8 * p.blk) = make_uint2(w[0], w[1]);
-    s[p.blk] = (uint8_t)sb;
+#pragma unroll
+    for (int u = 0; u < kAppendAhead; ++u) {
+      if (page[u] < 0) continue;  // both lanes of a block alike
+      float v[8], m = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = Elem<T>::ld(in[u][j]);
+        m = max_skip_nan(m, v[j]);
+      }
+      m = fmaxf(m, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(m), 0xB1, 0xf, 0xf, true)));  // lane ^ 1
+      float s8 = div_rn(m, six, rsix);
+      s8 = s8 < kE4M3Max ? s8 : kE4M3Max;
+      int sb = __builtin_amdgcn_cvt_pk_fp8_f32(s8, s8, 0, false) & 0xff;
+      const float q = __builtin_amdgcn_cvt_f32_fp8(sb, 0) * g;
+      uint32_t w = 0;
+      if (q >= 1e-5f) {
+        const float rq = 1.0f / q;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float t = fminf(div_rn(fabsf(v[j]), q, rq), 6.0f);  // inf and NaN: 6
+          v[j] = v[j] >= 0.f ? t : -t;
+        }
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], 1.0f, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], 1.0f, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], 1.0f, 2);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], 1.0f, 3);
+      } else {
+        sb = 0;
+      }
+      const int64_t at = (lk - lq + i0 + u * r.step) & ((1 << c.shift) - 1);
+      *reinterpret_cast<uint32_t *>(d + page[u] * dp + at * dt) = w;
+      if (!(r.col & 8)) s[page[u] * sp + at * st] = (uint8_t)sb;
+    }
   }
 }
 
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void cache_read_kernel(RowArgs a) {
-  const int b = blockIdx.y, lq = a.c.len_q[b], lk = a.c.len_k[b], t0 = blockIdx.x * a.tok_per_wg;
-  if (t0 >= lq) return;
-  const float gs[2] = {global_scale_of(a.c.amax[0]), global_scale_of(a.c.amax[1])};
-  const int n = a.tok_per_wg * 2 * a.c.hkv * (a.c.head_dim / 16);
-  for (int idx = threadIdx.x; idx < n; idx += 256) {
-    Place p;
-    if (!place_block(a, b, lq, lk, t0, idx, p)) continue;
-    const int kv = p.kv;
-    uint2 w = make_uint2(0, 0);
-    int sb = 0;
-    if (p.page >= 0) {
-      w = *reinterpret_cast<const uint2 *>((kv ? a.c.data[1] : a.c.data[0]) + p.page * (kv ? a.c.d_page[1] : a.c.d_page[0]) +
-                                           p.h * (kv ? a.c.d_head[1] : a.c.d_head[0]) +
-                                           p.at * (kv ? a.c.d_tok[1] : a.c.d_tok[0]) + 8 * p.blk);
-      sb = ((kv ? a.c.scale[1] : a.c.scale[0]) + p.page * (kv ? a.c.s_page[1] : a.c.s_page[0]) +
-            p.h * (kv ? a.c.s_head[1] : a.c.s_head[0]) + p.at * (kv ? a.c.s_tok[1] : a.c.s_tok[0]))[p.blk];
+  const Cache &c = a.c;
+  const int b = blockIdx.y, lq = c.len_q[b], lk = c.len_k[b];
+  RowLane r;
+  if (!row_lane<kReadAhead>(a, lq, r)) return;
+  const int64_t start = c.start[b];
+  const int kv = r.kv;
+  const float g = global_scale_of(kv ? c.amax[1] : c.amax[0]);
+  T *x = reinterpret_cast<T *>(kv ? a.x[1] : a.x[0]) + r.h * (kv ? a.xh[1] : a.xh[0]) + r.col;
+  const uint8_t *d = (kv ? c.data[1] : c.data[0]) + r.h * (kv ? c.d_head[1] : c.d_head[0]) + (r.col >> 1);
+  const uint8_t *s = (kv ? c.scale[1] : c.scale[0]) + r.h * (kv ? c.s_head[1] : c.s_head[0]) + (r.col >> 4);
+  const int64_t xt = kv ? a.xt[1] : a.xt[0], dp = kv ? c.d_page[1] : c.d_page[0], dt = kv ? c.d_tok[1] : c.d_tok[0];
+  const int64_t sp = kv ? c.s_page[1] : c.s_page[0], st = kv ? c.s_tok[1] : c.s_tok[0];
+  uint32_t w[kReadAhead];
+  int sb[kReadAhead];
+#pragma unroll
+  for (int u = 0; u < kReadAhead; ++u) {
+    const int i = r.first + u * r.step, pos = lk - lq + i, page = i < r.end ? page_of(c, b, pos) : -1;
+    const int64_t at = pos & ((1 << c.shift) - 1);
+    w[u] = 0, sb[u] = 0;
+    if (page >= 0) {
+      w[u] = *reinterpret_cast<const uint32_t *>(d + page * dp + at * dt);
+      sb[u] = s[page * sp + at * st];
     }
-    const float q = __builtin_amdgcn_cvt_f32_fp8(sb, 0) * (kv ? gs[1] : gs[0]);
-    T *x = reinterpret_cast<T *>(kv ? a.x[1] : a.x[0]) + p.row * (kv ? a.xt[1] : a.xt[0]) + p.h * (kv ? a.xh[1] : a.xh[0]) +
-           16 * p.blk;
-    float v[16];
+  }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint32_t u = k ? w.y : w.x;
-      auto pair = [&](auto e, int i) { v[8 * k + 2 * i] = e[0] * q, v[8 * k + 2 * i + 1] = e[1] * q; };
-      pair(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 0), 0);
-      pair(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 1), 1);
-      pair(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 2), 2);
-      pair(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 3), 3);
-    }
-    if constexpr (VEC) {
-#pragma unroll
-      for (int i = 0; i < 16; i += Vec<T>::N) {
-        Vec<T> o;
-#pragma unroll
-        for (int j = 0; j < Vec<T>::N; ++j) o.e[j] = Elem<T>::st(v[i + j]);
-        stg_vec(x + i, o);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = Elem<T>::st(v[i]);
-    }
+  for (int u = 0; u < kReadAhead; ++u) {
+    const int i = r.first + u * r.step;
+    const int64_t row = start + i;
+    if (i >= r.end || row < 0 || row >= a.rows) continue;
+    const float q = __builtin_amdgcn_cvt_f32_fp8(sb[u], 0) * g;
+    Row8<T, VEC> o;
+    auto pair = [&](auto e, int j) { o[j] = Elem<T>::st(e[0] * q), o[j + 1] = Elem<T>::st(e[1] * q); };
+    pair(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], 1.0f, 0), 0);
+    pair(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], 1.0f, 1), 2);
+    pair(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], 1.0f, 2), 4);
+    pair(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], 1.0f, 3), 6);
+    o.store(x + row * xt);
   }
 }
 
@@ -878,17 +895,24 @@ int rows_call(bool append, const mtq_kv_cache *cache, void *k, void *v, const in
   if (!k || !v || !make_cache(cache, table, table_stride, table_cols, start, len_q, len_k, batch, a.c)) return MTQ_ERR_INVALID_ARG;
   a.x[0] = k, a.x[1] = v;
   a.xt[0] = strides[0], a.xh[0] = strides[1], a.xt[1] = strides[2], a.xh[1] = strides[3];
-  a.rows = rows, a.max_len = max_len;
-  const int bpt = 2 * a.c.hkv * (a.c.head_dim / 16);
-  a.tok_per_wg = bpt >= 512 ? 1 : 512 / bpt;  // two blocks a lane
-  if (a.tok_per_wg > max_len) a.tok_per_wg = max_len;
+  a.rows = rows;
+  // tokens of a head a pass of the workgroup takes: as many as there are, at most the pass's rows
+  const int rows_wg = 2048 / a.c.head_dim;
+  a.lt = 0;
+  while ((2 << a.lt) <= rows_wg && (1 << a.lt) < max_len) a.lt++;
   const int es = dtype == MTQ_F32 ? 4 : 2;
   bool vec = al16p(k) && al16p(v);
   for (int i = 0; i < 4; ++i) {
     if (strides[i] < 0) return MTQ_ERR_INVALID_ARG;
     vec = vec && (strides[i] * es) % 16 == 0;
   }
-  const dim3 g((unsigned)((max_len + a.tok_per_wg - 1) / a.tok_per_wg), (unsigned)batch);
+  const int toks = (append ? kAppendAhead : kReadAhead) << a.lt, heads = rows_wg >> a.lt;
+  const int64_t gz = (2 * (int64_t)a.c.hkv + heads - 1) / heads, all = ((int64_t)max_len + toks - 1) / toks * batch * gz;
+  const int64_t most = (int64_t)kAppendWgs * host_num_cus();
+  a.passes = append ? (int)((all + most - 1) / most) : 1;
+  const int64_t gx = ((int64_t)max_len + (int64_t)toks * a.passes - 1) / ((int64_t)toks * a.passes);
+  if (gz > 65535) return MTQ_ERR_INVALID_ARG;
+  const dim3 g((unsigned)gx, (unsigned)batch, (unsigned)gz);
   auto go = [&](auto t) {
     using T = decltype(t);
     if (append)
