@@ -645,7 +645,11 @@ template <typename T, int OP> int launch_skinny(SkinnyArgs a, hipStream_t stream
 // (mtq_awq_gemm.hip, awq_search_pp_kernel): operands come by LDS-DMA into two buffers of four
 // half-tiles, a K tile is four phases of a 64 x 32 quadrant each, every phase issues the DMA of one
 // half-tile two to five phases ahead and waits with a counted vmcnt, and waves 4-7 run one barrier
-// behind waves 0-3, so that one wave of a SIMD reads LDS while the other multiplies.
+// behind waves 0-3, so that one wave of a SIMD reads LDS while the other multiplies.  The K tiles of all
+// the workgroup's tiles of y are one stream: what is loaded ahead at a tile's end is the next tile's.
+// us for xq 8192 x 4096, W 14336 x 4096: 257 E2M1 (3.74 PFLOP/s; each further 4096 columns: 205, 4.7), 390
+// E4M3 (2.47); without the stores 226 and 353: they come from all CUs at once, 128 KiB a tile, and loads
+// are waited for in order behind them.
 // The exponent bytes are laid out by K tile first ([K tile][row][BK / 32], zero past the matrix; one
 // small pass per operand), so a tile's are two DMAs a wave into a ring of three; a lane's exponents of
 // both 128-column steps are one 16-bit read (bytes 2 g + s for its block 4 s + g).
@@ -687,19 +691,21 @@ template <bool F8> __device__ __forceinline__ f32x4 pp_mma(const i32x8 &w, const
            : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, 4, 0, ws, 0, xs);
 }
 
-// one lane's 8 values of a row of y
-template <typename T> __device__ __forceinline__ void pp_store8(T *y, const float (&v)[8], int64_t n, int N) {
-  if (n + 8 <= N) {  // one store (fp32: two), of any alignment (rows of an odd N)
-    T e[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) e[k] = Elem<T>::st(v[k]);
-    __builtin_memcpy(y + n, e, sizeof(e));
+// 16 bytes of a row of y
+template <typename T> __device__ __forceinline__ void pp_store(T *y, const T (&e)[16 / sizeof(T)], int64_t n, int N) {
+  constexpr int EC = 16 / sizeof(T);
+  if (n + EC <= N) {  // of any alignment (rows of an odd N)
+    __builtin_memcpy(y + n, e, 16);
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (n + k < N) y[n + k] = Elem<T>::st(v[k]);
+    for (int k = 0; k < EC; ++k)
+      if (n + k < N) y[n + k] = e[k];
   }
 }
+
+// W's row at LDS row r of 32 (two operands of 16): operand 1's rows come between operand 0's by fours, so that a
+// lane's results of both (rows 4 fq .. of each) are 8 columns of y in a piece
+__device__ __forceinline__ int pp_wrow(int r) { return (r & 12) << 1 | (r & 16) >> 2 | (r & 3); }
 
 template <typename T, bool F8>
 __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
@@ -709,13 +715,11 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
   constexpr int AU = 2, BU = F8 ? 1 : 2, SU = F8 ? 1 : 2;  // DMAs a wave: half-tiles, a tile's exponents
   constexpr int CNT = 2 * AU + 2 * BU + SU;
   constexpr int NS = F8 ? 1 : 2;                       // 128-column steps of a K tile
-  constexpr int OP = 64 + 4, OBUF = 8 * OP;            // epilogue: 8 rows x 64 columns of a wave, fp32
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF + 3 * SBUF + 8 * OBUF * 4];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF + 3 * SBUF + 8 * 2048];
   unsigned char *const sring = lds + 2 * BUF;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int grp = wave >> 2, wn = wave & 3, fr = lane & 15, fq = lane >> 4;
-  float *const ostage = reinterpret_cast<float *>(lds + 2 * BUF + 3 * SBUF) + wave * OBUF;
 
   const int xrow = F8 ? p.K : p.K / 2, wrow = p.K / 2;  // bytes of a row
   const int nt = (p.K + BK - 1) / BK;
@@ -741,28 +745,10 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
     }
     return false;
   };
-  unsigned a_off[2][AU], b_off[2][BU];
   __amdgpu_buffer_rsrc_t xr, wr, xsr, wsr;
   auto set_tile = [&]() {
     const int64_t m0 = (int64_t)tm * kPpTile, n0 = (int64_t)tn * kPpTile;
     const int rows_x = (int)(p.M - m0 < kPpTile ? p.M - m0 : kPpTile), rows_w = (int)(p.N - n0 < kPpTile ? p.N - n0 : kPpTile);
-    // xq half h, round u: LDS row rr = u * 64 + wave * 8 + lane / 8, chunk slot lane % 8; W half h: the
-    // same, or (64-byte rows) rr = wave * 16 + lane / 4, slot lane % 4.  Rows past the matrix re-read
-    // its last one (their results are not stored).
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int u = 0; u < AU; ++u) {
-        const int rr = u * 64 + wave * 8 + (lane >> 3), row = (rr >> 6) * 128 + h * 64 + (rr & 63);
-        a_off[h][u] = (unsigned)(row < rows_x ? row : rows_x - 1) * (unsigned)xrow + a_chunk * 16;
-      }
-#pragma unroll
-      for (int u = 0; u < BU; ++u) {
-        const int rr = F8 ? wave * 16 + (lane >> 2) : u * 64 + wave * 8 + (lane >> 3);
-        const int row = (rr >> 5) * 64 + h * 32 + (rr & 31);
-        b_off[h][u] = (unsigned)(row < rows_w ? row : rows_w - 1) * (unsigned)wrow + b_chunk * 16;
-      }
-    }
     xr = wave_rsrc(p.x + m0 * xrow, (uint32_t)rows_x * (uint32_t)xrow);
     wr = wave_rsrc(p.w + n0 * wrow, (uint32_t)rows_w * (uint32_t)wrow);
     // rows without exponents: any bytes (not read from LDS)
@@ -770,25 +756,30 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
     wsr = wave_rsrc(p.wsc + n0 * NB, (uint32_t)(nt - 1) * ws_step + SOP);
   };
 
-  auto load_a = [&](int h, int t) {
-    unsigned char *dst = lds + (t & 1) * BUF + h * AH + wave * 1024;
-    const int tt = t < nt ? t : nt - 1;  // past the end: harmless re-loads
+  // xq half h, round u: LDS row rr = u * 64 + wave * 8 + lane / 8, chunk slot lane % 8, is row u * 128 + h * 64 +
+  // rr % 64 of the tile; W half h: the same, or (64-byte rows) rr = wave * 16 + lane / 4, slot lane % 4, is row
+  // rr / 32 * 64 + h * 32 + pp_wrow(rr % 32).  Rows past the matrix are out of their buffer's range (the row is
+  // in the vector offset): they read as zeros and their results are not stored.
+  const int b_rr = F8 ? wave * 16 + (lane >> 2) : wave * 8 + (lane >> 3);
+  const unsigned a_off = (unsigned)(wave * 8 + (lane >> 3)) * (unsigned)xrow + a_chunk * 16;
+  const unsigned b_off = (unsigned)((b_rr >> 5) * 64 + pp_wrow(b_rr & 31)) * (unsigned)wrow + b_chunk * 16;
+  // K tile tt of set_tile's tile, into buffer `buf`
+  auto load_a = [&](int h, int tt, int buf) {
+    unsigned char *dst = lds + buf * BUF + h * AH + wave * 1024;
     const uint32_t soff = __builtin_amdgcn_readfirstlane((uint32_t)tt * 128);
-    const unsigned back = tt == nt - 1 ? a_tail : 0;
+    const unsigned off = a_off - (tt == nt - 1 ? a_tail : 0);
 #pragma unroll
-    for (int u = 0; u < AU; ++u) MX_DMA(xr, dst + u * 8192, 16, a_off[h][u] - back, soff);
+    for (int u = 0; u < AU; ++u) MX_DMA(xr, dst + u * 8192, 16, off + (unsigned)((u * 128 + h * 64) * xrow), soff);
   };
-  auto load_b = [&](int h, int t) {
-    unsigned char *dst = lds + (t & 1) * BUF + 2 * AH + h * BH + wave * 1024;
-    const int tt = t < nt ? t : nt - 1;
+  auto load_b = [&](int h, int tt, int buf) {
+    unsigned char *dst = lds + buf * BUF + 2 * AH + h * BH + wave * 1024;
     const uint32_t soff = __builtin_amdgcn_readfirstlane((uint32_t)tt * (BK / 2));
-    const unsigned back = tt == nt - 1 ? b_tail : 0;
+    const unsigned off = b_off - (tt == nt - 1 ? b_tail : 0);
 #pragma unroll
-    for (int u = 0; u < BU; ++u) MX_DMA(wr, dst + u * 8192, 16, b_off[h][u] - back, soff);
+    for (int u = 0; u < BU; ++u) MX_DMA(wr, dst + u * 8192, 16, off + (unsigned)((u * 128 + h * 32) * wrow), soff);
   };
-  auto load_s = [&](int t, int slot) {
+  auto load_s = [&](int tt, int slot) {
     unsigned char *dst = sring + slot * SBUF;
-    const int tt = t < nt ? t : nt - 1;
     const uint32_t sx = __builtin_amdgcn_readfirstlane((uint32_t)tt * xs_step), sw = __builtin_amdgcn_readfirstlane((uint32_t)tt * ws_step);
     if constexpr (F8) {  // 1 KiB each: waves 0-3 and 4-7
       if (wave < 4)
@@ -801,18 +792,8 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
     }
   };
   // stream order of the DMAs: per K tile t  B1(t+1) | A1(t+1) | B0(t+2) | S(t+2) A0(t+2); CNT are those
-  // issued after the half-tile that the next phase reads.  A tile of y starts with the DMAs that the
-  // phases before its first K tile would have issued.
-  auto start_tile = [&]() {
-    load_b(0, 0);
-    load_s(0, 0);
-    load_a(0, 0);
-    load_b(1, 0);
-    load_a(1, 0);
-    load_b(0, 1);
-    load_s(1, 1);
-    load_a(0, 1);
-  };
+  // issued after the half-tile that the next phase reads.  Past a tile's end comes the next tile of y: what is
+  // two K tiles ahead belongs to it from the second half of K tile nt - 2 on, where the offsets change.
 
   // ---- fragments.  E2M1 operand, step s: block 4 s + fq (E4M3 form: block fq of 4); E4M3 operand:
   // columns 16 fq .. and 64 + 16 fq ..
@@ -843,24 +824,34 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
   int id = blockIdx.x;
   if (!next_tile(id)) return;  // the whole workgroup, before any barrier
   set_tile();
-  start_tile();
+  // what the phases before the first K tile would have issued
+  load_b(0, 0, 0);
+  load_s(0, 0);
+  load_a(0, 0, 0);
+  load_b(1, 0, 0);
+  load_a(1, 0, 0);
+  load_b(0, 1, 1);
+  load_s(1, 1);
+  load_a(0, 1, 1);
+  wait_vm<CNT>();
+  __builtin_amdgcn_s_barrier();
+  int buf = 0, slot = 0;  // of the stream
   for (bool more = true; more;) {
+    const int64_t m0 = (int64_t)tm * kPpTile + grp * 128, n0 = (int64_t)tn * kPpTile + wn * 64;
     f32x4 acc[8][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    wait_vm<CNT>();
-    __builtin_amdgcn_s_barrier();
-    if (grp == 1) __builtin_amdgcn_s_barrier();  // one barrier behind
 
+    if (grp == 1) __builtin_amdgcn_s_barrier();  // one barrier behind
     i32x8 af[4][NS], b0f[2][NS], b1f[2][NS];
     int sa[4], sb0[2], sb1[2];
-    int slot = 0;
     for (int t = 0; t < nt; ++t) {
-      const unsigned char *cur = lds + (t & 1) * BUF;
+      const unsigned char *cur = lds + buf * BUF;
       const unsigned char *sx = sring + slot * SBUF, *sw = sx + SOP;
-      const int slot2 = slot == 0 ? 2 : slot - 1;  // (t + 2) % 3
+      const int slot2 = slot == 0 ? 2 : slot - 1;  // two ahead
+      const int t1 = t + 1 < nt ? t + 1 : 0, t2 = t + 2 < nt ? t + 2 : t + 2 - nt;
       // rows without exponents: 2^0, past K 2^-127
       const int unit = F8 && !p.xsc ? ((t == nt - 1 && (nt - 1) * BK + 32 * fq >= p.K) ? 0 : 127) : 0;
 #pragma unroll
@@ -880,7 +871,7 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
           for (int j = 0; j < 2; ++j) {
 #pragma unroll
             for (int s = 0; s < NS; ++s) b0f[j][s] = read_b(cur, j, s);
-            sb0[j] = read_s(sw, wn * 64 + 16 * j + fr);
+            sb0[j] = read_s(sw, wn * 64 + pp_wrow(16 * j + fr));
           }
         }
         if (q == 1) {
@@ -888,15 +879,22 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
           for (int j = 0; j < 2; ++j) {
 #pragma unroll
             for (int s = 0; s < NS; ++s) b1f[j][s] = read_b(cur, 2 + j, s);
-            sb1[j] = read_s(sw, wn * 64 + 16 * (2 + j) + fr);
+            sb1[j] = read_s(sw, wn * 64 + 32 + pp_wrow(16 * j + fr));
           }
         }
-        if (q == 0) load_b(1, t + 1);
-        if (q == 1) load_a(1, t + 1);
-        if (q == 2) load_b(0, t + 2);
+        if (q == 0) load_b(1, t1, buf ^ 1);
+        if (q == 1) load_a(1, t1, buf ^ 1);
+        if (q == 2) {
+          if (t == nt - 2) {  // (nt >= 2)
+            id += gridDim.x;
+            more = next_tile(id);
+            if (more) set_tile();  // else the last tile's own K tiles again, which nothing reads
+          }
+          load_b(0, t2, buf);
+        }
         if (q == 3) {
-          load_s(t + 2, slot2);
-          load_a(0, t + 2);
+          load_s(t2, slot2);
+          load_a(0, t2, buf);
         }
         wait_vm<CNT>();
         __builtin_amdgcn_s_barrier();
@@ -913,53 +911,53 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
         __builtin_amdgcn_s_barrier();
       }
       slot = slot == 2 ? 0 : slot + 1;
+      buf ^= 1;
     }
-    if (grp == 0) __builtin_amdgcn_s_barrier();  // balance the stagger: every wave is done with the buffers
-    wait_vm<0>();                                // this tile's re-loads past the end have landed ...
-    __builtin_amdgcn_s_barrier();                // ... every wave's: the next tile's DMAs may begin
-
-    const int64_t m0 = (int64_t)tm * kPpTile + grp * 128, n0 = (int64_t)tn * kPpTile + wn * 64;
-    id += gridDim.x;
-    more = next_tile(id);
-    if (more) {
-      set_tile();
-      start_tile();  // in flight under the epilogue
-    }
-
-    // ---- y of the wave's 128 x 64: a lane holds y[m][n .. n + 3], m = 16 i + fr, n = 16 j + 4 fq; through
-    // LDS, 8 rows at a time, so that 8 lanes store a row's 64 columns
-    const int orow = lane >> 3, ocol = 8 * (lane & 7);
-    const int64_t n = n0 + ocol;
-    float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (p.bias) {
+    // both halves of the workgroup store at a time: one behind the other, each would wait for the other's stores
+    // (282 against 269 us)
+    if (grp == 0) __builtin_amdgcn_s_barrier();
+    // ---- y of the wave's 128 x 64: a lane holds y[m][n .. n + 7], m = 16 i + er, n = 32 h + 8 eq.  Through LDS (2 KiB
+    // of the wave's own: 16 rows of 128 bytes, chunk c of row r at c ^ r % 8), so that 8 lanes store 128 bytes of
+    // a row (64 bytes of 16 rows at once, what the lanes hold: 1 to 5 us slower of 390)
+    int el = lane;
+    asm volatile("" : "+v"(el));  // (addresses made here, not kept over the K tiles)
+    const int er = el & 15, eq = el >> 4, sr = el >> 3, sc = el & 7;
+    unsigned char *const stage = lds + 2 * BUF + 3 * SBUF + wave * 2048;
+    float bias[2][8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int64_t nk = n + k < p.N ? n + k : p.N - 1;
-        bias[k] = p.bias_f32 ? reinterpret_cast<const float *>(p.bias)[nk] : Elem<T>::ld(reinterpret_cast<const T *>(p.bias)[nk]);
+    for (int k = 0; k < 16; ++k) {
+      const int64_t n = n0 + 32 * (k >> 3) + 8 * eq + (k & 7), nk = n < p.N ? n : p.N - 1;
+      bias[k >> 3][k & 7] = !p.bias ? 0.f : p.bias_f32 ? reinterpret_cast<const float *>(p.bias)[nk] : Elem<T>::ld(reinterpret_cast<const T *>(p.bias)[nk]);
+    }
+    constexpr int EC = 16 / sizeof(T), PASSES = 64 / (8 * EC);  // columns of a chunk; 128-byte pieces of a row
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t mf = m0 + 16 * i + er;
+      const float f = p.xf ? p.xf[(mf < p.M ? mf : p.M - 1) * p.xf_stride] : 1.f;
+#pragma unroll
+      for (int ps = 0; ps < PASSES; ++ps) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {  // the lane's two chunks of this piece
+          const int h = PASSES == 1 ? c : ps, k0 = PASSES == 1 ? 0 : 4 * c;
+          const int chunk = PASSES == 1 ? 4 * c + eq : 2 * eq + c;
+          T e[EC];
+#pragma unroll
+          for (int k = 0; k < EC; ++k) e[k] = Elem<T>::st(acc[i][2 * h + ((k0 + k) >> 2)][(k0 + k) & 3] * f + bias[h][k0 + k]);
+          __builtin_memcpy(stage + er * 128 + 16 * (chunk ^ (er & 7)), e, 16);
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          T e[EC];
+          __builtin_memcpy(e, stage + (8 * u + sr) * 128 + 16 * (sc ^ sr), 16);
+          const int64_t m = m0 + 16 * i + 8 * u + sr;
+          if (m < p.M) pp_store<T>(reinterpret_cast<T *>(p.y) + m * p.N, e, n0 + ps * 8 * EC + EC * sc, p.N);
+        }
+        __builtin_amdgcn_wave_barrier();
       }
-    }
-    float f0 = 1.f, f1 = 1.f;  // the factors of rows lane and 64 + lane
-    if (p.xf) {
-      const int64_t r0 = m0 + lane < p.M ? m0 + lane : p.M - 1, r1 = m0 + 64 + lane < p.M ? m0 + 64 + lane : p.M - 1;
-      f0 = p.xf[r0 * p.xf_stride], f1 = p.xf[r1 * p.xf_stride];
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if ((fr >> 3) == (i & 1)) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4 *>(ostage + (fr & 7) * OP + 16 * j + 4 * fq) = acc[i >> 1][j];
-      }
-      __builtin_amdgcn_wave_barrier();
-      const int64_t m = m0 + 8 * i + orow;
-      float v[8];
-      const f32x4 lo = *reinterpret_cast<const f32x4 *>(ostage + orow * OP + ocol), hi = *reinterpret_cast<const f32x4 *>(ostage + orow * OP + ocol + 4);
-      const float f = __shfl(i < 8 ? f0 : f1, (8 * i + orow) & 63, 64);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = (k < 4 ? lo[k] : hi[k - 4]) * f + bias[k];
-      if (m < p.M) pp_store8<T>(reinterpret_cast<T *>(p.y) + m * p.N, v, n, p.N);
-      __builtin_amdgcn_wave_barrier();
     }
   }
+  wait_vm<0>();                                // the re-loads past the last tile
 }
 
 // ---- y = xq . W^T in between ---------------------------------------------------------------------
@@ -1214,7 +1212,7 @@ LinearPlan linear_plan(int64_t M, int64_t N, int64_t K, int kind) {
   if (M <= kSkinnyRows || pad * (K / 32 + 8) >= (1ll << 31)) return p;
   const int64_t cus = host_num_cus();
   auto tiles = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-  if (M > 128 && tiles(256, 256) * 4 >= cus * 3) {
+  if (M > 128 && tiles(256, 256) * 4 >= cus * 3 && K > pp_bk(kind != MTQ_MXFP4)) {  // two K tiles at least
     p.form = LinearPlan::kPp;
     return p;
   }

@@ -204,7 +204,8 @@ def check_product(y, xq, w, ws, bias, k, e4m3):
 
 # rows that meet every form: streaming (1 .. 16), 64-row tiles, 128-row tiles, 256-row tiles; K and N that no tile divides
 SHAPES = [(1, 16, 32), (1, 4096, 4096), (7, 33, 544), (8, 1000, 96), (16, 257, 4128), (16, 17000, 224), (17, 40, 32), (33, 100, 2080),
-          (64, 300, 1696), (65, 129, 512), (200, 333, 160), (300, 8200, 416), (700, 6151, 288), (2100, 6500, 352)]
+          (64, 300, 1696), (65, 129, 512), (200, 333, 160), (300, 8200, 416), (700, 6151, 288), (2100, 6500, 352),
+          (2100, 6500, 96), (4300, 5001, 544)]
 
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8", "fp8", "fp8_token"])
