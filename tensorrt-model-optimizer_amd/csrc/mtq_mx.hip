@@ -1166,28 +1166,40 @@ __global__ __launch_bounds__(256) void mx_pad_scales_kernel(const uint8_t *__res
   *reinterpret_cast<uint32_t *>(o + row * stride + b) = w;
 }
 
-// exponents [rows][nb] -> [K tile][rows padded to 256][NB], 0 past the matrix
-template <int NB>
-__global__ __launch_bounds__(256) void mx_tile_scales_kernel(const uint8_t *__restrict__ s, int rows, int nb, int pad, int nt,
-                                                             uint8_t *__restrict__ o) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / nt;
-  const int t = (int)(i - row * nt);
+// exponents [rows][nb] -> [K tile][rows padded to 256][NB], 0 past the matrix; both operands' in one launch
+struct TileScales {
+  const uint8_t *s[2];
+  uint8_t *o[2];
+  int rows[2], pad[2], blocks0, nb, nt;  // blocks0: workgroups of the first
+};
+template <int NB> __global__ __launch_bounds__(256) void mx_tile_scales_kernel(TileScales a) {
+  const int op = (int)blockIdx.x >= a.blocks0 ? 1 : 0;
+  const int64_t i = (int64_t)(blockIdx.x - (op ? a.blocks0 : 0)) * 256 + threadIdx.x;
+  const int64_t row = i / a.nt;
+  const int t = (int)(i - row * a.nt), nb = a.nb, pad = op ? a.pad[1] : a.pad[0];
   if (row >= pad) return;
+  const uint8_t *s = (op ? a.s[1] : a.s[0]) + row * nb + t * NB;
+  const bool in = row < (op ? a.rows[1] : a.rows[0]);
   uint32_t w[NB / 4];
 #pragma unroll
   for (int k = 0; k < NB / 4; ++k) {
     w[k] = 0;
+    const int left = nb - t * NB - 4 * k;
+    if (in && nb % 4 == 0 && left > 0) {  // 4-byte aligned rows: a dword is inside or outside
+      w[k] = *reinterpret_cast<const uint32_t *>(s + 4 * k);
+    } else if (in) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      // E2M1: a lane's two blocks 4 s + g of a K tile next to each other
-      const int at = 4 * k + j, b = t * NB + (NB == 8 ? (at >> 1) + 4 * (at & 1) : at);
-      if (row < rows && b < nb) w[k] |= (uint32_t)s[row * nb + b] << (8 * j);
+      for (int j = 0; j < 4; ++j)
+        if (j < left) w[k] |= (uint32_t)s[4 * k + j] << (8 * j);
     }
   }
-  uint32_t *d = reinterpret_cast<uint32_t *>(o + ((int64_t)t * pad + row) * NB);
-#pragma unroll
-  for (int k = 0; k < NB / 4; ++k) d[k] = w[k];
+  uint32_t *d = reinterpret_cast<uint32_t *>((op ? a.o[1] : a.o[0]) + ((int64_t)t * pad + row) * NB);
+  if constexpr (NB == 8) {  // E2M1: a lane's two blocks g and 4 + g of a K tile next to each other
+    d[0] = __builtin_amdgcn_perm(w[1], w[0], 0x05010400);
+    d[1] = __builtin_amdgcn_perm(w[1], w[0], 0x07030602);
+  } else {
+    d[0] = w[0];
+  }
 }
 
 bool is_mx(int kind) { return kind == MTQ_MXFP4 || kind == MTQ_MXFP8; }
@@ -1265,10 +1277,14 @@ template <typename T, bool F8> int launch_mid(MidArgs a, const LinearPlan &p, hi
   mx_join_kernel<T><<<(unsigned)(((int64_t)a.M * ((a.N + 3) / 4) + 255) / 256), 256, 0, stream>>>(a);
   return host_check_launch();
 }
-template <bool F8> int launch_tile_scales(const uint8_t *s, int rows, int K, uint8_t *o, hipStream_t stream) {
+// xs may be null: W's only
+template <bool F8>
+int launch_tile_scales(const uint8_t *xs, int M, uint8_t *xo, const uint8_t *ws, int N, uint8_t *wo, int K, hipStream_t stream) {
   constexpr int BK = pp_bk(F8);
-  const int nt = (K + BK - 1) / BK, pad = (rows + 255) / 256 * 256;
-  mx_tile_scales_kernel<BK / 32><<<(unsigned)(((int64_t)pad * nt + 255) / 256), 256, 0, stream>>>(s, rows, K / 32, pad, nt, o);
+  TileScales a{{xs, ws}, {xo, wo}, {M, N}, {(M + 255) / 256 * 256, (N + 255) / 256 * 256}, 0, K / 32, (K + BK - 1) / BK};
+  auto blocks = [&](int pad) { return ((int64_t)pad * a.nt + 255) / 256; };
+  a.blocks0 = xs ? (int)blocks(a.pad[0]) : 0;
+  mx_tile_scales_kernel<BK / 32><<<(unsigned)(a.blocks0 + blocks(a.pad[1])), 256, 0, stream>>>(a);
   return host_check_launch();
 }
 template <typename T, bool F8> int launch_pp(PpArgs a, hipStream_t stream) {
@@ -1374,21 +1390,20 @@ int mtq_mx_linear(const void *x, int64_t x_stride, int x_dtype, const void *x_sc
     const int bk = pp_bk(f8), nb = (int)(K / 32), per = (int)((K + bk - 1) / bk * (bk / 32));
     const uint8_t *xt = a.xsc, *wt = w_scale;
     int st = MTQ_OK;
-    auto lay = [&](const uint8_t *&s, int64_t rows, size_t off) {
-      if (!s || st != MTQ_OK) return;
-      uint8_t *d = (uint8_t *)ws + off;
-      if (plan.form == LinearPlan::kPp) {
-        st = f8 ? launch_tile_scales<true>(s, (int)rows, a.K, d, stream) : launch_tile_scales<false>(s, (int)rows, a.K, d, stream);
-      } else if (K % bk) {
+    uint8_t *const xo = (uint8_t *)ws + o.xt, *const wo = (uint8_t *)ws + o.wt;
+    if (plan.form == LinearPlan::kPp) {
+      st = f8 ? launch_tile_scales<true>(xt, a.M, xo, wt, a.N, wo, a.K, stream) : launch_tile_scales<false>(xt, a.M, xo, wt, a.N, wo, a.K, stream);
+      xt = xt ? xo : nullptr, wt = wo;
+    } else if (K % bk) {  // else as they are (4-byte aligned: checked)
+      auto pad = [&](const uint8_t *&s, int64_t rows, uint8_t *d) {
+        if (!s || st != MTQ_OK) return;
         mx_pad_scales_kernel<<<(unsigned)((rows * (per / 4) + 255) / 256), 256, 0, stream>>>(s, rows, nb, per, d);
         st = host_check_launch();
-      } else {
-        return;  // as they are (4-byte aligned: checked)
-      }
-      s = d;
-    };
-    lay(xt, M, o.xt);
-    lay(wt, N, o.wt);
+        s = d;
+      };
+      pad(xt, M, xo);
+      pad(wt, N, wo);
+    }
     if (st != MTQ_OK) return st;
     auto go = [&](auto t) {
       using T = decltype(t);
