@@ -150,9 +150,12 @@ __device__ __forceinline__ float wave_max(float v) {
 // Bound by HBM: x, r, h and a byte of codes per element, each touched once.  A workgroup takes one
 // row and keeps it in registers (NV groups of 8 columns a lane) between the sum of squares and the
 // output, so nothing is read twice.
-// A code flips where y or a block's maximum lies within its own error of a rounding border, so that
-// error is kept near half a unit of fp32: squares are summed in fp32 by eights and those sums in
-// double, rsqrt is a pair of floats, and x * w of 16-bit operands is exact before the one product.
+// A code flips where y lies within its own error of a rounding border, a block's exponent where its maximum
+// does, so that error is kept small: squares are summed in fp32 by eights and those sums in double, rsqrt is a
+// pair of floats, and x * w of 16-bit operands is exact before the one product.  The MX formats, whose
+// factors are powers of two, take y rounded to odd where it matters (round_odd): rounding that again to a code, or
+// comparing it with a border, is then as good as y itself (a 16384 x 4096 call: 2 to 5 codes off by a step, 20 to
+// 40 without).
 struct NormArgs {
   const void *x, *r, *w;
   void *h;
@@ -164,10 +167,19 @@ struct NormArgs {
   int w_dtype;
 };
 
+// v = p * (rh + rl) rounded to nearest -> toward zero, the last bit set where something was cut
+__device__ __forceinline__ float round_odd(float v, float p, float rh, float rl) {
+  const float rest = __builtin_fmaf(p, rh, -v) + p * rl;
+  const uint32_t cut = rest < 0.f || rest > 0.f ? 1u : 0u;  // (an infinite v: rest is NaN)
+  const uint32_t up = (__float_as_uint(rest) ^ __float_as_uint(v)) >> 31;
+  return __uint_as_float((__float_as_uint(v) - (up & cut)) | cut);
+}
+
 template <typename T, int KIND, int NV, bool VEC>
 __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
   __shared__ double red[16];
   __shared__ float redm[16];
+  constexpr bool MX = KIND == MTQ_MXFP4 || KIND == MTQ_MXFP8;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
   const T *x = reinterpret_cast<const T *>(a.x) + row * a.xs;
@@ -213,10 +225,9 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float p = f[u][j] * w[j];
-      f[u][j] = __builtin_fmaf(p, rh, p * rl);
+      f[u][j] = MX ? p : __builtin_fmaf(p, rh, p * rl);
     }
   }
-  constexpr bool MX = KIND == MTQ_MXFP4 || KIND == MTQ_MXFP8;
   float s = 1.f;
   if constexpr (KIND == MTQ_FP8_TOKEN) {
     float m = 0.f;
@@ -244,7 +255,20 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
     if constexpr (MX) {
       // a block's 4 lanes are all live or all past the row (cols % 32 == 0)
       uint8_t *q = a.q + row * (KIND == MTQ_MXFP4 ? a.cols / 2 : a.cols);
-      mx_store8<KIND>(f[u], col, q, reinterpret_cast<uint8_t *>(a.scale) + row * (a.cols / 32), col < a.cols);
+      float v[8];
+      uint32_t low = ~0u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = __builtin_fmaf(f[u][j], rh, f[u][j] * rl);
+        const uint32_t b = __float_as_uint(v[j]) & 0x7ffff;
+        low = low < b ? low : b;
+      }
+      // halfway between codes, or a border, only where the bits below the 4th are zeros
+      if (__builtin_amdgcn_ballot_w64(low == 0)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = round_odd(v[j], f[u][j], rh, rl);
+      }
+      mx_store8<KIND>(v, col, q, reinterpret_cast<uint8_t *>(a.scale) + row * (a.cols / 32), col < a.cols);
     } else if (col < a.cols) {
       fp8_store8<VEC>(f[u], s, col, a.cols, a.q + row * a.cols);
     }
