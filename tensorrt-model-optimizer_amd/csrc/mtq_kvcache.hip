@@ -253,6 +253,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(RowArgs a) {
 // A wave takes 32 keys at a time, the waves of a workgroup every fourth 32 keys, and keep statistics
 // of their own, joined through LDS at the end (in wave order).  Where there are few sequences the
 // keys are cut into splits; their partial results are joined by a second small kernel, in order.
+// Bound by the cache's bytes: 64 single tokens over up to 16384 keys, 32 / 8 heads of 128: 163 us (717 MB, 4.4
+// TB/s; the loads alone take 134).
 struct AttnArgs {
   Cache c;
   const void *q;
@@ -592,8 +594,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 // are 16 KiB of fragments: 128 cycles of LDS beside 512 of one SIMD's matrix core, four SIMDs at once).  A
 // workgroup is 8 waves of 32 rows (v_mfma_f32_32x32x16_f16) on one KV head, two waves a SIMD; 64 keys at
 // a time are turned into fp16 by the whole workgroup, once per 256 rows, into one of three LDS stages.
-// (64 rows a wave, one wave a SIMD, half the LDS reads: 546 us against 409 for chunks of 500 to 1024
-// tokens behind contexts of up to 8192, 4 sequences, 32 / 8 heads: nothing of its one wave overlaps.)
+// Chunks of 500 to 1024 tokens behind contexts of up to 8192, 4 sequences, 32 / 8 heads of 128: 365 us (810
+// TFLOP/s).  64 rows a wave, one wave a SIMD, half the LDS reads took 546 where this layout took 409 (before
+// its page entries were loaded ahead): nothing of its one wave overlaps.
 // The loop over 32-key tiles is pipelined in registers: the step of tile j multiplies K of tile j + 1
 // and V of tile j - 1 while the softmax of tile j runs, three chains without a dependency between them.
 __device__ __forceinline__ float xmax32(float v) {  // v and its lane ^ 32 partner

@@ -153,9 +153,11 @@ __device__ __forceinline__ float wave_max(float v) {
 // A code flips where y lies within its own error of a rounding border, a block's exponent where its maximum
 // does, so that error is kept small: squares are summed in fp32 by eights and those sums in double, rsqrt is a
 // pair of floats, and x * w of 16-bit operands is exact before the one product.  The MX formats, whose
-// factors are powers of two, take y rounded to odd where it matters (round_odd): rounding that again to a code, or
-// comparing it with a border, is then as good as y itself (a 16384 x 4096 call: 2 to 5 codes off by a step, 20 to
-// 40 without).
+// factors are powers of two, take y rounded to odd where it matters (round_odd): rounding that again to a code,
+// or comparing it with a border, is then as good as y itself (16384 x 4096: 2 to 5 codes off by a step, 20 to
+// 40 without; 94 us with, 88 without).
+// us: 16 x 4096 with residual 4.5 (a launch); 16384 x 4096 with residual 92 (472 MB, 5.1 TB/s: the rate of a
+// large copy); 2501 x 5000 fp16 per token 15 (37 MB, 2.5 TB/s; a row is less than a workgroup can hide).
 struct NormArgs {
   const void *x, *r, *w;
   void *h;
@@ -348,7 +350,8 @@ __device__ __forceinline__ void mxfp4_store8_packed(const u32x4 &x, int64_t col,
 }
 
 // ---- quantising rows ---------------------------------------------------------------------------
-// MX and per-tensor FP8: 8 values a lane over all rows (a block's 4 lanes are neighbours).
+// MX and per-tensor FP8: 8 values a lane over all rows (a block's 4 lanes are neighbours).  Bound by HBM:
+// 8192 x 4096 bf16 to MXFP4 22 us (86 MB, 3.9 TB/s).
 template <typename T, int KIND, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ x, int64_t xs, int64_t rows, int64_t cols,
                                                           const float *__restrict__ amax, uint8_t *__restrict__ q,
@@ -511,6 +514,7 @@ template <typename T> __device__ __forceinline__ void block_codes(const u32x4 (&
 // (nothing of W is shared, so LDS would only add a trip), and the partial tiles meet in LDS at the end,
 // summed in wave order.  A wave takes 512 columns at a time: 4 NT loads of codes, one 16-byte load of
 // exponents a row, all in flight together; the other waves of the SIMD cover the rest.
+// 1 x 4096 x 4096, quantised on the way: 6.0 us (8.9 MB).
 struct SkinnyArgs {
   const void *x;             // xq, or the 16-bit activations (FUSED)
   const uint8_t *xsc;        // exponent bytes [M, K / 32] (MX formats)
@@ -990,6 +994,7 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
 // DMA STAGES - 1 ahead, one barrier a K tile (a stage is refilled after the barrier behind its last
 // read).  Where there are still fewer tiles than CUs, K is cut into splits whose fp32 tiles a second
 // small kernel adds in order.  Exponents: [rows][stride], stride a multiple of 4, zero past K.
+// 48 x 28672 x 8192 E4M3: 42 us (3.0 TB/s of W); 1531 x 6151 x 1696: 38 us.
 struct MidArgs {
   const uint8_t *x, *w, *xsc, *wsc;
   const float *xf;
