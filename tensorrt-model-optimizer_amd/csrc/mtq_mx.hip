@@ -994,7 +994,7 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
 // DMA STAGES - 1 ahead, one barrier a K tile (a stage is refilled after the barrier behind its last
 // read).  Where there are still fewer tiles than CUs, K is cut into splits whose fp32 tiles a second
 // small kernel adds in order.  Exponents: [rows][stride], stride a multiple of 4, zero past K.
-// 48 x 28672 x 8192 E4M3: 42 us (3.0 TB/s of W); 1531 x 6151 x 1696: 38 us.
+// 48 x 28672 x 8192 E4M3: 43 us (2.9 TB/s of W); 1531 x 6151 x 1696: 46 us.
 struct MidArgs {
   const uint8_t *x, *w, *xsc, *wsc;
   const float *xf;
