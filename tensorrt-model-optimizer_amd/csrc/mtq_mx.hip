@@ -88,17 +88,43 @@ __device__ __forceinline__ uint32_t e2m1_codes8(const float (&v)[8], float unsca
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, a[6], a[7], unscale, 3);
   return w;
 }
-// 8 values -> 8 E4M3 bytes of v * s, saturating, NaN kept
-__device__ __forceinline__ uint2 e4m3_codes8(const float (&v)[8], float s) {
-  float a[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) a[j] = clamp_nan(v[j] * s, -kE4M3Max, kE4M3Max);
+// 8 values of at most 448 (or NaN) -> their E4M3 bytes
+__device__ __forceinline__ uint2 e4m3_bytes8(const float (&a)[8]) {
   int lo = 0, hi = 0;
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(a[0], a[1], lo, false);
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(a[2], a[3], lo, true);
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(a[4], a[5], hi, false);
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(a[6], a[7], hi, true);
   return make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+// ... of v * s, saturating, NaN kept
+__device__ __forceinline__ uint2 e4m3_codes8(const float (&v)[8], float s) {
+  float a[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = clamp_nan(v[j] * s, -kE4M3Max, kE4M3Max);
+  return e4m3_bytes8(a);
+}
+// A row's own factor d = max|x| / 448 (1 where that is 0): codes of the quotient x / d, rounded once.  A product with
+// 1 / d would be rounded twice (codes flip at their borders), and 1 / d is past fp32 for d < 2^-128: rows of a
+// small d have both sides multiplied by 2^64 first, exactly.
+struct RowFactor {
+  float d, by, up, r, most;  // x / d = x up / by, r = 1 / by; |x up| is cut at `most`: infinities, a d rounded down
+};
+__device__ __forceinline__ RowFactor row_factor(float most) {
+  RowFactor f;
+  f.d = most / kE4M3Max;
+  f.d = f.d > 0.f ? f.d : 1.f;
+  f.up = f.d < 0x1p-64f ? 0x1p64f : 1.f;
+  f.by = f.d * f.up;
+  f.r = 1.0f / f.by;
+  f.most = clamp_flt_max(f.by * kE4M3Max);
+  return f;
+}
+__device__ __forceinline__ uint2 e4m3_codes8(const float (&v)[8], const RowFactor &f) {
+  float a[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = div_rn(clamp_nan(v[j] * f.up, -f.most, f.most), f.by, f.r);
+  return e4m3_bytes8(a);
 }
 
 // One block of 32 in 4 consecutive lanes of 8 values: codes to the row q, the exponent byte to sc[]
@@ -121,8 +147,7 @@ __device__ __forceinline__ void mx_store8(const float (&v)[8], int64_t col, uint
   }
 }
 template <bool VEC>
-__device__ __forceinline__ void fp8_store8(const float (&v)[8], float s, int64_t col, int64_t cols, uint8_t *q) {
-  const uint2 w = e4m3_codes8(v, s);
+__device__ __forceinline__ void fp8_store8(uint2 w, int64_t col, int64_t cols, uint8_t *q) {
   if constexpr (VEC) {
     *reinterpret_cast<uint2 *>(q + col) = w;
   } else {
@@ -231,6 +256,7 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
     }
   }
   float s = 1.f;
+  RowFactor rf{};
   if constexpr (KIND == MTQ_FP8_TOKEN) {
     float m = 0.f;
 #pragma unroll
@@ -242,10 +268,8 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
     __syncthreads();
     m = 0.f;
     for (int i = 0; i < nw; ++i) m = fmaxf(m, redm[i]);
-    float d = m / kE4M3Max;
-    d = d > 0.f ? d : 1.f;
-    if (tid == 0) reinterpret_cast<float *>(a.scale)[row] = d;
-    s = 1.0f / d;
+    rf = row_factor(m);
+    if (tid == 0) reinterpret_cast<float *>(a.scale)[row] = rf.d;
   } else if constexpr (KIND == MTQ_FP8_TENSOR) {
     const Fp8Q p = make_fp8q(*a.amax);
     s = p.s;
@@ -272,7 +296,7 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
       }
       mx_store8<KIND>(v, col, q, reinterpret_cast<uint8_t *>(a.scale) + row * (a.cols / 32), col < a.cols);
     } else if (col < a.cols) {
-      fp8_store8<VEC>(f[u], s, col, a.cols, a.q + row * a.cols);
+      fp8_store8<VEC>(KIND == MTQ_FP8_TOKEN ? e4m3_codes8(f[u], rf) : e4m3_codes8(f[u], s), col, a.cols, a.q + row * a.cols);
     }
   }
 }
@@ -371,7 +395,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ 
   if constexpr (KIND == MTQ_FP8_TENSOR) {
     const Fp8Q p = make_fp8q(*amax);
     if (i == 0) *reinterpret_cast<float *>(scale) = p.inv;
-    if (live) fp8_store8<VEC>(v, p.s, col, cols, q + row * cols);
+    if (live) fp8_store8<VEC>(e4m3_codes8(v, p.s), col, cols, q + row * cols);
   } else {
     mx_store8<KIND>(v, col, q + row * (KIND == MTQ_MXFP4 ? cols / 2 : cols),
                     reinterpret_cast<uint8_t *>(scale) + row * (cols / 32), live);
@@ -397,14 +421,12 @@ __global__ __launch_bounds__(256) void token_quantize_kernel(const T *__restrict
   if ((tid & 63) == 0) red[tid >> 6] = m;
   __syncthreads();
   m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  float d = m / kE4M3Max;
-  d = d > 0.f ? d : 1.f;
-  if (tid == 0) scale[row] = d;
-  const float s = 1.0f / d;
+  const RowFactor f = row_factor(m);
+  if (tid == 0) scale[row] = f.d;
   for (int64_t col = 8 * tid; col < cols; col += 2048) {
     float v[8];
     load8<T, VEC>(x, col, cols, v);
-    fp8_store8<VEC>(v, s, col, cols, q + row * cols);
+    fp8_store8<VEC>(e4m3_codes8(v, f), col, cols, q + row * cols);
   }
 }
 
