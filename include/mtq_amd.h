@@ -529,7 +529,8 @@ int mtq_kv_read(const mtq_kv_cache *cache, void *k, void *v, const int64_t *stri
 
 /* o = softmax(softmax_scale q k^T) v for the queries (rows b_start_loc[b] + i, i < b_seq_len[b], the
  * last positions of their sequence) over the cached keys; causal or not; keys without a page are not
- * seen, a row that sees no key is zero, rows of no sequence are not touched.  q, o: [rows][heads]
+ * seen, a row that sees no key is zero, rows of no sequence are not touched, nor are a sequence's rows
+ * from max_len_q on.  q, o: [rows][heads]
  * [head_dim] bf16 / f16 (element strides q token, q head, o token, o head, multiples of 8),
  * 16-byte aligned.  max_len_k sizes the split over the keys (any value is correct).  ws:
  * mtq_kv_attention_workspace_bytes bytes, 16-byte aligned, contents overwritten. */

@@ -262,12 +262,19 @@ struct AttnArgs {
   float *part;  // the splits' rows: o, m, l
   int64_t qt, qh, ot, oh, rows;
   int group, causal, splits, chunk, tiles, part_tiles, batch;  // tiles: of the kernel's rows, part_tiles: of 16
+  int max_q;  // new tokens of a sequence that the grid and `part` have room for
   float sm_log2;  // softmax_scale * log2(e)
 };
 
 // where a row of a split's results lies: [splits][batch][hkv][16-row tiles][16][D + 4]
 template <int D> __device__ __forceinline__ int64_t part_row(const AttnArgs &a, int split, int b, int kvh, int row) {
   return (((((int64_t)split * a.batch + b) * a.c.hkv + kvh) * a.part_tiles + (row >> 4)) * 16 + (row & 15)) * (D + 4);
+}
+
+// rows of a sequence of lq new tokens: those past max_q, should the device hold a longer length, are left out
+__device__ __forceinline__ int attn_rows(const AttnArgs &a, int lq) {
+  lq = lq < a.max_q ? lq : a.max_q;
+  return lq > 0 ? lq * a.group : 0;
 }
 
 // Weights are 2^(s qs - m) in one fused step, so that m, which is rounded, leaves the rounding of the largest
@@ -348,7 +355,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
   const int cap = c.table_cols << c.shift;
   const int off = lk - lq;  // a query token's place in its sequence
   lk = lk < cap ? lk : cap;
-  const int nrows = lq > 0 ? lq * a.group : 0;
+  const int nrows = attn_rows(a, lq);
   if (16 * tile >= nrows) return;
   const int last_tok = (16 * tile + 15 < nrows ? 16 * tile + 15 : nrows - 1) / a.group;
   int kv_end = a.causal ? off + last_tok + 1 : lk;
@@ -556,7 +563,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const int kvh = blockIdx.y, row = blockIdx.x, b = blockIdx.z, grp = threadIdx.x / LN, d4 = 4 * (threadIdx.x % LN);
   const int lq = c.len_q[b], off = c.len_k[b] - lq, cap = c.table_cols << c.shift;
   const int lk = c.len_k[b] < cap ? c.len_k[b] : cap;
-  if (row >= (lq > 0 ? lq * a.group : 0)) return;
+  if (row >= attn_rows(a, lq)) return;
   const int64_t orow = (int64_t)c.start[b] + row / a.group;
   if (orow < 0 || orow >= a.rows) return;
   int kv_end = a.causal ? off + row / a.group + 1 : lk;
@@ -627,7 +634,7 @@ __global__ __launch_bounds__(512, 2) void attn_prompt_kernel(AttnArgs a) {
   const int b = pair / c.hkv, kvh = pair - b * c.hkv;
   const int lq = c.len_q[b], off = c.len_k[b] - lq, cap = c.table_cols << c.shift;
   const int lk = c.len_k[b] < cap ? c.len_k[b] : cap;
-  const int nrows = lq > 0 ? lq * a.group : 0;
+  const int nrows = attn_rows(a, lq);
   if (256 * tile >= nrows) return;  // the whole workgroup
   const int last_tok = (256 * tile + 255 < nrows ? 256 * tile + 255 : nrows - 1) / a.group;
   int kv_end = a.causal ? off + last_tok + 1 : lk;
@@ -1010,6 +1017,7 @@ int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const in
   a.qt = strides[0], a.qh = strides[1], a.ot = strides[2], a.oh = strides[3], a.rows = rows;
   a.causal = is_causal ? 1 : 0;
   a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles, a.part_tiles = p.part_tiles, a.batch = batch;
+  a.max_q = max_len_q;
   a.sm_log2 = (float)(softmax_scale * 1.44269504088896);
   const dim3 g((unsigned)p.splits, (unsigned)(p.tiles * a.c.hkv), (unsigned)batch), gj((unsigned)(max_len_q * a.group), (unsigned)a.c.hkv, (unsigned)batch);
   auto go = [&](auto t, auto d) {

@@ -95,7 +95,7 @@ class NVFP4KVCache:
         (bf16 or fp16; ``num_q_heads`` a multiple of ``num_kv_heads``).
 
         Causal: a query sees the keys up to its own position.  A query that sees no key gives zeros; rows of
-        no sequence are not written, as ``attention()``.  ``max_kv_len`` (a bound of ``b_seq_len_k``, default what
+        no sequence are not written, as ``attention()``, nor a sequence's rows from ``max_input_len`` on.  ``max_kv_len`` (a bound of ``b_seq_len_k``, default what
         ``block_table`` can hold) sizes the split over the keys."""
         check_device("NVFP4KVCache.attention", q)
         refuse_grad("NVFP4KVCache.attention", q)

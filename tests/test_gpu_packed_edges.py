@@ -99,3 +99,65 @@ def test_mx_linear_fp8_token_rows_of_small_magnitude(gpu):
         y = ops().mx_linear(x, w, ws, format="fp8_token", out_dtype=torch.float32)
         assert torch.isfinite(y).all()
         check_product(y, values(data, scale, "fp8_token"), w, ws, None, k, True)
+
+
+# ---- lengths past the bounds that a call names ---------------------------------------------------------------
+
+
+def c_attention(b, q, o, max_q, max_k, guard=1 << 16):
+    """mtq_kv_attention through the C entry, its workspace followed by ``guard`` bytes that have to stay."""
+    import ctypes
+
+    from modelopt_amd import _ext
+    from test_packed_ops_host import I64, SZ, I, KvCache, F64, P
+
+    lib = ctypes.CDLL(_ext.kernel_cdll()._name)
+    lib.mtq_kv_attention.argtypes = [P, P, P, P, I64, I, P, I64, I, P, P, P, I, I, I, I, F64, I, P, SZ, P]
+    lib.mtq_kv_attention_workspace_bytes.argtypes = [I, I, I, I, I, I]
+    lib.mtq_kv_attention_workspace_bytes.restype = SZ
+    c = KvCache()
+    for i, (d, s, a) in enumerate(((b.cache.k_data, b.cache.k_scale, b.cache.k_amax), (b.cache.v_data, b.cache.v_scale, b.cache.v_amax))):
+        c.data[i], c.scale[i], c.amax[i] = d.data_ptr(), s.data_ptr(), a.data_ptr()
+        for j in range(3):
+            c.data_strides[i][j], c.scale_strides[i][j] = d.stride(j), s.stride(j)
+    c.num_pages, c.num_kv_heads, c.page_size, c.head_dim = *b.cache.k_data.shape[:3], b.d
+    st, ql, kl, table = b.meta()
+    need = lib.mtq_kv_attention_workspace_bytes(len(b.q_len), q.shape[1], b.hkv, b.d, max_q, max_k)
+    ws = torch.full((need + guard,), 0x5A, dtype=torch.uint8, device=q.device)
+    status = lib.mtq_kv_attention(ctypes.byref(c), q.data_ptr(), o.data_ptr(), (I64 * 4)(q.stride(0), q.stride(1), o.stride(0), o.stride(1)),
+                                  q.shape[0], q.shape[1], table.data_ptr(), table.stride(0), table.shape[1], st.data_ptr(), ql.data_ptr(),
+                                  kl.data_ptr(), len(b.q_len), max_q, max_k, 1, b.d ** -0.5, 2 if q.dtype == torch.bfloat16 else 1,
+                                  ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    return status, need, bool((ws[need:] == 0x5A).all())
+
+
+# new tokens, contexts, bound of the new tokens: prompts (256 rows a workgroup), single tokens
+@pytest.mark.parametrize("q_len,kv_len,bound", [([64, 20], [4000, 3000], 33), ([20, 64], [3000, 4000], 33), ([9, 1], [2000, 900], 3),
+                                                ([200, 1], [5000, 40], 1)])
+@pytest.mark.parametrize("d", [128, 256])
+def test_attention_of_sequences_longer_than_the_bound(gpu, q_len, kv_len, bound, d):
+    """A length on the device past max_input_len (a captured call keeps its bound): the first rows are computed, the
+    others left alone, nothing is written past the workspace or into another sequence's part of it."""
+    from test_gpu_kv_fp4 import Batch
+
+    b = Batch(gpu, q_len, kv_len, 16, 2, d, seed=1).fill()
+    q = b.queries(8)
+    qg = q.to(gpu)
+    st, ql, kl, table = b.meta()
+    full = b.cache.attention(qg, st, ql, kl, table, max(q_len), max(kv_len))
+    out = torch.full_like(qg, 9.0)
+    status, need, whole = c_attention(b, qg, out, bound, max(kv_len))
+    assert status == 0 and need > 0 and whole  # split over the keys
+    left = torch.ones(b.tokens, dtype=torch.bool)
+    for s, n in zip(b.start, b.q_len):
+        left[s:s + min(n, bound)] = False
+    assert (out[left.to(gpu)] == 9).all()
+    out[left.to(gpu)] = full[left.to(gpu)]
+    b.check(out, q)
+    # unsplit: every row has all keys in one piece
+    out = torch.full_like(qg, 9.0)
+    status, need, whole = c_attention(b, qg, out, bound, 1)
+    assert status == 0 and need == 0 and whole and (out[left.to(gpu)] == 9).all()
+    out[left.to(gpu)] = full[left.to(gpu)]
+    b.check(out, q)
