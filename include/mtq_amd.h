@@ -517,7 +517,8 @@ typedef struct {
  * [rows][heads][head_dim] tensors k and v (element strides: k token, k head, v token, v head), into
  * / out of the pages block_table[b * table_stride + position / page_size].  Positions without a page
  * (an entry outside 0 .. num_pages - 1, a position past the table) are dropped / read as zeros;
- * other rows are not touched.  A page that a call writes must belong to one sequence. */
+ * other rows are not touched, nor are a sequence's tokens from max_len on.  A page that a call writes must
+ * belong to one sequence. */
 int mtq_kv_append(const mtq_kv_cache *cache, const void *k, const void *v, const int64_t *strides,
                   int64_t rows, const int32_t *block_table, int64_t table_stride, int table_cols,
                   const int32_t *b_start_loc, const int32_t *b_seq_len, const int32_t *b_seq_len_k,

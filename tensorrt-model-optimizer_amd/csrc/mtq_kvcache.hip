@@ -80,6 +80,7 @@ struct RowArgs {
   int64_t xt[2], xh[2];   // element strides (token, head)
   int64_t rows;
   int lt, passes;
+  int max_len;  // tokens of a sequence from max_len on are left out, also where its last pass reaches them
 };
 // Tokens of a lane in flight at once, and whether it loops over more.  us for the prompts of 7 sequences, 131 MB
 // at 8 heads of 128: 1 / 2 / 4 tokens: append 51 / 46 / 44, read 50 / 45 / 39; looping, with at most 48
@@ -99,8 +100,9 @@ template <int AHEAD> __device__ __forceinline__ bool row_lane(const RowArgs &a, 
   r.h = kvh - r.kv * a.c.hkv;
   r.step = 1 << a.lt;
   r.first = (blockIdx.x * a.passes * AHEAD << a.lt) + (row & (r.step - 1));
-  const int end = (blockIdx.x + 1) * a.passes * AHEAD << a.lt;
-  r.end = end < lq ? end : lq;
+  const int64_t end = (int64_t)(blockIdx.x + 1) * a.passes * AHEAD << a.lt;
+  lq = lq < a.max_len ? lq : a.max_len;
+  r.end = end < lq ? (int)end : lq;
   return kvh < 2 * a.c.hkv;
 }
 
@@ -906,6 +908,9 @@ int rows_call(bool append, const mtq_kv_cache *cache, void *k, void *v, const in
   a.x[0] = k, a.x[1] = v;
   a.xt[0] = strides[0], a.xh[0] = strides[1], a.xt[1] = strides[2], a.xh[1] = strides[3];
   a.rows = rows;
+  if (max_len > rows) max_len = (int)rows;  // a sequence has no more new tokens than there are rows
+  if (max_len > 1 << 30) return MTQ_ERR_INVALID_ARG;
+  a.max_len = max_len;
   // tokens of a head a pass of the workgroup takes: as many as there are, at most the pass's rows
   const int rows_wg = 2048 / a.c.head_dim;
   a.lt = 0;
@@ -919,7 +924,8 @@ int rows_call(bool append, const mtq_kv_cache *cache, void *k, void *v, const in
   const int toks = (append ? kAppendAhead : kReadAhead) << a.lt, heads = rows_wg >> a.lt;
   const int64_t gz = (2 * (int64_t)a.c.hkv + heads - 1) / heads, all = ((int64_t)max_len + toks - 1) / toks * batch * gz;
   const int64_t most = (int64_t)kAppendWgs * host_num_cus();
-  a.passes = append ? (int)((all + most - 1) / most) : 1;
+  const int64_t passes = (all + most - 1) / most, enough = ((int64_t)max_len + toks - 1) / toks;
+  a.passes = append ? (int)(passes < enough ? passes : enough) : 1;
   const int64_t gx = ((int64_t)max_len + (int64_t)toks * a.passes - 1) / ((int64_t)toks * a.passes);
   if (gz > 65535) return MTQ_ERR_INVALID_ARG;
   const dim3 g((unsigned)gx, (unsigned)batch, (unsigned)gz);

@@ -28,7 +28,7 @@ class NVFP4KVCache:
     are the rows of a sequence's new tokens in the flat ``[tokens, heads, head_dim]`` tensors,
     ``b_seq_len_k`` its length in the cache with them (the new tokens are its last positions), and
     ``block_table`` (int32 ``[batch, pages per sequence]``) the page of every ``page_size`` positions;
-    ``max_input_len`` bounds ``b_seq_len``.  All of them stay on the device: no call synchronises, and each can
+    ``max_input_len`` bounds ``b_seq_len`` (tokens from it on are left out).  All of them stay on the device: no call synchronises, and each can
     be captured into a graph.  An entry outside ``[0, num_pages)`` stands for no page: rows for it are
     dropped, read as zeros and not seen by the attention.  A page that ``append`` writes must belong to one
     sequence; pages that are only read may be shared.
@@ -95,7 +95,7 @@ class NVFP4KVCache:
         (bf16 or fp16; ``num_q_heads`` a multiple of ``num_kv_heads``).
 
         Causal: a query sees the keys up to its own position.  A query that sees no key gives zeros; rows of
-        no sequence are not written, as ``attention()``, nor a sequence's rows from ``max_input_len`` on.  ``max_kv_len`` (a bound of ``b_seq_len_k``, default what
+        no sequence are not written, as ``attention()``.  ``max_kv_len`` (a bound of ``b_seq_len_k``, default what
         ``block_table`` can hold) sizes the split over the keys."""
         check_device("NVFP4KVCache.attention", q)
         refuse_grad("NVFP4KVCache.attention", q)

@@ -161,3 +161,33 @@ def test_attention_of_sequences_longer_than_the_bound(gpu, q_len, kv_len, bound,
     assert status == 0 and need == 0 and whole and (out[left.to(gpu)] == 9).all()
     out[left.to(gpu)] = full[left.to(gpu)]
     b.check(out, q)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_of_sequences_longer_than_the_bound(gpu, d):
+    """append and read take the first max_input_len tokens of a sequence; any bound above its length will do."""
+    from modelopt_amd import _ext
+    from test_gpu_kv_fp4 import Batch
+
+    for bound in (1, 3, 7, 33):
+        b = Batch(gpu, [40, 2], [60, 2], 16, 2, d, seed=bound)
+        k, v = (torch.randn(b.tokens, 2, d, generator=b.g).bfloat16().to(gpu) for _ in range(2))
+        st, ql, kl, table = b.meta()
+        b.cache.append(k, v, st, ql, kl, table, bound)
+        full = [torch.full_like(k, 7.0) for _ in range(2)]
+        _ext.ops().kv_read(b.cache._tensors(), *full, st, ql, kl, table, 40)
+        cut = [torch.full_like(k, 7.0) for _ in range(2)]
+        _ext.ops().kv_read(b.cache._tensors(), *cut, st, ql, kl, table, bound)
+        for whole, some in zip(full, cut):
+            for s, n in zip(b.start, b.q_len):
+                m = min(n, bound)
+                assert (whole[s:s + m] != 0).any() and torch.equal(some[s:s + m], whole[s:s + m])
+                assert (whole[s + m:s + n] == 0).all()  # not written by append
+                assert (some[s + m:s + n] == 7).all()  # not read
+        for most in (100, 1 << 20, 2 ** 31 - 1):
+            b.cache.append(k, v, st, ql, kl, table, most)
+            want = b.cache.read(st, ql, kl, table, 40, b.tokens)
+            got = b.cache.read(st, ql, kl, table, most, b.tokens)
+            for s, n in zip(b.start, b.q_len):
+                assert all(torch.equal(w[s:s + n], x[s:s + n]) for w, x in zip(want, got))
+                assert (got[0][s:s + n] != 0).any(-1).all()
