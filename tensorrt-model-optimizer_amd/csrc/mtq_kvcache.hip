@@ -947,6 +947,9 @@ struct Plan {
 // rows of a KV head from which the prompt kernel is taken
 constexpr int kPromptRows = 128;
 
+// the rows of a KV head that a call has room for (ints in the kernels)
+bool attn_rows_fit(int max_len_q, int group) { return (int64_t)max_len_q * group <= INT32_MAX - 256; }
+
 // Splits of the keys: enough workgroups to fill the card (decode: 6 a CU, a split at least 256 keys, two
 // 32-key steps a wave; prompts: one a CU, at least 512 keys).  Up to 512 keys stay in one piece, which needs no
 // join: 9.7 us against 10.9 for one sequence of 500 keys, 10.1 / 13.8 for 32 of them; at 1000, split is faster
@@ -990,7 +993,8 @@ int mtq_kv_read(const mtq_kv_cache *cache, void *k, void *v, const int64_t *stri
 }
 
 size_t mtq_kv_attention_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim, int max_len_q, int max_len_k) {
-  if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_len_q < 1 || head_dim < 1) return 0;
+  if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_len_q < 1 || max_len_k < 0 || head_dim < 1) return 0;
+  if (!attn_rows_fit(max_len_q, num_q_heads / num_kv_heads)) return 0;  // which mtq_kv_attention refuses
   const Plan p = attn_plan(batch, num_kv_heads, num_q_heads / num_kv_heads, head_dim, max_len_q, max_len_k);
   return p.splits > 1 ? (size_t)p.splits * batch * num_kv_heads * p.part_tiles * 16 * (head_dim + 4) * sizeof(float) : 0;
 }
@@ -1012,7 +1016,7 @@ int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const in
   const int64_t cap = (int64_t)table_cols * cache->page_size;
   if (max_len_k > cap) max_len_k = (int)cap;
   a.group = num_q_heads / a.c.hkv;
-  if ((int64_t)max_len_q * a.group > INT32_MAX - 16) return MTQ_ERR_INVALID_ARG;
+  if (!attn_rows_fit(max_len_q, a.group)) return MTQ_ERR_INVALID_ARG;
   const Plan p = attn_plan(batch, a.c.hkv, a.group, a.c.head_dim, max_len_q, max_len_k);
   const int64_t pg = ((int64_t)batch * a.c.hkv + 7) / 8 * 8 * p.tiles;  // the prompt kernel's grid
   if (p.prompt ? pg > INT32_MAX : (int64_t)p.tiles * a.c.hkv > 65535) return MTQ_ERR_INVALID_ARG;

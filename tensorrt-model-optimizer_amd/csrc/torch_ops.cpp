@@ -1363,6 +1363,7 @@ KvCall kv_call(const at::TensorList &t, const at::Tensor &start, const at::Tenso
     for (int j = 0; j < 3; ++j) k.c.data_strides[i][j] = d.stride(j), k.c.scale_strides[i][j] = s.stride(j);
   }
   TORCH_CHECK_VALUE(t[0].size(0) <= INT32_MAX && t[0].size(1) <= 65535 && t[0].size(2) <= 32768, what, ": cache too large");
+  TORCH_CHECK_VALUE(t[0].size(1) >= 1, what, ": the cache has no heads");
   k.c.num_pages = (int)t[0].size(0), k.c.num_kv_heads = (int)t[0].size(1), k.c.page_size = (int)t[0].size(2), k.c.head_dim = (int)D;
   const int64_t batch = len_q.numel();
   auto ints = [&](const at::Tensor &x, const char *name) {
@@ -1437,6 +1438,7 @@ void kv_attention(at::TensorList cache, const at::Tensor &q, at::Tensor o, const
   TORCH_CHECK_VALUE(max_len_q >= 0 && max_len_q <= INT32_MAX && max_len_k >= 0, what, ": max_input_len / max_kv_len");
   max_len_k = std::min<int64_t>(max_len_k, c.table.size(1) * c.c.page_size);
   TORCH_CHECK_VALUE(max_len_k <= INT32_MAX / 2, what, ": block_table too wide");
+  max_len_q = std::min<int64_t>(max_len_q, q.size(0));  // a sequence has no more new tokens than there are rows
   at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
   const int64_t st[4] = {q.stride(0), q.stride(1), o.stride(0), o.stride(1)};
   const size_t nb = mtq_kv_attention_workspace_bytes(c.batch, (int)q.size(1), c.c.num_kv_heads, c.c.head_dim, (int)max_len_q,

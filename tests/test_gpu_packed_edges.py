@@ -191,3 +191,23 @@ def test_rows_of_sequences_longer_than_the_bound(gpu, d):
             for s, n in zip(b.start, b.q_len):
                 assert all(torch.equal(w[s:s + n], x[s:s + n]) for w, x in zip(want, got))
                 assert (got[0][s:s + n] != 0).any(-1).all()
+
+
+def test_attention_under_a_loose_bound(gpu):
+    """A bound of the new tokens far above their number: the plan goes by the rows that there are."""
+    from test_gpu_kv_fp4 import Batch
+
+    for d, q_len in ((128, [1, 2]), (256, [3, 1]), (64, [50, 4])):
+        b = Batch(gpu, q_len, [700, 90], 16, 2, d).fill()
+        q = b.queries(8)
+        for bound in (4096, 1 << 24, 2 ** 31 - 1):
+            b.check(b.cache.attention(q.to(gpu), *b.meta(), bound, 700), q)
+
+
+def test_a_cache_without_heads_is_refused(gpu):
+    from modelopt_amd.torch.kernels.common.attention import NVFP4KVCache
+
+    c = NVFP4KVCache(2, 16, 0, 128, device=gpu)
+    i = torch.ones(1, dtype=torch.int32, device=gpu)
+    with pytest.raises(ValueError, match="no heads"):
+        c.attention(torch.randn(1, 4, 128, device=gpu).bfloat16(), 0 * i, i, i, i.view(1, 1), 1)
