@@ -954,8 +954,11 @@ bool attn_rows_fit(int max_len_q, int group) { return (int64_t)max_len_q * group
 // 32-key steps a wave; prompts: one a CU, at least 512 keys).  Up to 512 keys stay in one piece, which needs no
 // join: 9.7 us against 10.9 for one sequence of 500 keys, 10.1 / 13.8 for 32 of them; at 1000, split is faster
 // (10.8 / 12.8).
+// The workspace's size and the call's plan are this function's of the same arguments, max_len_k as the caller gave it
+// (the size is no monotone function of it: fewer keys can mean more splits).
 Plan attn_plan(int batch, int hkv, int group, int head_dim, int max_len_q, int max_len_k) {
   Plan p;
+  if (max_len_k > INT32_MAX / 2) max_len_k = INT32_MAX / 2;  // the most positions that a cache can have
   const int64_t rows = (int64_t)max_len_q * group;
   p.prompt = rows >= kPromptRows && head_dim <= 128;  // head_dim 256: its three stages do not fit LDS
   p.part_tiles = (int)((rows + 15) / 16);
@@ -1013,8 +1016,6 @@ int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const in
   for (int i = 0; i < 4; ++i)
     if (strides[i] < 0 || strides[i] % 8) return MTQ_ERR_INVALID_ARG;
   if (!al16p(q) || !al16p(o) || !(softmax_scale > 0.0 && softmax_scale < 3.4e38)) return MTQ_ERR_INVALID_ARG;
-  const int64_t cap = (int64_t)table_cols * cache->page_size;
-  if (max_len_k > cap) max_len_k = (int)cap;
   a.group = num_q_heads / a.c.hkv;
   if (!attn_rows_fit(max_len_q, a.group)) return MTQ_ERR_INVALID_ARG;
   const Plan p = attn_plan(batch, a.c.hkv, a.group, a.c.head_dim, max_len_q, max_len_k);

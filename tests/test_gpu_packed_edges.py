@@ -211,3 +211,16 @@ def test_a_cache_without_heads_is_refused(gpu):
     i = torch.ones(1, dtype=torch.int32, device=gpu)
     with pytest.raises(ValueError, match="no heads"):
         c.attention(torch.randn(1, 4, 128, device=gpu).bfloat16(), 0 * i, i, i, i.view(1, 1), 1)
+
+
+@pytest.mark.parametrize("batch,max_k", [(38, 1537), (38, 4096), (3, 2 ** 31 - 1), (2, 100000)])
+def test_attention_takes_the_workspace_that_it_asked_for(gpu, batch, max_k):
+    """max_len_k above what the table holds: any value is correct, with the workspace reported for it."""
+    from test_gpu_kv_fp4 import Batch
+
+    b = Batch(gpu, [1] * batch, [1536 - 7 * i for i in range(batch)], 16, 8, 128).fill()
+    q = b.queries(32)
+    out = torch.zeros_like(q, device=gpu)
+    status, need, whole = c_attention(b, q.to(gpu), out, 1, max_k)
+    assert status == 0 and need > 0 and whole
+    b.check(out, q)

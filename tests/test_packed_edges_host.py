@@ -28,3 +28,23 @@ print("answered")
 """
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
     assert run.returncode == 0 and "answered" in run.stdout, (run.returncode, run.stderr)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="a call that is not refused would launch")
+def test_attention_is_not_refused_the_workspace_that_it_asked_for():
+    """Bounds of the keys above the table's positions, for which fewer keys mean a larger workspace."""
+    from test_packed_ops_host import ARG, FAKE, I64, BF16, kv_cache
+
+    lib = _ext.kernel_cdll()
+    size, attend = lib.mtq_kv_attention_workspace_bytes, lib.mtq_kv_attention
+    P, I, F64, SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_double, ctypes.c_size_t
+    size.argtypes, size.restype = [I] * 6, SZ
+    attend.argtypes = [P, P, P, P, I64, I, P, I64, I, P, P, P, I, I, I, I, F64, I, P, SZ, P]
+    strides = (I64 * 4)(4096, 128, 4096, 128)
+    for batch in (1, 3, 38, 100):
+        for lq in (1, 64):
+            for lk in (0, 1, 600, 1500, 1537, 1600, 2500, 100000, 2 ** 31 - 1):
+                need = size(batch, 32, 8, 128, lq, lk)
+                status = attend(ctypes.byref(kv_cache(page_size=64)), FAKE, FAKE, strides, batch * lq, 32, FAKE, 24, 24, FAKE, FAKE, FAKE,
+                                batch, lq, lk, 1, 0.1, BF16, FAKE, need, None)
+                assert status != ARG, (batch, lq, lk, need)
