@@ -351,7 +351,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attn_decode_kernel(Attn
   __shared__ float ml[2][4][16];
   const Cache &c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), t = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x, kvh = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles, b = blockIdx.z;
+  const int tile = blockIdx.x / a.splits, split = blockIdx.x - tile * a.splits, kvh = blockIdx.y, b = blockIdx.z;
   const int lq = c.len_q[b];
   int lk = c.len_k[b];
   const int cap = c.table_cols << c.shift;
@@ -1020,7 +1020,8 @@ int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const in
   if (!attn_rows_fit(max_len_q, a.group)) return MTQ_ERR_INVALID_ARG;
   const Plan p = attn_plan(batch, a.c.hkv, a.group, a.c.head_dim, max_len_q, max_len_k);
   const int64_t pg = ((int64_t)batch * a.c.hkv + 7) / 8 * 8 * p.tiles;  // the prompt kernel's grid
-  if (p.prompt ? pg > INT32_MAX : (int64_t)p.tiles * a.c.hkv > 65535) return MTQ_ERR_INVALID_ARG;
+  // (a grid's dimension has fewer than 2^32 lanes)
+  if (p.prompt ? pg > UINT32_MAX / 512 : (int64_t)p.tiles * p.splits > UINT32_MAX / 256) return MTQ_ERR_INVALID_ARG;
   if (a.c.hkv > 65535) return MTQ_ERR_INVALID_ARG;
   const size_t need = mtq_kv_attention_workspace_bytes(batch, num_q_heads, a.c.hkv, a.c.head_dim, max_len_q, max_len_k);
   if (need && (!ws || ws_bytes < need || !al16p(ws))) return MTQ_ERR_INVALID_ARG;
@@ -1030,7 +1031,7 @@ int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const in
   a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles, a.part_tiles = p.part_tiles, a.batch = batch;
   a.max_q = max_len_q;
   a.sm_log2 = (float)(softmax_scale * 1.44269504088896);
-  const dim3 g((unsigned)p.splits, (unsigned)(p.tiles * a.c.hkv), (unsigned)batch), gj((unsigned)(max_len_q * a.group), (unsigned)a.c.hkv, (unsigned)batch);
+  const dim3 g((unsigned)(p.tiles * p.splits), (unsigned)a.c.hkv, (unsigned)batch), gj((unsigned)(max_len_q * a.group), (unsigned)a.c.hkv, (unsigned)batch);
   auto go = [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;

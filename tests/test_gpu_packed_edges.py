@@ -224,3 +224,25 @@ def test_attention_takes_the_workspace_that_it_asked_for(gpu, batch, max_k):
     status, need, whole = c_attention(b, q.to(gpu), out, 1, max_k)
     assert status == 0 and need > 0 and whole
     b.check(out, q)
+
+
+@pytest.mark.parametrize("group,q_len,kv_len", [(4, [300, 17], [300, 900]), (1, [513], [2000]), (5, [129, 1, 64], [400, 333, 64])])
+def test_attention_of_prompts_at_head_dim_256(gpu, group, q_len, kv_len):
+    from test_gpu_kv_fp4 import Batch
+
+    for causal in (True, False):
+        b = Batch(gpu, q_len, kv_len, 32, 2, 256).fill()
+        q = b.queries(2 * group)
+        b.check(b.cache.attention(q.to(gpu), *b.meta(), b.max_q, max(kv_len), is_causal=causal), q, causal)
+
+
+def test_attention_at_head_dim_256_has_no_bound_of_rows(gpu):
+    """40000 rows of q of 32 heads: more tiles of 16 rows than a grid's second dimension counts."""
+    from test_gpu_kv_fp4 import Batch
+
+    b = Batch(gpu, [40, 3], [90, 70], 16, 8, 256).fill()
+    q = b.queries(32)
+    wide = torch.zeros(40000, 32, 256, dtype=q.dtype, device=gpu)
+    wide[: b.tokens] = q.to(gpu)
+    out = b.cache.attention(wide, *b.meta(), 40000, 90)
+    b.check(out[: b.tokens], q)
