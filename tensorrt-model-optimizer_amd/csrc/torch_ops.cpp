@@ -1403,6 +1403,8 @@ void kv_append(at::TensorList cache, const at::Tensor &k, const at::Tensor &v, c
   check_status(mtq_kv_append(&c.c, k.data_ptr(), v.data_ptr(), st, k.size(0), c.table.data_ptr<int32_t>(), c.table.stride(0),
                              (int)c.table.size(1), c.start.data_ptr<int32_t>(), c.len_q.data_ptr<int32_t>(),
                              c.len_k.data_ptr<int32_t>(), c.batch, (int)max_len, dtype_code(k.scalar_type()), cur_stream(k)), what);
+  for (int i = 0; i < 4; ++i)  // the pages' contents are others now (views of them were perhaps saved)
+    if (!cache[i].is_inference()) cache[i].unsafeGetTensorImpl()->bump_version();
 }
 
 void kv_read(at::TensorList cache, at::Tensor k, at::Tensor v, const at::Tensor &start, const at::Tensor &len_q,
@@ -1516,7 +1518,7 @@ TORCH_LIBRARY(modelopt_amd, m) {
         "(Tensor, Tensor, Tensor)");
   m.def("mx_linear(Tensor x, Tensor? x_scale, Tensor weight, Tensor weight_scale, Tensor? bias, int kind, "
         "Tensor? amax=None, ScalarType? out_dtype=None) -> Tensor");
-  m.def("kv_append(Tensor[] cache, Tensor k, Tensor v, Tensor b_start_loc, Tensor b_seq_len, Tensor b_seq_len_k, "
+  m.def("kv_append(Tensor(a!)[] cache, Tensor k, Tensor v, Tensor b_start_loc, Tensor b_seq_len, Tensor b_seq_len_k, "
         "Tensor block_table, int max_input_len) -> ()");
   m.def("kv_read(Tensor[] cache, Tensor(a!) k, Tensor(b!) v, Tensor b_start_loc, Tensor b_seq_len, Tensor b_seq_len_k, "
         "Tensor block_table, int max_input_len) -> ()");

@@ -246,3 +246,20 @@ def test_attention_at_head_dim_256_has_no_bound_of_rows(gpu):
     wide[: b.tokens] = q.to(gpu)
     out = b.cache.attention(wide, *b.meta(), 40000, 90)
     b.check(out[: b.tokens], q)
+
+
+def test_append_moves_the_version_of_its_pages(gpu):
+    from test_gpu_kv_fp4 import Batch
+
+    b = Batch(gpu, [4], [9], 16, 2, 64)
+    c = b.cache
+    k = torch.randn(b.tokens, 2, 64, device=gpu).bfloat16()
+    pages = [c.k_data, c.k_scale, c.v_data, c.v_scale]
+    before = [t._version for t in pages] + [c.k_amax._version, k._version]
+    c.append(k, k, *b.meta(), 4)
+    assert [t._version for t in pages] == [v + 1 for v in before[:4]]
+    assert [c.k_amax._version, k._version] == before[4:]
+    with torch.inference_mode():  # pages without a version
+        d = Batch(gpu, [4], [9], 16, 2, 64)
+        d.cache.append(k, k, *d.meta(), 4)
+        assert torch.equal(d.cache.read(*d.meta(), 4, 5)[0][1:], c.read(*b.meta(), 4, 5)[0][1:])

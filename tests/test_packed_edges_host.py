@@ -48,3 +48,19 @@ def test_attention_is_not_refused_the_workspace_that_it_asked_for():
                 status = attend(ctypes.byref(kv_cache(page_size=64)), FAKE, FAKE, strides, batch * lq, 32, FAKE, 24, 24, FAKE, FAKE, FAKE,
                                 batch, lq, lk, 1, 0.1, BF16, FAKE, need, None)
                 assert status != ARG, (batch, lq, lk, need)
+
+
+def test_what_an_op_writes_is_declared():
+    """A graph pass may drop or move a call whose schema says that it changes nothing."""
+    _ext.require_ops()
+    ops = torch.ops.modelopt_amd
+    for name, written in (("kv_append", {"cache"}), ("kv_read", {"k", "v"}), ("kv_attention", {"o"})):
+        schema = getattr(ops, name).default._schema
+        assert schema.is_mutable, name
+        assert {a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write} == written, name
+    graph = torch.fx.Graph()
+    x = graph.placeholder("x")
+    graph.call_function(ops.kv_append.default, ([x] * 6, x, x, x, x, x, x, 1))
+    graph.output(x)
+    graph.eliminate_dead_code()
+    assert any(n.target is ops.kv_append.default for n in graph.nodes)
