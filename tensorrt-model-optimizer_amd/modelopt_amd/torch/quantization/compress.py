@@ -53,10 +53,20 @@ class CompressConfig(dict):
         return self.get("mx_gemm", False)
 
 
+def _runs_more_than_its_forward(module) -> bool:
+    """Whether a call of ``module`` does more than its class's forward: hooks of its own or of every module, a
+    forward put in its place."""
+    hooks = torch.nn.modules.module
+    return bool(
+        module._forward_hooks or module._forward_pre_hooks or hooks._global_forward_hooks or hooks._global_forward_pre_hooks
+        or "forward" in module.__dict__
+    )
+
+
 def _mx_gemm_format(module, input):
     """``(format, amax)`` when ``module``'s forward on ``input`` is ``mx_linear`` of its packed weight: an
     MXFP4 weight with the input's dtype, an input quantizer that only fake-quantises to a format
-    ``mx_linear`` takes, no gradient; else None."""
+    ``mx_linear`` takes, no gradient, nothing hooked to the quantizers' calls, which do not happen; else None."""
     weight = module._parameters.get("weight")
     if not isinstance(weight, QTensorWrapper) or weight.metadata["qtensor_class"] is not MXFP4QTensor:
         return None
@@ -66,6 +76,8 @@ def _mx_gemm_format(module, input):
         return None
     wq, iq = module._modules.get("weight_quantizer"), module._modules.get("input_quantizer")
     if type(wq) is not TensorQuantizer or type(iq) is not TensorQuantizer:
+        return None
+    if _runs_more_than_its_forward(wq) or _runs_more_than_its_forward(iq):
         return None
     if not wq.is_enabled or not wq._if_quant or wq._if_calib or not wq.is_mxfp(4) or wq.pre_quant_scale is not None:
         return None

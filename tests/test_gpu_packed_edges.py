@@ -263,3 +263,52 @@ def test_append_moves_the_version_of_its_pages(gpu):
         d = Batch(gpu, [4], [9], 16, 2, 64)
         d.cache.append(k, k, *d.meta(), 4)
         assert torch.equal(d.cache.read(*d.meta(), 4, 5)[0][1:], c.read(*b.meta(), 4, 5)[0][1:])
+
+
+# ---- a compressed linear with mx_gemm does what its dequantising forward does -----------------------------------
+
+
+def compressed(gpu, preset="MXFP4_DEFAULT_CFG", dtype=torch.bfloat16, bias=True):
+    import modelopt_amd.torch.quantization as mtq
+
+    torch.manual_seed(1)
+    m = torch.nn.Sequential(torch.nn.Linear(256, 384, bias=bias)).to(gpu).to(dtype)
+    data = torch.randn(37, 256, device=gpu).to(dtype)
+    mtq.quantize(m, getattr(mtq, preset), lambda mm: mm(data))
+    mtq.compress(m, {"mx_gemm": True})
+    return m[0], data
+
+
+@pytest.fixture
+def packed_calls(monkeypatch):
+    import importlib
+
+    C = importlib.import_module("modelopt_amd.torch.quantization.compress")  # the package's own name is the function
+    calls, real = [], C.mx_linear
+    monkeypatch.setattr(C, "mx_linear", lambda *a, **k: (calls.append(k["format"]), real(*a, **k))[1])
+    return calls
+
+
+@pytest.mark.parametrize("which", ["input_quantizer", "weight_quantizer"])
+def test_mx_gemm_runs_the_quantizers_hooks(gpu, packed_calls, which):
+    layer, data = compressed(gpu)
+    q = getattr(layer, which)
+    with torch.no_grad():
+        layer(data)
+        assert packed_calls == ["mxfp4"]
+        seen = []
+        for add in (q.register_forward_hook, q.register_forward_pre_hook, torch.nn.modules.module.register_module_forward_hook,
+                    torch.nn.modules.module.register_module_forward_pre_hook):
+            handle = add(lambda mod, *a: seen.append(mod) and None)
+            seen.clear()
+            layer(data)
+            assert q in seen
+            handle.remove()
+        assert packed_calls == ["mxfp4"]
+        forward = q.forward
+        q.forward = lambda x: (seen.append("own"), forward(x))[1]
+        layer(data)
+        assert seen[-1] == "own"
+        del q.forward
+        layer(data)
+        assert packed_calls == ["mxfp4"] * 2
