@@ -74,6 +74,8 @@ def _mx_gemm_format(module, input):
         return None
     if input.dtype not in (torch.bfloat16, torch.float16, torch.float32) or weight.device != input.device:
         return None
+    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") != input.dtype:
+        return None  # the linear's output would have the autocast dtype
     wq, iq = module._modules.get("weight_quantizer"), module._modules.get("input_quantizer")
     if type(wq) is not TensorQuantizer or type(iq) is not TensorQuantizer:
         return None

@@ -312,3 +312,22 @@ def test_mx_gemm_runs_the_quantizers_hooks(gpu, packed_calls, which):
         del q.forward
         layer(data)
         assert packed_calls == ["mxfp4"] * 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_mx_gemm_under_autocast(gpu, packed_calls, dtype):
+    """The output has the dtype that the dequantising forward gives it."""
+    layer, data = compressed(gpu, dtype=dtype)
+    for cast in (torch.bfloat16, torch.float16):
+        packed_calls.clear()
+        with torch.no_grad(), torch.autocast("cuda", cast):
+            y = layer(data)
+            layer._use_mx_gemm = False
+            want = layer(data)
+            layer._use_mx_gemm = True
+        assert y.dtype == want.dtype == cast
+        assert packed_calls == (["mxfp4"] if cast == dtype else [])
+        if cast != dtype:
+            assert torch.equal(y, want)
+        with torch.no_grad(), torch.autocast("cuda", cast, enabled=False):
+            assert layer(data).dtype == dtype and packed_calls[-1] == "mxfp4"
