@@ -14,12 +14,14 @@ quant (block 32), ``"fp8"`` of the per-tensor FP8 quant with a calibrated ``amax
 byte, the even column in the low half -- ``MXFP4QTensor``'s layout, so the ``weight`` / ``_scale`` of a
 compressed linear are ``mx_linear``'s ``weight`` / ``weight_scale`` as they are.
 
-Forward only: an input that needs a gradient is refused while gradients are recorded.
+Forward only: an input that needs a gradient is refused while gradients are recorded, one with a forward-mode
+tangent always.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from ...._ext import ops
 
@@ -35,9 +37,15 @@ def format_code(format: str) -> int:
     return kind
 
 
+def needs_grad(*tensors) -> bool:
+    """Whether a gradient is recorded for one of them, or one carries a forward-mode tangent."""
+    record = torch.is_grad_enabled()
+    return any(t is not None and (record and t.requires_grad or forward_ad.unpack_dual(t).tangent is not None) for t in tensors)
+
+
 def refuse_grad(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError(f"{name}: forward only; call it under torch.no_grad() or on detached tensors")
+    if needs_grad(*tensors):
+        raise NotImplementedError(f"{name}: forward only; call it under torch.no_grad() or on detached tensors without a tangent")
 
 
 def check_device(name: str, x: torch.Tensor) -> None:

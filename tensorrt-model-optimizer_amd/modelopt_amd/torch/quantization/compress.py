@@ -21,6 +21,7 @@ import torch
 import torch.nn as nn
 
 from ..kernels.quantization import mx_linear
+from ..kernels.quantization.mx import needs_grad
 from .conversion import set_quantizer_attributes_partial
 from .nn.modules.quant_linear import _QuantLinear
 from .nn.modules.tensor_quantizer import TensorQuantizer
@@ -90,7 +91,7 @@ def _mx_gemm_format(module, input):
     bias = module._parameters.get("bias")
     if bias is not None and bias.dtype not in (input.dtype, torch.float32):
         return None
-    if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
+    if needs_grad(input, bias):
         return None
     if not iq.is_enabled or not iq._if_quant or iq._if_calib or not iq._fake_quant:
         return None

@@ -331,3 +331,19 @@ def test_mx_gemm_under_autocast(gpu, packed_calls, dtype):
             assert torch.equal(y, want)
         with torch.no_grad(), torch.autocast("cuda", cast, enabled=False):
             assert layer(data).dtype == dtype and packed_calls[-1] == "mxfp4"
+
+
+def test_mx_gemm_keeps_forward_mode_tangents(gpu, packed_calls):
+    from torch.autograd import forward_ad
+
+    layer, data = compressed(gpu)
+    with torch.no_grad(), forward_ad.dual_level():
+        bias = torch.nn.Parameter(layer.bias.detach().clone())
+        layer(data)
+        assert packed_calls == ["mxfp4"]
+        tangent = torch.randn_like(bias)
+        del layer._parameters["bias"]
+        layer._parameters["bias"] = forward_ad.make_dual(bias.detach(), tangent)
+        y = forward_ad.unpack_dual(layer(data))
+        assert packed_calls == ["mxfp4"]
+        assert torch.equal(y.tangent, tangent.expand_as(y.primal))

@@ -64,3 +64,24 @@ def test_what_an_op_writes_is_declared():
     graph.output(x)
     graph.eliminate_dead_code()
     assert any(n.target is ops.kv_append.default for n in graph.nodes)
+
+
+def test_forward_mode_tangents_are_refused():
+    """An operator without a derivative would drop them without a word."""
+    from torch.autograd import forward_ad
+
+    from modelopt_amd.torch.kernels.quantization.mx import refuse_grad
+
+    x, w = torch.randn(4, 32), torch.zeros(4, dtype=torch.uint8)
+    refuse_grad("op", x, w, None)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        refuse_grad("op", x, w, None)
+        for no_grad in (False, True):
+            with torch.set_grad_enabled(not no_grad), pytest.raises(NotImplementedError, match="forward only"):
+                refuse_grad("op", w, d)
+        refuse_grad("op", forward_ad.unpack_dual(d).primal)
+    with pytest.raises(NotImplementedError, match="forward only"):
+        torch.func.jvp(lambda t: refuse_grad("op", t), (x,), (x,))
+    with pytest.raises(NotImplementedError, match="forward only"):
+        torch.func.grad(lambda t: refuse_grad("op", t) or t.sum())(x)
