@@ -1185,6 +1185,11 @@ void attention_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v
 // ---- microscaled rows and products ------------------------------------------------------------
 namespace {
 
+// The operators below also stand for their Meta kernels: the same checks and outputs, without a launch.
+c10::optional<c10::Device> hip_device(const at::Tensor &x) {
+  return x.is_meta() ? c10::nullopt : c10::optional<c10::Device>(x.device());
+}
+
 // x as [rows, cols] with a row stride and contiguous columns, copied only where it is no such view
 at::Tensor as_rows(const at::Tensor &x) {
   if (x.dim() == 2 && x.stride(1) == 1 && (x.size(0) < 2 || x.stride(0) >= x.size(1))) return x;
@@ -1201,7 +1206,7 @@ const float *amax_of(const c10::optional<at::Tensor> &amax, int kind, const at::
   TORCH_CHECK_VALUE(amax.has_value() && amax->defined(), what, ": the per-tensor FP8 format needs amax");
   TORCH_CHECK_VALUE(amax->numel() == 1 && amax->scalar_type() == at::kFloat && amax->device() == x.device(), what,
                     ": amax must be one fp32 value on the input's device");
-  return amax->data_ptr<float>();
+  return x.is_meta() ? nullptr : amax->data_ptr<float>();
 }
 
 // (codes, scales) of rows shaped like x
@@ -1218,7 +1223,7 @@ std::pair<at::Tensor, at::Tensor> row_outputs(const at::Tensor &x, int kind, con
 }
 
 void check_float_rows(const at::Tensor &x, const char *what) {
-  check_device(x, what);
+  if (!x.is_meta()) check_device(x, what);
   const int dt = dtype_code(x.scalar_type());
   TORCH_CHECK(dt == MTQ_BF16 || dt == MTQ_F16 || dt == MTQ_F32, what, ": bf16, fp16 or fp32 input expected, got ",
               x.scalar_type());
@@ -1231,10 +1236,10 @@ std::tuple<at::Tensor, at::Tensor> mx_quantize(const at::Tensor &x, int64_t kind
   const char *what = "mx_quantize";
   const int kind = row_kind(kind_, what);
   check_float_rows(x, what);
-  at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(hip_device(x));
   auto [q, s] = row_outputs(x, kind, what);
   const float *am = amax_of(amax, kind, x, what);
-  if (x.numel() == 0) return {q, s};
+  if (x.numel() == 0 || x.is_meta()) return {q, s};
   const at::Tensor v = as_rows(x);
   check_status(mtq_mx_quantize(v.data_ptr(), v.stride(0), v.size(0), v.size(1), dtype_code(v.scalar_type()), kind, am,
                                (uint8_t *)q.data_ptr(), s.data_ptr(), cur_stream(v)), what);
@@ -1259,11 +1264,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_quantize(const at::Tenso
     TORCH_CHECK_VALUE(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type() &&
                           residual->device() == x.device(),
                       what, ": residual must have the input's shape, dtype and device");
-  at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(hip_device(x));
   auto [q, s] = row_outputs(x, kind, what);
   const float *am = amax_of(amax, kind, x, what);
   at::Tensor h = has_r ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
-  if (x.numel() == 0) return {q, s, h};
+  if (x.numel() == 0 || x.is_meta()) return {q, s, h};
   const at::Tensor v = as_rows(x), w = weight.contiguous();
   const at::Tensor r = has_r ? as_rows(*residual) : at::Tensor();
   check_status(mtq_rms_norm_quantize(v.data_ptr(), v.stride(0), has_r ? r.data_ptr() : nullptr, has_r ? r.stride(0) : 0,
@@ -1279,7 +1284,7 @@ at::Tensor mx_linear(const at::Tensor &x, const c10::optional<at::Tensor> &x_sca
   const char *what = "mx_linear";
   const int kind = row_kind(kind_, what);
   const bool packed = x_scale.has_value() && x_scale->defined();
-  check_device(x, what);
+  if (!x.is_meta()) check_device(x, what);
   TORCH_CHECK_VALUE(w.dim() == 2 && w.scalar_type() == at::kByte && w.device() == x.device(), what,
                     ": weight must be [N, K / 2] packed E2M1 codes (uint8) on the input's device");
   const int64_t N = w.size(0), K = 2 * w.size(1);
@@ -1303,11 +1308,11 @@ at::Tensor mx_linear(const at::Tensor &x, const c10::optional<at::Tensor> &x_sca
                           x_scale->device() == x.device(),
                       what, ": x_scale does not fit the format");
     xs = x_scale->contiguous();
-    if ((uintptr_t)xs.data_ptr() % 4) xs = xs.clone();
+    if (!x.is_meta() && (uintptr_t)xs.data_ptr() % 4) xs = xs.clone();
   } else {
     check_float_rows(x, what);
   }
-  at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(hip_device(x));
   const float *am = packed ? nullptr : amax_of(amax, kind, x, what);
   at::Tensor b;
   if (bias.has_value() && bias->defined()) {
@@ -1319,7 +1324,7 @@ at::Tensor mx_linear(const at::Tensor &x, const c10::optional<at::Tensor> &x_sca
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = N;
   at::Tensor y = at::empty(shape, x.options().dtype(od));
-  if (M == 0) return y;
+  if (M == 0 || x.is_meta()) return y;
   auto dense16 = [](const at::Tensor &t) {  // contiguous and 16-byte aligned (a copy only where it is neither)
     at::Tensor c = t.contiguous();
     return (uintptr_t)c.data_ptr() % 16 ? c.clone() : c;
@@ -1588,6 +1593,15 @@ TORCH_LIBRARY_IMPL(modelopt_amd, CPU, m) {
 }
 
 TORCH_LIBRARY_IMPL(modelopt_amd, Meta, m) {
+  m.impl("mx_quantize", &mx_quantize);
+  m.impl("rms_norm_quantize", &rms_norm_quantize);
+  m.impl("mx_linear", &mx_linear);
+  m.impl("kv_append", [](at::TensorList, const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                         const at::Tensor &, const at::Tensor &, int64_t) {});
+  m.impl("kv_read", [](at::TensorList, at::Tensor, at::Tensor, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                       const at::Tensor &, int64_t) {});
+  m.impl("kv_attention", [](at::TensorList, const at::Tensor &, at::Tensor, const at::Tensor &, const at::Tensor &,
+                            const at::Tensor &, const at::Tensor &, int64_t, int64_t, bool, double) {});
   m.impl("qlinear_small_m", [](const at::Tensor &x, const at::Tensor &w, const c10::optional<at::Tensor> &,
                                const at::Tensor &, int64_t, int64_t, int64_t, bool, bool) {
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());

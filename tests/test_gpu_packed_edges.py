@@ -347,3 +347,31 @@ def test_mx_gemm_keeps_forward_mode_tangents(gpu, packed_calls):
         y = forward_ad.unpack_dual(layer(data))
         assert packed_calls == ["mxfp4"]
         assert torch.equal(y.tangent, tangent.expand_as(y.primal))
+
+
+def test_a_traced_step_writes_its_cache(gpu):
+    """norm -> k/v -> append -> attention, functionalised by a tracing compiler: the pages are written before they are read."""
+    from modelopt_amd.torch.kernels.quantization import mx_linear, rms_norm_quantize
+    from test_gpu_kv_fp4 import Batch
+    from test_gpu_mx_linear import packed_weight
+
+    wk = packed_weight(2 * 64, 256, 1, gpu)
+    wv = packed_weight(2 * 64, 256, 2, gpu)
+    wq = packed_weight(8 * 64, 256, 3, gpu)
+    norm = torch.ones(256, device=gpu).bfloat16()
+    runs = []
+    for trace in (False, True):
+        b = Batch(gpu, [3, 1], [20, 40], 16, 2, 64, seed=4).fill()
+
+        def step(x, meta):
+            q, s, _ = rms_norm_quantize(x, norm, format="mxfp8")
+            h, k, v = (mx_linear(q, *w, format="mxfp8", x_scale=s).view(x.shape[0], -1, 64) for w in (wq, wk, wv))
+            b.cache.append(k, v, *meta, 3)
+            return b.cache.attention(h, *meta, 3, 40)
+
+        x = torch.randn(b.tokens, 256, generator=torch.Generator().manual_seed(7)).bfloat16().to(gpu)
+        with torch.no_grad():
+            out = (torch.compile(step, backend="aot_eager", fullgraph=True) if trace else step)(x, b.meta())
+        live = torch.cat([torch.arange(s, s + n) for s, n in zip(b.start, b.q_len)]).to(gpu)
+        runs.append((out[live], b.cache.k_data.clone(), b.cache.v_scale.view(torch.uint8).clone()))
+    assert all(torch.equal(p, q) for p, q in zip(*runs))

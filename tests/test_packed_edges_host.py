@@ -85,3 +85,39 @@ def test_forward_mode_tangents_are_refused():
         torch.func.jvp(lambda t: refuse_grad("op", t), (x,), (x,))
     with pytest.raises(NotImplementedError, match="forward only"):
         torch.func.grad(lambda t: refuse_grad("op", t) or t.sum())(x)
+
+
+def test_shapes_without_a_device():
+    """The operators under FakeTensorMode: outputs' shapes and types, and the refusals that go by them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from modelopt_amd.torch.kernels.common.attention import NVFP4KVCache
+    from modelopt_amd.torch.kernels.quantization import mx_linear, mx_quantize, rms_norm_quantize
+
+    _ext.require_ops()
+    forms = {"mxfp4": (32, torch.uint8, (3, 5, 2), torch.uint8), "mxfp8": (64, torch.float8_e4m3fn, (3, 5, 2), torch.uint8),
+             "fp8": (64, torch.float8_e4m3fn, (1,), torch.float32), "fp8_token": (64, torch.float8_e4m3fn, (3, 5, 1), torch.float32)}
+    with FakeTensorMode():
+        def new(*shape, dtype=torch.bfloat16):
+            return torch.empty(*shape, dtype=dtype, device="cuda")
+
+        x, w, ws = new(3, 5, 64), new(48, 32, dtype=torch.uint8), new(48, 2, dtype=torch.uint8)
+        for fmt, (cols, qt, ss, st) in forms.items():
+            amax = new(1, dtype=torch.float32) if fmt == "fp8" else None
+            for q, s in (mx_quantize(x, fmt, amax), rms_norm_quantize(x, new(64), residual=x, format=fmt, amax=amax)[:2]):
+                assert (*q.shape,) == (3, 5, cols) and q.dtype == qt and (*s.shape,) == ss and s.dtype == st
+                y = mx_linear(q, w, ws, new(48), format=fmt, x_scale=s)
+                assert (*y.shape,) == (3, 5, 48) and y.dtype == torch.bfloat16 and y.device.type == "cuda"
+            assert mx_linear(x, w, ws, format=fmt, amax=amax, out_dtype=torch.float32).dtype == torch.float32
+        assert rms_norm_quantize(x, new(64))[2] is None and rms_norm_quantize(x, new(64), residual=x)[2].shape == x.shape
+        with pytest.raises(ValueError, match="multiple of 32"):
+            mx_quantize(x[..., :40])
+        with pytest.raises(ValueError, match="columns"):
+            mx_linear(x, w[:, :16], ws[:, :1])
+        cache = NVFP4KVCache(4, 16, 2, 64)
+        n, table = new(1, dtype=torch.int32), new(1, 4, dtype=torch.int32)
+        cache.append(new(7, 2, 64), new(7, 2, 64), n, n, n, table, 7)
+        k, v = cache.read(n, n, n, table, 7, 9, dtype=torch.float16)
+        assert (*k.shape,) == (*v.shape,) == (9, 2, 64) and k.dtype == torch.float16
+        o = cache.attention(new(7, 8, 64), n, n, n, table, 7)
+        assert (*o.shape,) == (7, 8, 64) and o.dtype == torch.bfloat16
