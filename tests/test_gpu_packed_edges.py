@@ -375,3 +375,34 @@ def test_a_traced_step_writes_its_cache(gpu):
         live = torch.cat([torch.arange(s, s + n) for s, n in zip(b.start, b.q_len)]).to(gpu)
         runs.append((out[live], b.cache.k_data.clone(), b.cache.v_scale.view(torch.uint8).clone()))
     assert all(torch.equal(p, q) for p, q in zip(*runs))
+
+
+# ---- the factors that the norm hands over ---------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("h", [64, 5000, 20000])
+def test_rms_norm_quantize_factors(gpu, dtype, h):
+    """FP8 per tensor: the factor of the calibrated amax, to the bit, and codes of y / factor; per token: max|y| / 448."""
+    t = DTYPES[dtype]
+    g = torch.Generator().manual_seed(h)
+    x = (torch.randn(6, h, generator=g) * torch.tensor([1.0, 1e-3, 30.0, 1.0, 0.0, 1.0])[:, None]).to(t)
+    w = (1 + 0.3 * torch.randn(h, generator=g)).to(t)
+    y = x.double() * torch.rsqrt((x.double() ** 2).mean(-1, keepdim=True) + 1e-5) * w.double()
+    data, scale, _ = ops().rms_norm_quantize(x.to(gpu), w.to(gpu), 1e-5, format="fp8_token")
+    assert scale.shape == (6, 1) and float(scale[4]) == 1  # a row of zeros
+    want = y.abs().amax(-1, keepdim=True) / 448
+    # y: the sum's, the root's and two products' roundings in 32 bits, the quotient's
+    assert ((scale.cpu().double() - want).abs()[want > 0] <= want[want > 0] * 2.0 ** -21).all()
+    top = y.abs().argmax(-1, keepdim=True)
+    assert (data.cpu().float().abs().gather(-1, top)[want > 0] == 448).all()  # a row's largest uses the whole range
+    for amax in (0.7, 3.3, 250.0, 1e-9):
+        a = torch.tensor([amax])
+        safe = a if amax > 2.0 ** -24 else torch.ones(1)
+        s = safe.reciprocal() * 448
+        data, scale, _ = ops().rms_norm_quantize(x.to(gpu), w.to(gpu), 1e-5, format="fp8", amax=a.to(gpu))
+        assert torch.equal(scale.cpu(), s.reciprocal())
+        lim = y.clamp(-448 / s.double(), 448 / s.double())
+        got = data.cpu().double()
+        # half a step of E4M3 and y's roundings, times s's
+        assert ((got - lim * s.double()).abs() <= (2.0 ** -4 * (lim * s.double()).abs() + 2.0 ** -10) * (1 + 2.0 ** -20)).all()
