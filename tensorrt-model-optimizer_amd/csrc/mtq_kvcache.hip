@@ -927,7 +927,7 @@ int rows_call(bool append, const mtq_kv_cache *cache, void *k, void *v, const in
   const int64_t passes = (all + most - 1) / most, enough = ((int64_t)max_len + toks - 1) / toks;
   a.passes = append ? (int)(passes < enough ? passes : enough) : 1;
   const int64_t gx = ((int64_t)max_len + (int64_t)toks * a.passes - 1) / ((int64_t)toks * a.passes);
-  if (gz > 65535) return MTQ_ERR_INVALID_ARG;
+  if (gz > 65535 || gx > UINT32_MAX / 256) return MTQ_ERR_INVALID_ARG;  // (a grid's dimension has fewer than 2^32 lanes)
   const dim3 g((unsigned)gx, (unsigned)batch, (unsigned)gz);
   auto go = [&](auto t) {
     using T = decltype(t);

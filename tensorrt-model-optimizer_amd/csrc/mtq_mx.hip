@@ -13,6 +13,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "mtq_amd.h"
 #include "mtq_device.hpp"
 
@@ -29,6 +31,20 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 inline bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+bool is_mx(int kind) { return kind == MTQ_MXFP4 || kind == MTQ_MXFP8; }
+
+// A grid's dimension holds fewer than 2^32 lanes and wraps silently beyond: `rows` rows of `lanes` lanes each
+// (rounded up by less than 1024 in all) go in as few launches as they need, launch(first row, rows of it).
+template <typename F> int in_launches(int64_t rows, int64_t lanes, F launch) {
+  const int64_t most = (UINT32_MAX - 1024) / lanes;
+  for (int64_t r = 0; r < rows; r += most) {
+    launch(r, rows - r < most ? rows - r : most);
+    const int st = host_check_launch();
+    if (st != MTQ_OK) return st;
+  }
+  return MTQ_OK;
+}
 
 // ---- 8 consecutive values --------------------------------------------------------------------
 // VEC: 16-byte aligned groups of 8 columns, none of them past the row; else element by element.
@@ -302,23 +318,30 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
 }
 
 template <typename T, int KIND, bool VEC>
-int launch_norm(const NormArgs &a, int64_t rows, hipStream_t stream) {
+int launch_norm(const NormArgs &all, int64_t rows, hipStream_t stream) {
   // 256 lanes of 8 columns a group, up to 4 groups in registers; wider rows take more lanes
-  const int64_t groups = (a.cols + 7) / 8;
+  const int64_t groups = (all.cols + 7) / 8;
   int threads = 256;
   while (threads < 1024 && groups > 4 * threads) threads *= 2;
   if (groups < 256) threads = (int)((groups + 63) / 64 * 64);
   const int nv = (int)((groups + threads - 1) / threads);
-  const unsigned g = (unsigned)rows;
-  if (nv <= 1)
-    rms_norm_kernel<T, KIND, 1, VEC><<<g, threads, 0, stream>>>(a);
-  else if (nv <= 2)
-    rms_norm_kernel<T, KIND, 2, VEC><<<g, threads, 0, stream>>>(a);
-  else if (nv <= 4)
-    rms_norm_kernel<T, KIND, 4, VEC><<<g, threads, 0, stream>>>(a);
-  else
-    rms_norm_kernel<T, KIND, 8, VEC><<<g, threads, 0, stream>>>(a);
-  return host_check_launch();
+  return in_launches(rows, threads, [&](int64_t r, int64_t n) {
+    NormArgs a = all;
+    a.x = reinterpret_cast<const T *>(all.x) + r * all.xs;
+    if (all.r) a.r = reinterpret_cast<const T *>(all.r) + r * all.rs, a.h = reinterpret_cast<T *>(all.h) + r * all.cols;
+    a.q = all.q + r * (KIND == MTQ_MXFP4 ? all.cols / 2 : all.cols);
+    if (KIND == MTQ_FP8_TOKEN) a.scale = reinterpret_cast<float *>(all.scale) + r;
+    if (KIND == MTQ_MXFP4 || KIND == MTQ_MXFP8) a.scale = reinterpret_cast<uint8_t *>(all.scale) + r * (all.cols / 32);
+    const unsigned g = (unsigned)n;
+    if (nv <= 1)
+      rms_norm_kernel<T, KIND, 1, VEC><<<g, threads, 0, stream>>>(a);
+    else if (nv <= 2)
+      rms_norm_kernel<T, KIND, 2, VEC><<<g, threads, 0, stream>>>(a);
+    else if (nv <= 4)
+      rms_norm_kernel<T, KIND, 4, VEC><<<g, threads, 0, stream>>>(a);
+    else
+      rms_norm_kernel<T, KIND, 8, VEC><<<g, threads, 0, stream>>>(a);
+  });
 }
 template <typename T, int KIND> int launch_norm_v(const NormArgs &a, bool vec, int64_t rows, hipStream_t stream) {
   return vec ? launch_norm<T, KIND, true>(a, rows, stream) : launch_norm<T, KIND, false>(a, rows, stream);
@@ -433,17 +456,21 @@ __global__ __launch_bounds__(256) void token_quantize_kernel(const T *__restrict
 template <typename T, bool VEC>
 int launch_quantize(const T *x, int64_t xs, int64_t rows, int64_t cols, int kind, const float *amax, uint8_t *q,
                     void *scale, hipStream_t stream) {
-  const int64_t n = rows * ((cols + 7) / 8);
-  const unsigned g = (unsigned)((n + 255) / 256);
-  switch (kind) {
-  case MTQ_MXFP4: mx_quantize_kernel<T, MTQ_MXFP4, VEC><<<g, 256, 0, stream>>>(x, xs, rows, cols, amax, q, scale); break;
-  case MTQ_MXFP8: mx_quantize_kernel<T, MTQ_MXFP8, VEC><<<g, 256, 0, stream>>>(x, xs, rows, cols, amax, q, scale); break;
-  case MTQ_FP8_TENSOR:
-    mx_quantize_kernel<T, MTQ_FP8_TENSOR, VEC><<<g, 256, 0, stream>>>(x, xs, rows, cols, amax, q, scale);
-    break;
-  default: token_quantize_kernel<T, VEC><<<(unsigned)rows, 256, 0, stream>>>(x, xs, cols, q, (float *)scale); break;
-  }
-  return host_check_launch();
+  const int64_t gpr = (cols + 7) / 8;
+  return in_launches(rows, kind == MTQ_FP8_TOKEN ? 256 : gpr, [&](int64_t r, int64_t n) {
+    const T *const xr = x + r * xs;
+    uint8_t *const qr = q + r * (kind == MTQ_MXFP4 ? cols / 2 : cols);
+    void *const sr = is_mx(kind) ? (uint8_t *)scale + r * (cols / 32) : scale;
+    const unsigned g = (unsigned)((n * gpr + 255) / 256);
+    switch (kind) {
+    case MTQ_MXFP4: mx_quantize_kernel<T, MTQ_MXFP4, VEC><<<g, 256, 0, stream>>>(xr, xs, n, cols, amax, qr, sr); break;
+    case MTQ_MXFP8: mx_quantize_kernel<T, MTQ_MXFP8, VEC><<<g, 256, 0, stream>>>(xr, xs, n, cols, amax, qr, sr); break;
+    case MTQ_FP8_TENSOR:
+      mx_quantize_kernel<T, MTQ_FP8_TENSOR, VEC><<<g, 256, 0, stream>>>(xr, xs, n, cols, amax, qr, sr);
+      break;
+    default: token_quantize_kernel<T, VEC><<<(unsigned)n, 256, 0, stream>>>(xr, xs, cols, qr, (float *)scale + r); break;
+    }
+  });
 }
 
 // 4 consecutive columns of a row of y: v * f + bias, rounded once
@@ -671,20 +698,29 @@ __global__ __launch_bounds__(64 * WAVES, NT == 4 ? 2 : 4) void mx_skinny_kernel(
   }
 }
 
-template <typename T, int OP> int launch_skinny(SkinnyArgs a, hipStream_t stream) {
+template <typename T, int OP> int launch_skinny(const SkinnyArgs &all, hipStream_t stream) {
   // tiles of W that share a read of xq: four where that leaves a workgroup for nearly every CU (16 rows of
   // E4M3 against 28672 x 8192: 33 us, two 40, one 49), one where there are too few of them
-  const int64_t gm = (a.M + 15) / 16, cus = host_num_cus();
+  const int64_t gm = (all.M + 15) / 16, cus = host_num_cus();
+  auto go = [&](auto nt, auto waves) {
+    constexpr int NT = decltype(nt)::value, WAVES = decltype(waves)::value;
+    const int tiles_n = (all.N + 16 * NT - 1) / (16 * NT);
+    return in_launches(gm, (int64_t)tiles_n * 64 * WAVES, [&](int64_t t, int64_t n) {
+      SkinnyArgs a = all;
+      const int64_t m = 16 * t;
+      a.x = reinterpret_cast<const uint8_t *>(all.x) + m * (OP == kOpFused ? all.xs * 2 : OP == kOpFp4 ? all.K / 2 : all.K);
+      if (all.xsc) a.xsc = all.xsc + m * (all.K / 32);
+      if (all.xf) a.xf = all.xf + m * all.xf_stride;
+      a.y = reinterpret_cast<T *>(all.y) + m * all.N;
+      a.M = (int)(all.M - m < 16 * n ? all.M - m : 16 * n);
+      a.tiles_n = tiles_n;
+      mx_skinny_kernel<T, OP, NT, WAVES><<<(unsigned)(n * tiles_n), 64 * WAVES, 0, stream>>>(a);
+    });
+  };
   if constexpr (OP != kOpFused) {
-    if (a.N >= 48 * cus) {
-      a.tiles_n = (a.N + 63) / 64;
-      mx_skinny_kernel<T, OP, 4, 4><<<(unsigned)(gm * a.tiles_n), 64 * 4, 0, stream>>>(a);
-      return host_check_launch();
-    }
+    if (all.N >= 48 * cus) return go(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
   }
-  a.tiles_n = (a.N + 15) / 16;
-  mx_skinny_kernel<T, OP, 1, 8><<<(unsigned)(gm * a.tiles_n), 64 * 8, 0, stream>>>(a);
-  return host_check_launch();
+  return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
 }
 
 // ---- y = xq . W^T for many rows ------------------------------------------------------------------
@@ -1253,8 +1289,6 @@ template <int NB> __global__ __launch_bounds__(256) void mx_tile_scales_kernel(T
   }
 }
 
-bool is_mx(int kind) { return kind == MTQ_MXFP4 || kind == MTQ_MXFP8; }
-
 // rows up to which the weight-streaming kernel is taken
 constexpr int kSkinnyRows = 16;  // one 16-row operand
 // MXFP4 rows of at most 8 tokens against at most 16 MiB of W: quantised by every workgroup for itself, in
@@ -1360,7 +1394,7 @@ int mtq_mx_quantize(const void *x, int64_t row_stride, int64_t rows, int64_t col
   if (rows < 0 || cols < 1 || (is_mx(kind) && cols % 32) || (rows > 1 && row_stride < cols)) return MTQ_ERR_INVALID_ARG;
   if (rows == 0) return MTQ_OK;
   if (!x || !q || !scale || (kind == MTQ_FP8_TENSOR && !amax)) return MTQ_ERR_INVALID_ARG;
-  if (rows > (int64_t)INT32_MAX || rows * ((cols + 7) / 8) > (int64_t)INT32_MAX * 256) return MTQ_ERR_INVALID_ARG;
+  if (rows > (int64_t)INT32_MAX || (cols + 7) / 8 > (int64_t)INT32_MAX) return MTQ_ERR_INVALID_ARG;
   if ((uintptr_t)q % 8) return MTQ_ERR_INVALID_ARG;
   const int es = dtype == MTQ_F32 ? 4 : 2;
   const bool vec = al16(x) && cols % 8 == 0 && (rows == 1 || (row_stride * es) % 16 == 0);

@@ -406,3 +406,70 @@ def test_rms_norm_quantize_factors(gpu, dtype, h):
         got = data.cpu().double()
         # half a step of E4M3 and y's roundings, times s's
         assert ((got - lim * s.double()).abs() <= (2.0 ** -4 * (lim * s.double()).abs() + 2.0 ** -10) * (1 + 2.0 ** -20)).all()
+
+
+# ---- sizes past a launch's 2^32 lanes ---------------------------------------------------------------------------
+
+
+def test_fp8_token_of_more_rows_than_a_launch_takes(gpu):
+    rows = (1 << 24) + 5  # a workgroup of 256 lanes a row
+    x = torch.zeros(rows, 8, dtype=torch.bfloat16, device=gpu)
+    part = torch.randn(9, 8, generator=torch.Generator().manual_seed(0)).bfloat16()
+    x[:4], x[-5:] = part[:4].to(gpu), part[4:].to(gpu)
+    data, scale = ops().mx_quantize(x, "fp8_token")
+    want, factor = token_codes(part)
+    assert torch.equal(torch.cat((data[:4], data[-5:])).cpu().float(), want)
+    assert torch.equal(torch.cat((scale[:4], scale[-5:])).cpu(), factor) and bool((scale[4:-5] == 1).all())
+
+
+def test_rms_norm_of_more_rows_than_a_launch_takes(gpu):
+    rows = (1 << 26) + 5  # a wave a row
+    part = torch.randn(9, 8, generator=torch.Generator().manual_seed(0)).bfloat16().to(gpu)
+    x = torch.zeros(rows, 8, dtype=torch.bfloat16, device=gpu)
+    x[:4], x[-5:] = part[:4], part[4:]
+    r = torch.zeros_like(x)
+    w = torch.linspace(0.5, 2, 8, device=gpu).bfloat16()
+    for fmt in ("fp8_token", "fp8"):
+        amax = torch.ones(1, device=gpu) if fmt == "fp8" else None
+        want = ops().rms_norm_quantize(part, w, 1e-5, residual=torch.zeros_like(part), format=fmt, amax=amax)
+        got = ops().rms_norm_quantize(x, w, 1e-5, residual=r, format=fmt, amax=amax)
+        for p, q in zip(got, want):
+            p = torch.cat((p[:4], p[-5:])) if p.shape[0] == rows else p
+            assert torch.equal(p.view(torch.uint8), q.view(torch.uint8))
+        del got
+
+
+def test_mx_quantize_of_more_values_than_a_launch_takes(gpu):
+    rows, k = (1 << 23) + 3, 4096  # 2^32 lanes of 8 values
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("100 GiB of memory needed")
+    part = torch.randn(9, k, generator=torch.Generator().manual_seed(0)).bfloat16().to(gpu)
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device=gpu)
+    x[:4], x[-5:] = part[:4], part[4:]
+    data, scale = ops().mx_quantize(x, "mxfp4")
+    want = ops().mx_quantize(part, "mxfp4")
+    for p, q in zip((data, scale), want):
+        assert torch.equal(torch.cat((p[:4], p[-5:])), q)
+    del x, data, scale, p
+    torch.cuda.empty_cache()
+
+
+def test_mx_linear_of_more_workgroups_than_a_launch_takes(gpu):
+    """Rows by the million take the streaming form (their exponents' offsets pass 32 bits in the tiled ones)."""
+    from test_gpu_mx_linear import packed_weight
+
+    m, n, k = 1 << 24, 136, 3840
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("80 GiB of memory needed")
+    w, ws = packed_weight(n, k, 0, gpu)
+    part, scales = packed_weight(40, k, 1, gpu)
+    want = ops().mx_linear(part[:16], w, ws, x_scale=scales[:16], out_dtype=torch.bfloat16)
+    x = torch.zeros(m, k // 2, dtype=torch.uint8, device=gpu)
+    xs = torch.full((m, k // 32), 127, dtype=torch.uint8, device=gpu)
+    for at in (0, m // 2 - 8, m - 16):
+        x[at:at + 16], xs[at:at + 16] = part[:16], scales[:16]
+    y = ops().mx_linear(x, w, ws, x_scale=xs)
+    for at in (0, m // 2 - 8, m - 16):
+        assert torch.equal(y[at:at + 16], want)
+    del x, xs, y
+    torch.cuda.empty_cache()
