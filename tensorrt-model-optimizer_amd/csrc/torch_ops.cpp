@@ -1429,15 +1429,18 @@ void kv_read(at::TensorList cache, at::Tensor k, at::Tensor v, const at::Tensor 
                            c.len_k.data_ptr<int32_t>(), c.batch, (int)max_len, dtype_code(k.scalar_type()), cur_stream(k)), what);
 }
 
-void kv_attention(at::TensorList cache, const at::Tensor &q, at::Tensor o, const at::Tensor &start, const at::Tensor &len_q,
+void kv_attention(at::TensorList cache, const at::Tensor &q_in, at::Tensor o, const at::Tensor &start, const at::Tensor &len_q,
                   const at::Tensor &len_k, const at::Tensor &table, int64_t max_len_q, int64_t max_len_k, bool is_causal,
                   double softmax_scale) {
   const char *what = "kv_attention";
-  check_device(q, "q");
-  const int dt = dtype_code(q.scalar_type());
+  check_device(q_in, "q");
+  const int dt = dtype_code(q_in.scalar_type());
   TORCH_CHECK(dt == MTQ_BF16 || dt == MTQ_F16, what, ": q must be bf16 or fp16");
-  const KvCall c = kv_call(cache, start, len_q, len_k, table, q, what);
-  check_kv_rows(q, c, "q", what);
+  const KvCall c = kv_call(cache, start, len_q, len_k, table, q_in, what);
+  check_kv_rows(q_in, c, "q", what);
+  // the kernels read q in pieces of 16 bytes: a copy only where its rows are not that aligned
+  const bool rows16 = (uintptr_t)q_in.data_ptr() % 16 == 0 && q_in.stride(0) % 8 == 0 && q_in.stride(1) % 8 == 0;
+  const at::Tensor q = rows16 ? q_in : q_in.clone(at::MemoryFormat::Contiguous);
   check_kv_rows(o, c, "o", what);
   TORCH_CHECK_VALUE(o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.device() == q.device(), what, ": o must be like q");
   TORCH_CHECK_VALUE(q.size(1) >= 1 && q.size(1) % c.c.num_kv_heads == 0, what, ": num_q_heads ", q.size(1),

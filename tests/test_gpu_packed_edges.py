@@ -473,3 +473,23 @@ def test_mx_linear_of_more_workgroups_than_a_launch_takes(gpu):
         assert torch.equal(y[at:at + 16], want)
     del x, xs, y
     torch.cuda.empty_cache()
+
+
+# ---- operands of any alignment ------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("q_len", [[3, 1], [60, 40]])
+def test_attention_of_queries_at_any_address(gpu, q_len):
+    from test_gpu_kv_fp4 import Batch
+
+    b = Batch(gpu, q_len, [700, 90], 16, 2, 128).fill()
+    q = b.queries(8)
+    want = b.cache.attention(q.to(gpu), *b.meta(), b.max_q, 700)
+    live = torch.cat([torch.arange(s, s + n) for s, n in zip(b.start, b.q_len)]).to(gpu)
+    shifted = torch.zeros(q.numel() + 1, dtype=q.dtype, device=gpu)[1:].view(q.shape)
+    wide = torch.zeros(b.tokens, 8, 133, dtype=q.dtype, device=gpu)[..., 5:]
+    for other in (shifted, wide):
+        other.copy_(q)
+        assert torch.equal(b.cache.attention(other, *b.meta(), b.max_q, 700)[live], want[live])
+    one = q[:, :1].to(gpu).expand(b.tokens, 8, 128)  # heads that share a row
+    b.check(b.cache.attention(one, *b.meta(), b.max_q, 700), one.cpu())
