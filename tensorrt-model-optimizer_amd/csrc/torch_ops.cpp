@@ -1230,6 +1230,14 @@ void check_float_rows(const at::Tensor &x, const char *what) {
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, what, ": at least one column expected");
 }
 
+// the factor that a call without rows hands over: the per-tensor format's goes by amax alone
+void factor_of_no_rows(const at::Tensor &x, int kind, const float *amax, at::Tensor &s, const char *what) {
+  if (kind != MTQ_FP8_TENSOR) return;
+  const at::Tensor row = at::zeros({8}, x.options()), q = at::empty({8}, x.options().dtype(at::kByte));
+  check_status(mtq_mx_quantize(row.data_ptr(), 8, 1, 8, dtype_code(x.scalar_type()), kind, amax, q.data_ptr<uint8_t>(), s.data_ptr(),
+                               cur_stream(x)), what);
+}
+
 }  // namespace
 
 std::tuple<at::Tensor, at::Tensor> mx_quantize(const at::Tensor &x, int64_t kind_, const c10::optional<at::Tensor> &amax) {
@@ -1239,7 +1247,11 @@ std::tuple<at::Tensor, at::Tensor> mx_quantize(const at::Tensor &x, int64_t kind
   at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(hip_device(x));
   auto [q, s] = row_outputs(x, kind, what);
   const float *am = amax_of(amax, kind, x, what);
-  if (x.numel() == 0 || x.is_meta()) return {q, s};
+  if (x.is_meta()) return {q, s};
+  if (x.numel() == 0) {
+    factor_of_no_rows(x, kind, am, s, what);
+    return {q, s};
+  }
   const at::Tensor v = as_rows(x);
   check_status(mtq_mx_quantize(v.data_ptr(), v.stride(0), v.size(0), v.size(1), dtype_code(v.scalar_type()), kind, am,
                                (uint8_t *)q.data_ptr(), s.data_ptr(), cur_stream(v)), what);
@@ -1268,7 +1280,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_quantize(const at::Tenso
   auto [q, s] = row_outputs(x, kind, what);
   const float *am = amax_of(amax, kind, x, what);
   at::Tensor h = has_r ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
-  if (x.numel() == 0 || x.is_meta()) return {q, s, h};
+  if (x.is_meta()) return {q, s, h};
+  if (x.numel() == 0) {
+    factor_of_no_rows(x, kind, am, s, what);
+    return {q, s, h};
+  }
   const at::Tensor v = as_rows(x), w = weight.contiguous();
   const at::Tensor r = has_r ? as_rows(*residual) : at::Tensor();
   check_status(mtq_rms_norm_quantize(v.data_ptr(), v.stride(0), has_r ? r.data_ptr() : nullptr, has_r ? r.stride(0) : 0,

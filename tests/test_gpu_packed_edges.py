@@ -493,3 +493,21 @@ def test_attention_of_queries_at_any_address(gpu, q_len):
         assert torch.equal(b.cache.attention(other, *b.meta(), b.max_q, 700)[live], want[live])
     one = q[:, :1].to(gpu).expand(b.tokens, 8, 128)  # heads that share a row
     b.check(b.cache.attention(one, *b.meta(), b.max_q, 700), one.cpu())
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_factor_of_no_rows(gpu, dtype):
+    """A call without rows still hands over the per-tensor factor."""
+    x = torch.randn(3, 64, device=gpu).to(DTYPES[dtype])
+    w = torch.ones(64, device=gpu).to(DTYPES[dtype])
+    for amax in (torch.full((1,), 3.3, device=gpu), torch.full((1,), 1e-30, device=gpu)):
+        want = ops().mx_quantize(x, "fp8", amax)[1]
+        for _ in range(3):
+            junk = torch.full((128,), float("nan"), device=gpu)  # what the allocator hands out next
+            del junk
+            data, scale = ops().mx_quantize(x[:0], "fp8", amax)
+            assert data.shape == (0, 64) and torch.equal(scale, want)
+            junk = torch.full((128,), float("nan"), device=gpu)
+            del junk
+            data, scale, h = ops().rms_norm_quantize(x[:0], w, residual=x[:0], format="fp8", amax=amax)
+            assert data.shape == h.shape == (0, 64) and torch.equal(scale, want)
