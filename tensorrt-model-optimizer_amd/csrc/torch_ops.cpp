@@ -1372,7 +1372,8 @@ KvCall kv_call(const at::TensorList &t, const at::Tensor &start, const at::Tenso
   KvCall k;
   TORCH_CHECK_VALUE(t.size() == 6, what, ": k_data, k_scale, v_data, v_scale, k_amax, v_amax expected");
   for (const at::Tensor &x : t) TORCH_CHECK_VALUE(x.is_cuda() && x.device() == like.device(), what, ": the cache must be on the input's device");
-  const int64_t D = 2 * t[0].size(-1);
+  const int64_t D = t[0].dim() ? 2 * t[0].size(-1) : 0;
+  TORCH_CHECK(D == 64 || D == 128 || D == 256, what, ": head_dim ", D, " is not supported (supported: 64, 128, 256)");
   for (int i = 0; i < 2; ++i) {
     const at::Tensor &d = t[2 * i], &s = t[2 * i + 1], &a = t[4 + i];
     TORCH_CHECK_VALUE(d.dim() == 4 && s.dim() == 4 && d.scalar_type() == at::kByte && s.element_size() == 1 &&
@@ -1380,6 +1381,9 @@ KvCall kv_call(const at::TensorList &t, const at::Tensor &start, const at::Tenso
                           s.size(2) == d.size(2) && s.size(3) * 16 == D && d.stride(3) == 1 && s.stride(3) == 1,
                       what, ": cache tensors must be [pages, kv_heads, page_size, head_dim / 2] codes and [.., head_dim / 16] scales");
     TORCH_CHECK_VALUE(a.numel() == 1 && a.scalar_type() == at::kFloat, what, ": amax must be one fp32 value");
+    bool rows = (uintptr_t)d.data_ptr() % 16 == 0 && (uintptr_t)s.data_ptr() % s.size(3) == 0;
+    for (int j = 0; j < 3; ++j) rows = rows && d.stride(j) % 16 == 0 && s.stride(j) % s.size(3) == 0;
+    TORCH_CHECK_VALUE(rows, what, ": rows of codes must lie at multiples of 16 bytes, rows of scales at multiples of their size");
     k.c.data[i] = d.data_ptr(), k.c.scale[i] = s.data_ptr(), k.c.amax[i] = a.data_ptr<float>();
     for (int j = 0; j < 3; ++j) k.c.data_strides[i][j] = d.stride(j), k.c.scale_strides[i][j] = s.stride(j);
   }
@@ -1449,6 +1453,7 @@ void kv_attention(at::TensorList cache, const at::Tensor &q_in, at::Tensor o, co
                   const at::Tensor &len_k, const at::Tensor &table, int64_t max_len_q, int64_t max_len_k, bool is_causal,
                   double softmax_scale) {
   const char *what = "kv_attention";
+  TORCH_CHECK(softmax_scale > 0.0 && softmax_scale < 3.4e38, what, ": softmax_scale must be positive and finite, got ", softmax_scale);
   check_device(q_in, "q");
   const int dt = dtype_code(q_in.scalar_type());
   TORCH_CHECK(dt == MTQ_BF16 || dt == MTQ_F16, what, ": q must be bf16 or fp16");

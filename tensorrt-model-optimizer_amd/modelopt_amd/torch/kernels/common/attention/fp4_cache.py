@@ -36,8 +36,7 @@ class NVFP4KVCache:
 
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, *, k_amax=2688.0, v_amax=2688.0,
                  device="cuda"):
-        if head_dim not in (64, 128, 256):
-            raise NotImplementedError(f"head_dim {head_dim} is not supported (supported: 64, 128, 256)")
+        self._check_head_dim(head_dim)
         shape = (num_pages, num_kv_heads, page_size)
 
         def scalar(v):
@@ -47,10 +46,15 @@ class NVFP4KVCache:
         scale = [torch.zeros(*shape, head_dim // 16, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
         self._set(data[0], scale[0], data[1], scale[1], scalar(k_amax), scalar(v_amax))
 
+    @staticmethod
+    def _check_head_dim(head_dim):
+        if head_dim not in (64, 128, 256):
+            raise NotImplementedError(f"head_dim {head_dim} is not supported (supported: 64, 128, 256)")
+
     @classmethod
     def from_tensors(cls, k_data, k_scale, v_data, v_scale, k_amax, v_amax) -> "NVFP4KVCache":
-        """A cache over tensors that the caller holds (any strides over pages, heads and places, rows
-        contiguous)."""
+        """A cache over tensors that the caller holds (any strides over pages, heads and places; rows contiguous, of
+        codes at multiples of 16 bytes, of scales at multiples of ``head_dim / 16``)."""
         self = cls.__new__(cls)
         self._set(k_data, k_scale, v_data, v_scale, k_amax, v_amax)
         return self
@@ -58,6 +62,7 @@ class NVFP4KVCache:
     def _set(self, k_data, k_scale, v_data, v_scale, k_amax, v_amax):
         if k_data.dim() != 4 or v_data.shape != k_data.shape:
             raise ValueError("k_data and v_data must both be [num_pages, num_kv_heads, page_size, head_dim / 2]")
+        self._check_head_dim(2 * k_data.shape[3])
         page_size = k_data.shape[2]
         if not 16 <= page_size <= 32768 or page_size & (page_size - 1):
             raise ValueError(f"page_size must be a power of two from 16 to 32768, got {page_size}")
@@ -96,7 +101,8 @@ class NVFP4KVCache:
 
         Causal: a query sees the keys up to its own position.  A query that sees no key gives zeros; rows of
         no sequence are not written, as ``attention()``.  ``max_kv_len`` (a bound of ``b_seq_len_k``, default what
-        ``block_table`` can hold) sizes the split over the keys."""
+        ``block_table`` can hold) sizes the split over the keys.  ``softmax_scale`` is positive (default
+        ``head_dim ** -0.5``)."""
         check_device("NVFP4KVCache.attention", q)
         refuse_grad("NVFP4KVCache.attention", q)
         if max_kv_len is None:

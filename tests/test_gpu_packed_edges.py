@@ -15,6 +15,12 @@ def ops():
     return q
 
 
+def ops_lib():
+    from modelopt_amd import _ext
+
+    return _ext.ops()
+
+
 def token_codes(x):
     """The definition of FP8 per token: (codes as values, factors), by division in 32 bits."""
     a = torch.nan_to_num(x.float().abs(), nan=0.0, posinf=torch.finfo(torch.float32).max).amax(-1, keepdim=True)
@@ -511,3 +517,32 @@ def test_factor_of_no_rows(gpu, dtype):
             del junk
             data, scale, h = ops().rms_norm_quantize(x[:0], w, residual=x[:0], format="fp8", amax=amax)
             assert data.shape == h.shape == (0, 64) and torch.equal(scale, want)
+
+
+def test_refusals_say_why(gpu):
+    from modelopt_amd.torch.kernels.common.attention import NVFP4KVCache
+    from test_gpu_kv_fp4 import Batch
+
+    b = Batch(gpu, [3, 1], [70, 90], 16, 2, 128).fill()
+    c, q = b.cache, b.queries(8).to(gpu)
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(RuntimeError, match="softmax_scale"):
+            c.attention(q, *b.meta(), 3, 90, softmax_scale=scale)
+    codes = torch.zeros(c.k_data.numel() + 8, dtype=torch.uint8, device=gpu)[8:].view(c.k_data.shape)
+    pitch = torch.zeros(*c.k_data.shape[:3], 72, dtype=torch.uint8, device=gpu)[..., :64]
+    scales = torch.zeros(c.k_scale.numel() + 1, dtype=torch.uint8, device=gpu)[1:].view(c.k_scale.shape).view(torch.float8_e4m3fn)
+    for data, scale in ((codes, c.k_scale), (pitch, c.k_scale), (c.k_data, scales)):
+        bad = NVFP4KVCache.from_tensors(data, scale, c.v_data, c.v_scale, c.k_amax, c.v_amax)
+        k = torch.randn(b.tokens, 2, 128, device=gpu).bfloat16()
+        for call in (lambda: bad.attention(q, *b.meta(), 3, 90), lambda: bad.append(k, k, *b.meta(), 3),
+                     lambda: bad.read(*b.meta(), 3, b.tokens)):
+            with pytest.raises(ValueError, match="multiples"):
+                call()
+    for d in (0, 32, 96):
+        data, scale = c.k_data[..., :d // 2].contiguous(), c.k_scale.view(torch.uint8)[..., :d // 16].contiguous().view(torch.float8_e4m3fn)
+        if d == 96:
+            data, scale = torch.zeros(4, 2, 16, 48, dtype=torch.uint8, device=gpu), torch.zeros(4, 2, 16, 6, device=gpu).to(torch.float8_e4m3fn)
+        with pytest.raises(NotImplementedError, match="head_dim"):
+            NVFP4KVCache.from_tensors(data, scale, data, scale, c.k_amax, c.v_amax)
+        with pytest.raises(RuntimeError, match="head_dim"):
+            ops_lib().kv_attention([data, scale, data, scale, c.k_amax, c.v_amax], q[..., :d], q[..., :d].clone(), *b.meta(), 3, 90, True, 1.0)
