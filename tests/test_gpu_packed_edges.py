@@ -546,3 +546,16 @@ def test_refusals_say_why(gpu):
             NVFP4KVCache.from_tensors(data, scale, data, scale, c.k_amax, c.v_amax)
         with pytest.raises(RuntimeError, match="head_dim"):
             ops_lib().kv_attention([data, scale, data, scale, c.k_amax, c.v_amax], q[..., :d], q[..., :d].clone(), *b.meta(), 3, 90, True, 1.0)
+
+
+@pytest.mark.parametrize("calibrated", [True, False])
+@pytest.mark.parametrize("preset", ["W4A8_MXFP4_FP8_CFG", "MXFP4_DEFAULT_CFG"])
+def test_mx_gemm_of_no_rows(gpu, preset, calibrated):
+    """An expert that no token reached, in calibration or now."""
+    layer, data = compressed(gpu, preset)
+    if not calibrated:
+        layer.input_quantizer.reset_amax()
+    with torch.no_grad():
+        for x in (data[:0], data[:0].view(0, 3, 256)):
+            y = layer(x)
+            assert y.shape == (*x.shape[:-1], 384) and y.dtype == data.dtype
