@@ -124,7 +124,7 @@ __device__ __forceinline__ uint2 e4m3_codes8(const float (&v)[8], float s) {
 // 1 / d would be rounded twice (codes flip at their borders), and 1 / d is past fp32 for d < 2^-128: rows of a
 // small d have both sides multiplied by 2^64 first, exactly.
 struct RowFactor {
-  float d, by, up, r, most;  // x / d = x up / by, r = 1 / by; |x up| is cut at `most`: infinities, a d rounded down
+  float d, by, lo, up, r, most;  // x / d = x up / by, r = 1 / by; |x up| is cut at `most`: infinities, a d rounded down
 };
 __device__ __forceinline__ RowFactor row_factor(float most) {
   RowFactor f;
@@ -135,6 +135,27 @@ __device__ __forceinline__ RowFactor row_factor(float most) {
   f.r = 1.0f / f.by;
   f.most = clamp_flt_max(f.by * kE4M3Max);
   return f;
+}
+// The quotients x / (most / 448) before the divisor is rounded, for rows whose factor d is that times something
+// that they all share: by + lo is most / 448, |x| <= most.
+__device__ __forceinline__ RowFactor row_quotient(float most, float d) {
+  RowFactor f;
+  f.d = d;
+  f.up = most < 0x1p-56f ? 0x1p64f : 1.f;
+  f.by = most * f.up / kE4M3Max;
+  f.lo = __builtin_fmaf(-f.by, kE4M3Max, most * f.up) / kE4M3Max;
+  f.r = 1.0f / f.by;
+  return f;
+}
+__device__ __forceinline__ uint2 e4m3_quotients8(const float (&v)[8], const RowFactor &f) {
+  float a[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = v[j] * f.up, y = x * f.r;
+    const float e = __builtin_fmaf(-y, f.lo, __builtin_fmaf(-y, f.by, x));
+    a[j] = __builtin_copysignf(__builtin_fmaf(e, f.r, y), x);
+  }
+  return e4m3_bytes8(a);
 }
 __device__ __forceinline__ uint2 e4m3_codes8(const float (&v)[8], const RowFactor &f) {
   float a[8];
@@ -196,7 +217,8 @@ __device__ __forceinline__ float wave_max(float v) {
 // pair of floats, and x * w of 16-bit operands is exact before the one product.  The MX formats, whose
 // factors are powers of two, take y rounded to odd where it matters (round_odd): rounding that again to a code,
 // or comparing it with a border, is then as good as y itself (16384 x 4096: 2 to 5 codes off by a step, 20 to
-// 40 without; 94 us with, 88 without).
+// 40 without; 94 us with, 88 without).  FP8 per token takes y / (max|y| / 448) = p / (max|p| / 448), p = x w: the
+// root cancels, and of 2501 x 5000 codes 1 to 3 are off by a step (quotients that fp32 rounds onto a border).
 // us: 16 x 4096 with residual 4.5 (a launch); 16384 x 4096 with residual 92 (472 MB, 5.1 TB/s: the rate of a
 // large copy); 2501 x 5000 fp16 per token 15 (37 MB, 2.5 TB/s; a row is less than a workgroup can hide).
 struct NormArgs {
@@ -222,7 +244,7 @@ template <typename T, int KIND, int NV, bool VEC>
 __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
   __shared__ double red[16];
   __shared__ float redm[16];
-  constexpr bool MX = KIND == MTQ_MXFP4 || KIND == MTQ_MXFP8;
+  constexpr bool MX = KIND == MTQ_MXFP4 || KIND == MTQ_MXFP8, TOKEN = KIND == MTQ_FP8_TOKEN;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
   const T *x = reinterpret_cast<const T *>(a.x) + row * a.xs;
@@ -268,12 +290,13 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float p = f[u][j] * w[j];
-      f[u][j] = MX ? p : __builtin_fmaf(p, rh, p * rl);
+      f[u][j] = MX || TOKEN ? p : __builtin_fmaf(p, rh, p * rl);
     }
   }
   float s = 1.f;
   RowFactor rf{};
-  if constexpr (KIND == MTQ_FP8_TOKEN) {
+  bool regular = true;
+  if constexpr (TOKEN) {
     float m = 0.f;
 #pragma unroll
     for (int u = 0; u < NV; ++u)
@@ -284,7 +307,19 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
     __syncthreads();
     m = 0.f;
     for (int i = 0; i < nw; ++i) m = fmaxf(m, redm[i]);
-    rf = row_factor(m);
+    // y / (max|y| / 448) = p / (max|p| / 448): the root cancels, and with it y's own roundings
+    const float d = (float)((double)m * rd / (double)kE4M3Max);
+    regular = rd < __builtin_inf() && m < 3.402823466e38f && d > 0.f && d < __builtin_inff();
+    if (regular) {
+      rf = row_quotient(m, d);
+    } else {  // rows of y = 0, NaN, infinities, or below what a factor can be: through y itself
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[u][j] *= (float)rd;
+      const bool inf = rd > 0.0 && (m == 3.402823466e38f || (m > 0.f && (rd == __builtin_inf() || d == __builtin_inff())));
+      rf = row_factor(inf ? 3.402823466e38f : 0.f);
+    }
     if (tid == 0) reinterpret_cast<float *>(a.scale)[row] = rf.d;
   } else if constexpr (KIND == MTQ_FP8_TENSOR) {
     const Fp8Q p = make_fp8q(*a.amax);
@@ -312,7 +347,8 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
       }
       mx_store8<KIND>(v, col, q, reinterpret_cast<uint8_t *>(a.scale) + row * (a.cols / 32), col < a.cols);
     } else if (col < a.cols) {
-      fp8_store8<VEC>(KIND == MTQ_FP8_TOKEN ? e4m3_codes8(f[u], rf) : e4m3_codes8(f[u], s), col, a.cols, a.q + row * a.cols);
+      const uint2 w = !TOKEN ? e4m3_codes8(f[u], s) : regular ? e4m3_quotients8(f[u], rf) : e4m3_codes8(f[u], rf);
+      fp8_store8<VEC>(w, col, a.cols, a.q + row * a.cols);
     }
   }
 }
