@@ -308,8 +308,9 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
     m = 0.f;
     for (int i = 0; i < nw; ++i) m = fmaxf(m, redm[i]);
     // y / (max|y| / 448) = p / (max|p| / 448): the root cancels, and with it y's own roundings
-    const float d = (float)((double)m * rd / (double)kE4M3Max);
-    regular = rd < __builtin_inf() && m < 3.402823466e38f && d > 0.f && d < __builtin_inff();
+    const double top = (double)m * rd;  // max|y|
+    const float d = (float)(top / (double)kE4M3Max);
+    regular = rd < __builtin_inf() && m < 3.402823466e38f && d > 0.f && (float)top < __builtin_inff();
     if (regular) {
       rf = row_quotient(m, d);
     } else {  // rows of y = 0, NaN, infinities, or below what a factor can be: through y itself
@@ -317,7 +318,7 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a) {
       for (int u = 0; u < NV; ++u)
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[u][j] *= (float)rd;
-      const bool inf = rd > 0.0 && (m == 3.402823466e38f || (m > 0.f && (rd == __builtin_inf() || d == __builtin_inff())));
+      const bool inf = rd > 0.0 && (m == 3.402823466e38f || (m > 0.f && (float)top == __builtin_inff()));
       rf = row_factor(inf ? 3.402823466e38f : 0.f);
     }
     if (tid == 0) reinterpret_cast<float *>(a.scale)[row] = rf.d;

@@ -559,3 +559,62 @@ def test_mx_gemm_of_no_rows(gpu, preset, calibrated):
         for x in (data[:0], data[:0].view(0, 3, 256)):
             y = layer(x)
             assert y.shape == (*x.shape[:-1], 384) and y.dtype == data.dtype
+
+
+# ---- the norm to FP8 per token ------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,h", [("fp16", 5000), ("bf16", 4096), ("fp16", 20000)])
+def test_rms_norm_fp8_token_codes(gpu, dtype, h):
+    """y / (max|y| / 448) = x w / (max|x w| / 448), whose products are exact: codes are its rounding, halves to even, but
+    for quotients within half a step of 2^-23 of a border, which 32 bits put onto it."""
+    g = torch.Generator().manual_seed(h)
+    x = torch.randn(400, h, generator=g).to(DTYPES[dtype])
+    w = (1 + 0.2 * torch.randn(h, generator=g)).to(DTYPES[dtype])
+    data, _, _ = ops().rms_norm_quantize(x.to(gpu), w.to(gpu), 1e-5, format="fp8_token")
+    p = x.double() * w.double()
+    z = 448 * p / p.abs().amax(-1, keepdim=True)
+    step = torch.exp2(torch.floor(torch.log2(z.abs().clamp(min=2.0 ** -8))).clamp(min=-6) - 3)
+    t = z / step
+    want = torch.round(t) * step
+    gap = ((t - torch.floor(t)) - 0.5).abs()
+    close = (gap > 0) & (gap <= t.abs() * 2.0 ** -23)
+    off = data.cpu().double() != want
+    assert not (off & ~close).any()
+    assert close.sum() < 100 and ((gap == 0) & (z != 0)).any()  # ties were met
+
+
+@pytest.mark.parametrize("h", [64, 5001])
+def test_rms_norm_fp8_token_of_irregular_rows(gpu, h):
+    """Rows without a factor of their own (NaN, infinities, zeros, y past either end of 32 bits), as the plain form."""
+    most = torch.finfo(torch.float32).max
+
+    def run(x, w, eps):
+        data, scale, _ = ops().rms_norm_quantize(x.to(gpu), w.to(gpu), eps, format="fp8_token")
+        return data.cpu().float(), scale.cpu().flatten()
+
+    x, w = torch.randn(7, h), 1 + 0.1 * torch.randn(h)
+    x[1, 3], x[2, 4], x[3] = float("nan"), float("inf"), 0
+    x[4] *= 1e25  # squares past 32 bits
+    data, scale = run(x, w, 1e-6)
+    assert torch.isnan(data[1]).all() and scale[1] == 1
+    assert torch.isnan(data[2, 4]) and (data[2, :4] == 0).all() and (data[2, 5:] == 0).all() and scale[2] == 1
+    assert (data[3] == 0).all() and scale[3] == 1
+    assert (data[4] == 0).all() and scale[4] == 1
+    for r in (0, 5, 6):  # the others are what they are alone
+        alone = run(x[r:r + 1], w, 1e-6)
+        assert torch.equal(data[r], alone[0][0]) and scale[r] == alone[1][0] and data[r].abs().max() == 448
+    data, scale = run(x[3:4], w, 0.0)  # 0 / 0
+    assert torch.isnan(data).all() and scale[0] == 1
+    w[7] = float("nan")
+    data, scale = run(x[:1], w, 1e-6)
+    assert torch.isnan(data[0, 7]) and torch.isnan(data).sum() == 1 and data[0, :7].abs().max() > 0
+    w[7], x[0, 7] = float("inf"), -2.0
+    data, scale = run(x[:1], w, 1e-6)
+    assert data[0, 7] == -448 and scale[0] == torch.tensor(most) / 448 and (data[0, :7] == 0).all()
+    data, scale = run(torch.ones(1, h), torch.full((h,), 1e-44), 1e-6)  # below what a factor can be
+    assert (data == 0).all() and scale[0] == 1
+    x = torch.full((1, h), 1e-3)
+    x[0, 0] = 1.0
+    data, scale = run(x, torch.full((h,), 3e38), 1e-6)  # y = sqrt(h) 3e38 at column 0
+    assert scale[0] == torch.tensor(most) / 448 and data[0, 0] == 448
