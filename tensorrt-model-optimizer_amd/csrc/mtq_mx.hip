@@ -1346,7 +1346,14 @@ LinearPlan linear_plan(int64_t M, int64_t N, int64_t K, int kind) {
   if (M <= kSkinnyRows || pad * (K / 32 + 8) >= (1ll << 31)) return p;
   const int64_t cus = host_num_cus();
   auto tiles = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-  if (M > 128 && tiles(256, 256) * 4 >= cus * 3 && K > pp_bk(kind != MTQ_MXFP4)) {  // two K tiles at least
+  // 256 x 256 tiles for three quarters of the CUs, and two K tiles at least.  Their order goes by units of 8 x 4 tiles,
+  // and a unit that the matrix fills by half costs as much as a whole one: more than 9/16 of the slots have to hold a
+  // tile.  us, E2M1 rows / E4M3 rows, the tiles below in brackets: x 14336 x 4096, 1024 rows (1/2 of the slots) 68 (60) /
+  // 104 (89), 1280 (5/8) 69 (83) / 105 (101), 1536 69 (85) / 105 (121), 2304 (9/16) 130 (120) / 208 (184), 2560 (5/8)
+  // 129 (140) / 209 (205); 300 x 28672 x 8192 (1/4) 227 (94) / 384 (129); 30000 x 512 x 4096 68 (63) / 107 (98).
+  // x 4096 x 4096: 2048 rows (128 tiles) 42 (31) / 60 (46), 2560 (160) 41 (51) / 56 (62), 3328 (208) 40 (55) / 56 (82).
+  const int64_t slots = (M + 2047) / 2048 * 8 * ((N + 1023) / 1024 * 4);
+  if (tiles(256, 256) * 4 >= cus * 3 && tiles(256, 256) * 16 > slots * 9 && K > pp_bk(kind != MTQ_MXFP4)) {
     p.form = LinearPlan::kPp;
     return p;
   }

@@ -618,3 +618,59 @@ def test_rms_norm_fp8_token_of_irregular_rows(gpu, h):
     x[0, 0] = 1.0
     data, scale = run(x, torch.full((h,), 3e38), 1e-6)  # y = sqrt(h) 3e38 at column 0
     assert scale[0] == torch.tensor(most) / 448 and data[0, 0] == 448
+
+
+# ---- mx_linear's forms -------------------------------------------------------------------------------------------------
+
+
+def form_of(m, n, k, fmt):
+    """The bytes that each form's workspace has for quantised rows: the 256 x 256 tiles lay out both operands' exponents."""
+    import ctypes
+
+    from modelopt_amd import _ext
+
+    f = _ext.kernel_cdll().mtq_mx_linear_workspace_bytes
+    f.argtypes, f.restype = [ctypes.c_int64] * 3 + [ctypes.c_int] * 2, ctypes.c_size_t
+    kind = {"mxfp4": 0, "mxfp8": 1, "fp8": 2, "fp8_token": 3}[fmt]
+    per = -(-k // (256 if kind == 0 else 128)) * (8 if kind == 0 else 4)
+    up = lambda r: (r + 255) // 256 * 256
+    return "256" if f(m, n, k, kind, -1) == up(n) * per + (up(m) * per if kind < 2 else 0) and k % 256 == 0 else "other"
+
+
+def test_mx_linear_takes_the_large_tiles_where_their_order_is_filled(gpu):
+    for fmt in ("mxfp4", "mxfp8", "fp8"):
+        assert form_of(8192, 14336, 4096, fmt) == form_of(4096, 4096, 4096, fmt) == form_of(1536, 14336, 4096, fmt) == "256"
+        for m, n, k in ((300, 28672, 8192), (1024, 14336, 4096), (2304, 14336, 4096), (30000, 512, 4096), (2048, 4096, 4096)):
+            assert form_of(m, n, k, fmt) == "other", (m, n, k)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8", "fp8", "fp8_token"])
+@pytest.mark.parametrize("m,n,k", [(3900, 3700, 352), (3900, 3700, 288), (3801, 3583, 512), (3900, 3700, 160), (1301, 9999, 1056)])
+def test_mx_linear_large_tiles(gpu, fmt, m, n, k):
+    """256 x 256 tiles at sizes that nothing divides, NaN and infinities in rows of their own, from a graph too."""
+    from test_gpu_mx_linear import check_product, packed_weight, rows, values
+
+    x = rows(m, k, torch.bfloat16, seed=k, special=True)
+    x[m - 1, 3], x[m - 2, k - 1] = float("nan"), -float("inf")
+    xg = x.to(gpu)
+    w, ws = packed_weight(n, k, m, gpu)
+    bias = torch.randn(n, device=gpu)
+    amax = torch.full((1,), 5.0, device=gpu) if fmt == "fp8" else None
+    y = ops().mx_linear(xg, w, ws, bias, format=fmt, amax=amax)
+    data, scale = ops().mx_quantize(xg, fmt, amax)
+    v = values(data, scale, fmt)
+    keep = ~torch.isnan(v).any(-1)
+    assert (~keep).sum() == (0 if fmt == "mxfp4" else 2)
+    check_product(y[keep.to(gpu)], v[keep], w, ws, bias, k, fmt != "mxfp4")
+    assert torch.isnan(y[~keep.to(gpu)]).all()
+    ops().mx_linear(data, w, ws, bias, format=fmt, x_scale=scale)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops().mx_linear(xg, w, ws, bias, format=fmt, amax=amax)
+    for i in range(3):
+        xg.copy_(torch.randn(m, k, device=gpu) * (i + 1))
+        graph.replay()
+        want = ops().mx_linear(xg, w, ws, bias, format=fmt, amax=amax)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
