@@ -114,8 +114,8 @@ __device__ __forceinline__ float min448(float v) {
   return r;
 }
 
-// RN(a / s) for a pair of a >= +0 (or NaN) on the packed fp32 ALU: div_rn (mtq_device.hpp) without
-// its copysign -- p never is -0 -- two quotients per v_pk_mul / v_pk_fma
+// RN(a / s) for a pair of a >= +0 (or NaN): div_rn (mtq_device.hpp) without its copysign -- p never is
+// -0 (the build has no packed fp32 instructions, so a pair is two of each)
 __device__ __forceinline__ f2v div_rn_pos2(f2v q, float s, float r) {
   const f2v sv = {s, s}, rv = {r, r};
   const f2v y0 = q * rv;
@@ -380,7 +380,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs &a, int b, int h, int k
           mloc = fmaxf(mloc, x[j]);
         }
       } else {
-        const f2v qs2 = {a.qk_scale, a.qk_scale};  // two scores per v_pk_mul_f32 (same products)
+        const f2v qs2 = {a.qk_scale, a.qk_scale};
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
           const f2v xv = f2v{s[j], s[j + 1]} * qs2;

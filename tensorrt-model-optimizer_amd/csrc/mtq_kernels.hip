@@ -2561,8 +2561,8 @@ __device__ __forceinline__ float div_rn_pz(float q, float s, float r) {
   return __builtin_fmaf(e, r, y0) + 0.0f;
 }
 
-// div_rn on a pair through the packed fp32 ALU (v_pk_mul_f32 / v_pk_fma_f32: two lanes' worth of
-// work per issue), and the pair's dtype re-rounding (bf16: one v_cvt_pk_bf16_f32).
+// div_rn on a pair, and the pair's dtype re-rounding (bf16: one v_cvt_pk_bf16_f32).  (The build has no packed
+// fp32 instructions.)
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2_t div_rn2(f32x2_t q, float s, float r) {
   const f32x2_t sv = {s, s}, rv = {r, r};
@@ -2705,11 +2705,11 @@ __device__ __forceinline__ void export_int4_pack(const Int4Pair<T> &q, uint8_t *
   uint32_t b[N];
   constexpr float kInf = __builtin_huge_valf();
   if (__builtin_expect(r0 < kInf && r1 < kInf && s0 < kInf && s1 < kInf, 1)) {
-    // the (row 2p, row 2p+1) pair of column j on the packed ALU: div_rn of both quotients per
-    // v_pk_mul / v_pk_fma (no copysign: a -0 quotient packs as 0 like +0), clamp to [-8, 7] by
+    // the (row 2p, row 2p+1) pair of column j: div_rn of both quotients (no copysign: a -0
+    // quotient packs as 0 like +0), clamp to [-8, 7] by
     // v_med3_f32 (clamping before rounding is the same: the bounds are integers), then
     // RN-to-integer and the two's-complement nibble at once: q + 1.5 * 2^23 has ulp 1, so its low
-    // mantissa bits ARE rint(q) mod 2^22 (one v_pk_add_f32 for the pair).  A NaN quotient (an
+    // mantissa bits ARE rint(q) mod 2^22 (one addition each).  A NaN quotient (an
     // infinite weight, an overflowing quotient, a NaN weight) sends the lane to int4_pair_nan.
     const f32x2_t sv = {s0, s1}, rv = {r0, r1}, magic = {12582912.0f, 12582912.0f};
     f32x2_t d[N];

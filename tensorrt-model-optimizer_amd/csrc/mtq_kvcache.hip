@@ -73,7 +73,7 @@ __device__ __forceinline__ int page_of(const Cache &c, int b, int pos) { return 
 // neighbouring lanes.  A workgroup takes tokens of one head where the call has them (2^lt of them, then heads):
 // in the cache's layout these lie behind each other, 16 of them at head_dim 128 being 1 KiB of codes and a
 // line of scales, while k and v are met in pieces of a row (256 bytes there).  Bound by HBM (16 + 4.5 bytes a
-// lane): 3.4 TB/s each way at the size below.
+// lane): 3.7 TB/s each way at the size below.
 struct RowArgs {
   Cache c;
   void *x[2];             // k, v
@@ -82,9 +82,10 @@ struct RowArgs {
   int lt, passes;
   int max_len;  // tokens of a sequence from max_len on are left out, also where its last pass reaches them
 };
-// Tokens of a lane in flight at once, and whether it loops over more.  us for the prompts of 7 sequences, 131 MB
-// at 8 heads of 128: 1 / 2 / 4 tokens: append 51 / 46 / 44, read 50 / 45 / 39; looping, with at most 48
-// workgroups a CU: append 38 / 39 / 45, read 46 / 46 / 43 (16 workgroups: over 50, the sequences are unequal)
+// Tokens of a lane in flight at once, and whether it loops over more.  us for the prompts of 7 sequences, 27954 tokens
+// of 8 heads of 128 (147 MB each way), each call for itself: append, 1 / 2 / 4 tokens, looping with at most 48
+// workgroups a CU 39 / 40 / 46, without a loop 2 / 4 tokens 44 / 47; read 1 / 2 / 4 / 8 tokens 50 / 45 / 39 / 39.  (Right
+// behind the append, whose codes are still in the caches, the read takes 26 to 30.)
 constexpr int kAppendAhead = 2, kReadAhead = 4, kAppendWgs = 48;
 
 // what a lane works on: false where there is none of it
@@ -256,7 +257,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(RowArgs a) {
 // of their own, joined through LDS at the end (in wave order).  Where there are few sequences the
 // keys are cut into splits; their partial results are joined by a second small kernel, in order.
 // Bound by the cache's bytes: 64 single tokens over up to 16384 keys, 32 / 8 heads of 128: 163 us (717 MB, 4.4
-// TB/s; the loads alone take 134).
+// TB/s; matrix cores busy 14 % of the time); head_dim 64: 110 (3.2 TB/s), 256 with 16 / 4 heads: 179 (4.0).
 struct AttnArgs {
   Cache c;
   const void *q;
@@ -603,9 +604,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 // are 16 KiB of fragments: 128 cycles of LDS beside 512 of one SIMD's matrix core, four SIMDs at once).  A
 // workgroup is 8 waves of 32 rows (v_mfma_f32_32x32x16_f16) on one KV head, two waves a SIMD; 64 keys at
 // a time are turned into fp16 by the whole workgroup, once per 256 rows, into one of three LDS stages.
-// Chunks of 500 to 1024 tokens behind contexts of up to 8192, 4 sequences, 32 / 8 heads of 128: 365 us (810
-// TFLOP/s).  64 rows a wave, one wave a SIMD, half the LDS reads took 546 where this layout took 409 (before
-// its page entries were loaded ahead): nothing of its one wave overlaps.
+// Chunks of 500 to 1024 tokens behind contexts of up to 8192, 4 sequences, 32 / 8 heads of 128: 370 us (800 TFLOP/s)
+// back to back, 380 to 455 where each call is waited for; matrix cores busy 41 % of the time, LDS 36 %, 29 % of that
+// in conflicts.  head_dim 64: 277 us (536 TFLOP/s).  64 rows a wave, one wave a SIMD, half the LDS reads took 546
+// where this layout took 409 (before its page entries were loaded ahead): nothing of its one wave overlaps.
 // The loop over 32-key tiles is pipelined in registers: the step of tile j multiplies K of tile j + 1
 // and V of tile j - 1 while the softmax of tile j runs, three chains without a dependency between them.
 __device__ __forceinline__ float xmax32(float v) {  // v and its lane ^ 32 partner
@@ -944,7 +946,10 @@ struct Plan {
   int tiles, part_tiles, chunk, splits;
   bool prompt;
 };
-// rows of a KV head from which the prompt kernel is taken
+// Rows of a KV head from which the prompt kernel is taken.  us, prompt / decode kernel, 32 / 8 heads of 128 (4 rows a
+// token): 1 sequence of 8192 keys, 64 rows 29 / 22, 96 30 / 27, 128 32 / 30, 256 41 / 40, 512 46 / 58; 8 of them, 64 rows
+// 78 / 53, 96 83 / 76, 128 86 / 97, 256 99 / 159; 64 of 2048 keys, 64 rows 142 / 73, 128 144 / 139.  (Contexts of a few
+// hundred keys, which the prompt kernel does not split, would gain from more: 2 of 500 keys, 128 rows 24 / 10.)
 constexpr int kPromptRows = 128;
 
 // the rows of a KV head that a call has room for (ints in the kernels)
@@ -960,7 +965,9 @@ Plan attn_plan(int batch, int hkv, int group, int head_dim, int max_len_q, int m
   Plan p;
   if (max_len_k > INT32_MAX / 2) max_len_k = INT32_MAX / 2;  // the most positions that a cache can have
   const int64_t rows = (int64_t)max_len_q * group;
-  p.prompt = rows >= kPromptRows && head_dim <= 128;  // head_dim 256: its three stages do not fit LDS
+  // head_dim 256: the prompt kernel's three stages do not fit LDS, and the decode kernel unpacks every key again for 16
+  // rows (the chunks above with 16 / 4 heads of 256: 713 us, 416 TFLOP/s)
+  p.prompt = rows >= kPromptRows && head_dim <= 128;
   p.part_tiles = (int)((rows + 15) / 16);
   p.tiles = p.prompt ? (int)((rows + 255) / 256) : p.part_tiles;
   const int64_t wgs = (int64_t)batch * hkv * p.tiles, cus = host_num_cus();

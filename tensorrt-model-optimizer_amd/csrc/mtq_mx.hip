@@ -219,8 +219,9 @@ __device__ __forceinline__ float wave_max(float v) {
 // or comparing it with a border, is then as good as y itself (16384 x 4096: 2 to 5 codes off by a step, 20 to
 // 40 without; 94 us with, 88 without).  FP8 per token takes y / (max|y| / 448) = p / (max|p| / 448), p = x w: the
 // root cancels, and of 2501 x 5000 codes 1 to 3 are off by a step (quotients that fp32 rounds onto a border).
-// us: 16 x 4096 with residual 4.5 (a launch); 16384 x 4096 with residual 92 (472 MB, 5.1 TB/s: the rate of a
-// large copy); 2501 x 5000 fp16 per token 15 (37 MB, 2.5 TB/s; a row is less than a workgroup can hide).
+// us: 16 x 4096 with residual 5 (a launch); 16384 x 4096 with residual 94 to MXFP8 and MXFP4, 85 to FP8 per tensor, 90
+// per token (472 MB: 5.0 TB/s, 5.5, 5.2; a copy of 1 GiB 5.2, a sum of two such tensors 6.0); 2501 x 5000 fp16 per
+// token 15.6 (37 MB, 2.4 TB/s; a row is less than a workgroup can hide).
 struct NormArgs {
   const void *x, *r, *w;
   void *h;
@@ -434,8 +435,8 @@ __device__ __forceinline__ void mxfp4_store8_packed(const u32x4 &x, int64_t col,
 }
 
 // ---- quantising rows ---------------------------------------------------------------------------
-// MX and per-tensor FP8: 8 values a lane over all rows (a block's 4 lanes are neighbours).  Bound by HBM:
-// 8192 x 4096 bf16 to MXFP4 22 us (86 MB, 3.9 TB/s).
+// MX and per-tensor FP8: 8 values a lane over all rows (a block's 4 lanes are neighbours).  Bound by HBM: 16384 x 4096
+// bf16 to MXFP4 32 us (5.3 TB/s), to MXFP8 43 (4.8), to FP8 per tensor 38 (5.4), per token 45 (4.5).
 template <typename T, int KIND, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ x, int64_t xs, int64_t rows, int64_t cols,
                                                           const float *__restrict__ amax, uint8_t *__restrict__ q,
@@ -770,16 +771,16 @@ template <typename T, int OP> int launch_skinny(const SkinnyArgs &all, hipStream
 // half-tile two to five phases ahead and waits with a counted vmcnt, and waves 4-7 run one barrier
 // behind waves 0-3, so that one wave of a SIMD reads LDS while the other multiplies.  The K tiles of all
 // the workgroup's tiles of y are one stream: what is loaded ahead at a tile's end is the next tile's.
-// us for xq 8192 x 4096, W 14336 x 4096: 257 E2M1 (3.74 PFLOP/s; each further 4096 columns: 205, 4.7), 390
-// E4M3 (2.47); without the stores 226 and 353: they come from all CUs at once, 128 KiB a tile, and loads
-// are waited for in order behind them.
+// us for xq 8192 x 4096, W 14336 x 4096: 247 to 254 E2M1 (3.8 PFLOP/s; each further 4096 columns:
+// 193, 5.0), 371 to 384 E4M3 (2.5); without the stores 222 (of 254) and 349 (of 371): they come from all CUs at
+// once, 128 KiB a tile, and loads are waited for in order behind them.
 // The exponent bytes are laid out by K tile first ([K tile][row][BK / 32], zero past the matrix; one
 // small pass per operand), so a tile's are two DMAs a wave into a ring of three; a lane's exponents of
 // both 128-column steps are one 16-bit read (bytes 2 g + s for its block 4 s + g).
 // LDS rows are 16-byte chunks stored at chunk ^ f(row) (the XOR is applied to the global address),
 // f = row / 2 for 128-byte rows and -(row / 4) for 64-byte ones: a 128-bit read serves lanes 0-3, 12-15
 // and 20-27 together (then the others of 0-31), whose 16 chunks then fall on different banks
-// (SQ_LDS_BANK_CONFLICT 39 % -> 5 % of the LDS cycles against blocks 2 g + s, 266 -> 260 us).
+// (SQ_LDS_BANK_CONFLICT is 6 % of SQ_LDS_IDX_ACTIVE; blocks 2 g + s, which conflict, 266 us against 260).
 // Columns past K (K % BK != 0): chunks there are read from the row's first chunk of the tile, and
 // their exponents are 2^-127 on both sides, so what they add vanishes (below 2^-230).
 struct PpArgs {
@@ -1089,7 +1090,7 @@ __global__ __launch_bounds__(kPpThreads) void mx_pp_kernel(PpArgs p) {
 // DMA STAGES - 1 ahead, one barrier a K tile (a stage is refilled after the barrier behind its last
 // read).  Where there are still fewer tiles than CUs, K is cut into splits whose fp32 tiles a second
 // small kernel adds in order.  Exponents: [rows][stride], stride a multiple of 4, zero past K.
-// 48 x 28672 x 8192 E4M3: 43 us (2.9 TB/s of W); 1531 x 6151 x 1696: 46 us.
+// us: 48 x 28672 x 8192 E4M3 rows 43 (2.9 TB/s of W); 1531 x 6151 x 1696 E4M3 rows 37 to 46, E2M1 34.
 struct MidArgs {
   const uint8_t *x, *w, *xsc, *wsc;
   const float *xf;
@@ -1326,11 +1327,16 @@ template <int NB> __global__ __launch_bounds__(256) void mx_tile_scales_kernel(T
   }
 }
 
-// rows up to which the weight-streaming kernel is taken
-constexpr int kSkinnyRows = 16;  // one 16-row operand
+// Rows up to which the weight-streaming kernel is taken: one 16-row operand, since each further one reads W again.
+// us for rows handed over quantised, streaming / tiles:
+//   16 rows  4096 x 4096 E4M3 5.7 / 10.3, E2M1 4.9 / 8.1; 28672 x 8192 E4M3 34 / 39; 14336 x 4096 E2M1 9.3 / 9.4
+//   17 rows  7.3 / 10.4, 6.1 / 8.2; 53 / 40; 13.6 / 9.8        48 rows  11.7 / 12.5, 9.1 / 9.1; 82 / 43; 19.8 / 10.1
+// (a small W, which the caches hold, would gain from more rows)
+constexpr int kSkinnyRows = 16;
 // MXFP4 rows of at most 8 tokens against at most 16 MiB of W: quantised by every workgroup for itself, in
 // registers (kOpFused); else once, by a launch of its own.  us, fused / in two launches:
-// 4096 x 4096: 1 row 6.0 / 7.6, 8 rows 6.9 / 7.2, 16 rows 8.1 / 7.4; 14336 x 4096: 1 row 11.9 / 10.1
+// 1024 x 4096: 1 row 5.4 / 7.4; 4096 x 4096: 1 row 6.1 / 7.4, 8 rows 6.9 / 7.2, 16 rows 8.0 / 7.7; 8192 x 4096: 1 row
+// 8.5 / 7.9, 8 rows 10.4 / 8.7
 constexpr int kFusedRows = 8;
 constexpr int64_t kFusedWeights = 1 << 25;
 
@@ -1358,8 +1364,16 @@ LinearPlan linear_plan(int64_t M, int64_t N, int64_t K, int kind) {
     return p;
   }
   p.form = LinearPlan::kMid;
+  // The smaller tiles where the larger ones leave CUs idle.  us, 128 / 64 rows: 1024 x 8192 x 4096 (512 tiles of 128 x 128)
+  // E2M1 rows 30 / 42, E4M3 46 / 63; 512 x 8192 x 4096 (256) 20.1 / 20.9, 32.5 / 31.4; 512 x 4096 x 4096 (128) 25 / 13, 26 / 18;
+  // but 128 x 28672 x 8192 (224) 46 / 55, 61 / 68.  128 / 64 columns of 64 rows: 64 x 28672 x 8192 (224 tiles of 128) 36 / 44,
+  // 44 / 52; 512 x 4096 x 4096 (256) 13.0 / 13.7, 18.0 / 19.4; 64 x 14336 x 4096 (112) 17.9 / 11.0, 24 / 14.
   p.bm = M > 64 && tiles(128, 128) >= cus ? 128 : 64;
   p.bn = p.bm == 128 || tiles(64, 128) * 4 >= cus * 3 ? 128 : 64;
+  // K is split where fewer than three quarters of the CUs have a tile.  us, split / whole: 64 x 4096 x 14336 E4M3
+  // 19.5 / 39, 128 x 4096 x 14336 E2M1 21.8 / 27.7, 32 x 4096 x 4096 E4M3 11.1 / 11.6 (but 64 rows 13.8 / 11.6, 128 rows
+  // 14.7 / 11.7); with more tiles than that: 256 x 4096 x 4096 E4M3 18.2 / 12.0, 64 x 14336 x 4096 20.8 / 14.2, 48 x
+  // 28672 x 8192 48.8 / 42.9.
   const int bk = pp_bk(kind != MTQ_MXFP4);
   const int64_t nt = (K + bk - 1) / bk, have = tiles(p.bm, p.bn);
   int64_t splits = have * 4 >= 3 * cus ? 1 : (2 * cus + have - 1) / have;

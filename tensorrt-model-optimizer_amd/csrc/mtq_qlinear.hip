@@ -24,8 +24,8 @@
 // buffer, late vmcnt: the guide's GEMV recipe).  Loads go through a buffer descriptor over the
 // wave's 16 rows (32-bit lane offsets, scalar step offsets: no VALU address arithmetic).  x rows
 // >= M are not zero-filled: lanes of such rows re-read row M-1, and the MFMA output rows they
-// feed are never stored.  qdq runs on fp32 pairs (v_pk_mul/v_pk_fma, v_maximum3/v_minimum3
-// NaN-propagating clamps, v_cvt_pk_bf16_f32), ~6.5 VALU per weight for INT-n, ~5.5 for FP8.
+// feed are never stored.  qdq: div_rn, v_maximum3/v_minimum3 NaN-propagating clamps,
+// v_cvt_pk_bf16_f32 per pair (no packed fp32 instructions).
 // S > 1 writes fp32 partial tiles to a workspace and qlinear_splitk_finish sums them in chunk
 // order (deterministic), adds the bias in fp32 and rounds once.
 //

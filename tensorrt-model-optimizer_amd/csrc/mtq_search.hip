@@ -14,7 +14,7 @@
 //    (per-channel / static-block amax) or per-tensor losses through deterministic partials.
 //  * AWQ-clip (model_calib.py:1800-1882): a lane per (output row, clip variant) holds its
 //    quantised weight block in VGPRs; the sampled activations are wave-uniform and arrive as
-//    scalar loads (SGPR operands of v_pk_mul_f32); bf16/f16 products are rounded to the
+//    scalar loads (SGPR operands of the products); bf16/f16 products are rounded to the
 //    element type (v_cvt_pk_bf16_f32) and summed with v_dot2c_f32_bf16 against (1, 1), as the
 //    reference's ``(inputs * w).sum(-1)`` rounds each product to the dtype.  The original-weight
 //    dot product (variant 0) is shared with the clip variants of the same row by ds_bpermute.
