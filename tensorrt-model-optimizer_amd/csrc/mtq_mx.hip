@@ -1333,12 +1333,12 @@ template <int NB> __global__ __launch_bounds__(256) void mx_tile_scales_kernel(T
 //   17 rows  7.3 / 10.4, 6.1 / 8.2; 53 / 40; 13.6 / 9.8        48 rows  11.7 / 12.5, 9.1 / 9.1; 82 / 43; 19.8 / 10.1
 // (a small W, which the caches hold, would gain from more rows)
 constexpr int kSkinnyRows = 16;
-// MXFP4 rows of at most 8 tokens against at most 16 MiB of W: quantised by every workgroup for itself, in
+// MXFP4 rows of at most 8 tokens against at most 8 MiB of W: quantised by every workgroup for itself, in
 // registers (kOpFused); else once, by a launch of its own.  us, fused / in two launches:
 // 1024 x 4096: 1 row 5.4 / 7.4; 4096 x 4096: 1 row 6.1 / 7.4, 8 rows 6.9 / 7.2, 16 rows 8.0 / 7.7; 8192 x 4096: 1 row
 // 8.5 / 7.9, 8 rows 10.4 / 8.7
 constexpr int kFusedRows = 8;
-constexpr int64_t kFusedWeights = 1 << 25;
+constexpr int64_t kFusedWeights = 1 << 24;
 
 // which kernel, and its tile
 struct LinearPlan {
