@@ -948,8 +948,9 @@ struct Plan {
 };
 // Rows of a KV head from which the prompt kernel is taken.  us, prompt / decode kernel, 32 / 8 heads of 128 (4 rows a
 // token): 1 sequence of 8192 keys, 64 rows 29 / 22, 96 30 / 27, 128 32 / 30, 256 41 / 40, 512 46 / 58; 8 of them, 64 rows
-// 78 / 53, 96 83 / 76, 128 86 / 97, 256 99 / 159; 64 of 2048 keys, 64 rows 142 / 73, 128 144 / 139.  (Contexts of a few
-// hundred keys, which the prompt kernel does not split, would gain from more: 2 of 500 keys, 128 rows 24 / 10.)
+// 78 / 53, 96 83 / 76, 128 86 / 97, 256 99 / 159; 64 of 2048 keys, 64 rows 142 / 73, 128 144 / 139.  Few workgroups
+// on short contexts would gain from more rows: 1 prompt of 128 tokens alone 15 / 7, of 512 27 / 20, of 1024 71 / 45; 4 of 128
+// 16 / 12, but of 256 21 / 26, and 16 of 64 15 / 20.
 constexpr int kPromptRows = 128;
 
 // the rows of a KV head that a call has room for (ints in the kernels)
