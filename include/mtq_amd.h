@@ -470,7 +470,8 @@ int mtq_attention_fwd(const void *q, const void *k, const void *v, void *o,
  *   MTQ_FP8_TENSOR  q[row][K] E4M3; scale[1] fp32 factor (value = q * factor)
  *   MTQ_FP8_TOKEN   q[row][K] E4M3; scale[row] fp32 factors
  * Values: the MX kinds as mtq_fused_amax_convert (E8M0 scales, block 32), FP8_TENSOR as
- * mtq_fake_e4m3fy with the fp32 amax[0]; FP8_TOKEN: factor = max|x| / 448 (1 for a row of zeros). */
+ * mtq_fake_e4m3fy with the fp32 amax[0]; FP8_TOKEN: factor = max|x| / 448 (1 where that is 0), q =
+ * e4m3(x / factor). */
 enum mtq_row_kind { MTQ_MXFP4 = 0, MTQ_MXFP8 = 1, MTQ_FP8_TENSOR = 2, MTQ_FP8_TOKEN = 3 };
 
 /* Rows x[rows][cols] (row stride in elements; bf16 / f16 / f32) to q and scale; cols % 32 == 0 for
@@ -479,7 +480,8 @@ int mtq_mx_quantize(const void *x, int64_t row_stride, int64_t rows, int64_t col
                     int kind, const float *amax, uint8_t *q, void *scale, hipStream_t stream);
 
 /* h = x + residual (rounded to dtype; h may be the residual itself), y = h * rsqrt(mean(h^2) + eps)
- * * weight in fp32, quantised to q / scale as above without rounding y in between.  residual NULL:
+ * * weight in fp32, quantised to q / scale as above without rounding y in between (FP8_TOKEN: q =
+ * e4m3 of h weight over its maximum's 448th, before the root, which cancels).  residual NULL:
  * h = x and no h is written.  weight: dtype or fp32.  cols <= 65536. */
 int mtq_rms_norm_quantize(const void *x, int64_t x_stride, const void *residual, int64_t r_stride,
                           const void *weight, int weight_dtype, double eps, void *h, uint8_t *q,
@@ -517,8 +519,8 @@ typedef struct {
  * [rows][heads][head_dim] tensors k and v (element strides: k token, k head, v token, v head), into
  * / out of the pages block_table[b * table_stride + position / page_size].  Positions without a page
  * (an entry outside 0 .. num_pages - 1, a position past the table) are dropped / read as zeros;
- * other rows are not touched, nor are a sequence's tokens from max_len on.  A page that a call writes must
- * belong to one sequence. */
+ * other rows are not touched, nor are a sequence's tokens from max_len on.  A page that a call
+ * writes must belong to one sequence. */
 int mtq_kv_append(const mtq_kv_cache *cache, const void *k, const void *v, const int64_t *strides,
                   int64_t rows, const int32_t *block_table, int64_t table_stride, int table_cols,
                   const int32_t *b_start_loc, const int32_t *b_seq_len, const int32_t *b_seq_len_k,
@@ -530,11 +532,11 @@ int mtq_kv_read(const mtq_kv_cache *cache, void *k, void *v, const int64_t *stri
 
 /* o = softmax(softmax_scale q k^T) v for the queries (rows b_start_loc[b] + i, i < b_seq_len[b], the
  * last positions of their sequence) over the cached keys; causal or not; keys without a page are not
- * seen, a row that sees no key is zero, rows of no sequence are not touched, nor are a sequence's rows
- * from max_len_q on.  q, o: [rows][heads]
- * [head_dim] bf16 / f16 (element strides q token, q head, o token, o head, multiples of 8),
- * 16-byte aligned.  max_len_k sizes the split over the keys (any value is correct).  ws:
- * mtq_kv_attention_workspace_bytes bytes, 16-byte aligned, contents overwritten. */
+ * seen, a row that sees no key is zero, rows of no sequence are not touched, nor are a sequence's
+ * rows from max_len_q on.  q, o: [rows][heads][head_dim] bf16 / f16 (element strides q token, q head,
+ * o token, o head, multiples of 8), 16-byte aligned.  max_len_k sizes the split over the keys (any
+ * value is correct).  softmax_scale > 0.  ws: mtq_kv_attention_workspace_bytes bytes of the same
+ * arguments, 16-byte aligned, contents overwritten. */
 size_t mtq_kv_attention_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim,
                                         int max_len_q, int max_len_k);
 int mtq_kv_attention(const mtq_kv_cache *cache, const void *q, void *o, const int64_t *strides,

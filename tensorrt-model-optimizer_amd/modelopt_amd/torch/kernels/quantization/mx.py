@@ -6,7 +6,7 @@ Formats of a row of K values (``format``):
 ``"mxfp4"``    ``uint8 [..., K / 2]`` E2M1 codes   ``uint8 [..., K / 32]`` E8M0 exponent bytes
 ``"mxfp8"``    ``float8_e4m3fn [..., K]``          ``uint8 [..., K / 32]`` E8M0 exponent bytes
 ``"fp8"``      ``float8_e4m3fn [..., K]``          ``float32 [1]`` factor (per tensor, from ``amax``)
-``"fp8_token"``  ``float8_e4m3fn [..., K]``        ``float32 [..., 1]`` factor per row
+``"fp8_token"``  ``float8_e4m3fn [..., K]``        ``float32 [..., 1]`` factor per row, ``max|x| / 448``
 =============  =================================  ==========================================
 
 The values are those of the quantizers' fake quant: ``"mxfp4"`` / ``"mxfp8"`` of the dynamic MX block
@@ -80,7 +80,7 @@ def mx_linear(
     ``x [..., K]`` in bf16 / fp16 / fp32 is quantised to ``format`` on the way (``amax`` as in
     ``mx_quantize``); with ``x_scale`` it is already quantised (``mx_quantize``'s or
     ``rms_norm_quantize``'s pair).  ``weight uint8 [N, K / 2]``, ``weight_scale uint8`` with ``N * K / 32``
-    entries; ``bias [N]`` in the output's dtype or fp32.  ``out_dtype``: default ``x.dtype``, bf16 for a
+    entries; at most ``2**24`` rows on either side and ``K`` at most ``2**22``; ``bias [N]`` in the output's dtype or fp32.  ``out_dtype``: default ``x.dtype``, bf16 for a
     quantised ``x``.
 
     Sums of an ``"mxfp4"`` ``x`` are off by fp32 rounding only.  E4M3 rows meet the matrix cores' fixed-point

@@ -23,7 +23,8 @@ def rms_norm_quantize(
 
     ``data`` / ``scale`` are ``y`` in ``format`` (as ``mx_quantize``, what ``mx_linear`` takes with
     ``x_scale``), quantised from the fp32 ``y`` -- the rounding of ``y`` to ``x.dtype`` that a norm which
-    stores it makes does not happen.  ``h`` is the new residual stream, rounded to ``x.dtype`` before the norm
+    stores it makes does not happen (``"fp8_token"``: from the quotients of ``h * weight`` and its maximum, in
+    which the root cancels).  ``h`` is the new residual stream, rounded to ``x.dtype`` before the norm
     reads it, as a layer that stores it has it; ``None`` without ``residual``.  ``x [..., H]`` bf16, fp16 or
     fp32, ``H`` at most 65536 and a multiple of 32 for the MX formats; ``weight [H]`` in that dtype or fp32."""
     kind = format_code(format)
